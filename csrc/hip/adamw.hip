@@ -1,0 +1,486 @@
+// AdamW over many tensors in one launch, and the norm of many gradients.
+//
+//   c = min(1, max_norm / (|g| + 1e-6))          (1 without a norm)
+//   m = b1 m + (1 - b1) (c g)
+//   v = b2 v + (1 - b2) (c g)^2
+//   p = p (1 - lr wd) - lr / bc1 * m / (sqrt(v) / sqrt(bc2) + eps)
+//
+// All of it in fp32 with every product and sum rounded by itself (no
+// contraction), so that a plain elementwise program gets the same bits; the
+// scalars are formed in double on the host.
+//
+// 8-bit states: 256 consecutive values of a tensor share a power of two
+// 2^(E-127), the exponent of the largest magnitude among them, kept as one
+// byte. A value is its ratio to that power with 3 bits of mantissa:
+//   first moment   sign, 4 bits of exponent: 1.875 .. 2^-14, steps of 2^-17
+//                  below
+//   second moment  5 bits of exponent: 1.875 .. 2^-30, steps of 2^-33 below;
+//                  a value above zero never gets the code of zero, because a
+//                  zero in the denominator would blow the update up, while a
+//                  value held too large only makes it smaller
+// Rounding is to nearest even; a ratio above 1.875 (up to 2) takes the top
+// code, no further off than half a step. With a power of two as the scale
+// the ratio is exact, and so is the held value in bf16. E = 255 (an infinity
+// or NaN among the values) stands for NaN in the whole block.
+//
+// Memory bound: 28 bytes a value with fp32 states and parameters, 16 with
+// 8-bit states, some 60 and 120 vector instructions. One thread holds 4
+// consecutive values (16-byte accesses; with 8-bit states a wave is exactly
+// one block of 256, whose maximum is a wave reduction).
+#include <hip/hip_runtime.h>
+
+#include "train_ops.h"
+#include "typed.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kValues = 4;                       // consecutive, per thread
+constexpr int kPass = kThreads * kValues;        // values of one pass
+constexpr int kPasses = 4;
+constexpr int kChunk = kPass * kPasses;          // values of one workgroup
+constexpr int kBlock8 = 256;                     // values sharing a scale
+static_assert(kPass % kBlock8 == 0 && kBlock8 == 64 * kValues,
+              "a wave holds one block of an 8-bit state");
+
+// Pointers travel as kernel arguments (below 4 KB), so a launch needs no
+// copy to the device and can be captured.
+constexpr int kTensors32 = 88, kTensors8 = 62, kTensorsNorm = 180;
+
+template <int N>
+struct Table32 {
+  void* p[N];
+  const void* g[N];
+  void* m[N];
+  void* v[N];
+  long n[N];
+  int first[N];     // first workgroup of the tensor
+  int count;
+};
+
+template <int N>
+struct Table8 : Table32<N> {
+  unsigned char* ms[N];
+  unsigned char* vs[N];
+};
+
+struct TableNorm {
+  const void* g[kTensorsNorm];
+  long n[kTensorsNorm];
+  int first[kTensorsNorm];
+  int count;
+};
+
+// The last tensor whose first workgroup is not above `wg`.
+template <typename Table>
+__device__ inline int find_tensor(const Table& t, int wg) {
+  int lo = 0, hi = t.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (t.first[mid] <= wg) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+struct Hyper {
+  float beta1, one_minus_beta1, beta2, one_minus_beta2;
+  float eps, decay, rate, inv_bc2, max_norm;
+  const float* norm;       // null: no clipping
+};
+
+__device__ inline float clip_factor(const Hyper& h) {
+  if (h.norm == nullptr) return 1.0f;
+  const float c = h.max_norm / (*h.norm + 1e-6f);
+  return c > 1.0f ? 1.0f : c;                    // NaN stays NaN
+}
+
+__device__ inline void update(const Hyper& h, float c, float g, float& p,
+                              float& m, float& v) {
+#pragma clang fp contract(off)
+  g = g * c;
+  m = m * h.beta1 + g * h.one_minus_beta1;
+  v = v * h.beta2 + (g * g) * h.one_minus_beta2;
+  const float step = m / (sqrtf(v) * h.inv_bc2 + h.eps);
+  p = p * h.decay - step * h.rate;
+}
+
+template <typename T>
+__device__ inline void load4(const T* p, long left, bool wide,
+                             float (&out)[kValues]) {
+  if (wide && left >= kValues) {
+    load_f32<T, kValues>(p, out);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kValues; ++i)
+      out[i] = i < left ? static_cast<float>(p[i]) : 0.0f;
+  }
+}
+
+template <typename T>
+__device__ inline void store4(T* p, long left, bool wide,
+                              const float (&in)[kValues]) {
+  if (wide && left >= kValues) {
+    store_f32<T, kValues>(p, in);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kValues; ++i)
+      if (i < left) p[i] = static_cast<T>(in[i]);
+  }
+}
+
+__device__ inline bool aligned16(const void* a, const void* b, const void* c,
+                                 const void* d) {
+  return (((unsigned long)a | (unsigned long)b | (unsigned long)c |
+           (unsigned long)d) & 15) == 0;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void adamw32_kernel(
+    Table32<kTensors32> t, Hyper h) {
+  const int k = find_tensor(t, blockIdx.x);
+  const long at = (long)(blockIdx.x - t.first[k]) * kChunk +
+                  threadIdx.x * kValues;
+  const long n = t.n[k];
+  T* p = static_cast<T*>(t.p[k]);
+  const T* g = static_cast<const T*>(t.g[k]);
+  float* m = static_cast<float*>(t.m[k]);
+  float* v = static_cast<float*>(t.v[k]);
+  const bool wide = aligned16(p, g, m, v);
+  const float c = clip_factor(h);
+  for (int pass = 0; pass < kPasses; ++pass) {
+    const long i = at + (long)pass * kPass, left = n - i;
+    if (left <= 0) return;
+    float pf[kValues], gf[kValues], mf[kValues], vf[kValues];
+    load4(p + i, left, wide, pf);
+    load4(g + i, left, wide, gf);
+    load4(m + i, left, wide, mf);
+    load4(v + i, left, wide, vf);
+#pragma unroll
+    for (int j = 0; j < kValues; ++j) update(h, c, gf[j], pf[j], mf[j], vf[j]);
+    store4(p + i, left, wide, pf);
+    store4(m + i, left, wide, mf);
+    store4(v + i, left, wide, vf);
+  }
+}
+
+// ---------------------------------------------------------- 8-bit states
+
+__device__ inline float pow2_biased(int e) {     // 2^(e - 127), 1 <= e <= 254
+  return __int_as_float(e << 23);
+}
+
+// kLow: the exponent of the smallest normal code is -kLow.
+template <bool kSigned> struct Code8;
+template <> struct Code8<true> { static constexpr int low = 14, top = 127; };
+template <> struct Code8<false> { static constexpr int low = 30, top = 255; };
+
+constexpr int kMinExp = 40;  // keeps 2^(E-127) and every step a normal fp32
+
+template <bool kSigned>
+__device__ inline float decode8(unsigned code, int e) {
+  constexpr int low = Code8<kSigned>::low;
+  const unsigned mag = kSigned ? code & 127u : code;
+  float r = mag >= 8 ? __int_as_float((mag + ((126 - low) << 3)) << 20)
+                     : (float)mag * pow2_biased(127 - low - 3);
+  if (kSigned && code > 127) r = -r;
+  return e == 255 ? __int_as_float(0x7fc00000) : r * pow2_biased(e);
+}
+
+// `inv` = 2^(127 - E).
+template <bool kSigned>
+__device__ inline unsigned encode8(float x, float inv) {
+  constexpr int low = Code8<kSigned>::low;
+  const float r = fabsf(x) * inv;
+  const int b = __float_as_int(r);
+  int code;
+  if (r >= pow2_biased(127 - low)) {
+    code = ((b + 0x7ffff + ((b >> 20) & 1)) >> 20) - ((126 - low) << 3);
+    code = code > Code8<kSigned>::top ? Code8<kSigned>::top : code;
+  } else {
+    code = (int)rintf(r * pow2_biased(127 + low + 3));
+    if (!kSigned && x > 0.0f && code == 0) code = 1;
+  }
+  if (kSigned && __float_as_int(x) < 0) code |= 128;
+  return (unsigned)code & 255u;
+}
+
+// The block's biased exponent from the largest magnitude's bits: as an
+// unsigned maximum it lets infinities and NaN win.
+__device__ inline int block_exponent(const float (&x)[kValues]) {
+  unsigned top = 0;
+#pragma unroll
+  for (int j = 0; j < kValues; ++j) {
+    const unsigned b = __float_as_uint(x[j]) & 0x7fffffffu;
+    top = b > top ? b : top;
+  }
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) {
+    const unsigned o = __shfl_xor(top, d, 64);
+    top = o > top ? o : top;
+  }
+  const int e = (int)(top >> 23);
+  return e < kMinExp ? kMinExp : e;
+}
+
+template <bool kSigned>
+__device__ inline void store_block8(unsigned char* codes, unsigned char* scale,
+                                    long left, bool wide,
+                                    const float (&x)[kValues]) {
+  const int e = block_exponent(x);
+  const float inv = e == 255 ? 0.0f : pow2_biased(254 - e);
+  unsigned c[kValues];
+#pragma unroll
+  for (int j = 0; j < kValues; ++j)
+    c[j] = e == 255 ? 0u : encode8<kSigned>(x[j], inv);
+  if (wide && left >= kValues) {
+    *reinterpret_cast<unsigned*>(codes) =
+        c[0] | (c[1] << 8) | (c[2] << 16) | (c[3] << 24);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kValues; ++j)
+      if (j < left) codes[j] = (unsigned char)c[j];
+  }
+  if ((threadIdx.x & 63) == 0 && left > 0) *scale = (unsigned char)e;
+}
+
+template <bool kSigned>
+__device__ inline void load_block8(const unsigned char* codes, int e,
+                                   long left, bool wide,
+                                   float (&x)[kValues]) {
+  unsigned c[kValues] = {};
+  if (wide && left >= kValues) {
+    const unsigned w = *reinterpret_cast<const unsigned*>(codes);
+#pragma unroll
+    for (int j = 0; j < kValues; ++j) c[j] = (w >> (8 * j)) & 255u;
+  } else {
+#pragma unroll
+    for (int j = 0; j < kValues; ++j) c[j] = j < left ? codes[j] : 0u;
+  }
+#pragma unroll
+  for (int j = 0; j < kValues; ++j)
+    x[j] = j < left ? decode8<kSigned>(c[j], e) : 0.0f;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void adamw8_kernel(
+    Table8<kTensors8> t, Hyper h) {
+  const int k = find_tensor(t, blockIdx.x);
+  const long at = (long)(blockIdx.x - t.first[k]) * kChunk +
+                  threadIdx.x * kValues;
+  const long n = t.n[k];
+  T* p = static_cast<T*>(t.p[k]);
+  const T* g = static_cast<const T*>(t.g[k]);
+  unsigned char* m = static_cast<unsigned char*>(t.m[k]);
+  unsigned char* v = static_cast<unsigned char*>(t.v[k]);
+  const bool wide = aligned16(p, g, m, v);
+  const float c = clip_factor(h);
+  for (int pass = 0; pass < kPasses; ++pass) {
+    const long i = at + (long)pass * kPass, left = n - i;
+    const long b = i / kBlock8;
+    if (b * kBlock8 >= n) return;    // the whole wave is past the end
+    float pf[kValues], gf[kValues], mf[kValues], vf[kValues];
+    load4(p + i, left, wide, pf);
+    load4(g + i, left, wide, gf);
+    load_block8<true>(m + i, t.ms[k][b], left, wide, mf);
+    load_block8<false>(v + i, t.vs[k][b], left, wide, vf);
+#pragma unroll
+    for (int j = 0; j < kValues; ++j) {
+      update(h, c, gf[j], pf[j], mf[j], vf[j]);
+      if (j >= left) mf[j] = vf[j] = 0.0f;   // no part in the maximum
+    }
+    store4(p + i, left, wide, pf);
+    store_block8<true>(m + i, t.ms[k] + b, left, wide, mf);
+    store_block8<false>(v + i, t.vs[k] + b, left, wide, vf);
+  }
+}
+
+// ------------------------------------------------- packing and unpacking
+
+template <bool kSigned>
+__global__ __launch_bounds__(kThreads) void pack8_kernel(
+    const float* x, unsigned char* codes, unsigned char* scales, long n) {
+  const long i = ((long)blockIdx.x * kThreads + threadIdx.x) * kValues;
+  const long b = i / kBlock8, left = n - i;
+  if (b * kBlock8 >= n) return;
+  const bool wide = aligned16(x, codes, nullptr, nullptr);
+  float f[kValues];
+  load4(x + i, left, wide, f);
+  store_block8<kSigned>(codes + i, scales + b, left, wide, f);
+}
+
+template <bool kSigned, typename T>
+__global__ __launch_bounds__(kThreads) void unpack8_kernel(
+    const unsigned char* codes, const unsigned char* scales, T* out, long n) {
+  const long i = ((long)blockIdx.x * kThreads + threadIdx.x) * kValues;
+  const long left = n - i;
+  if (left <= 0) return;
+  const bool wide = aligned16(codes, out, nullptr, nullptr);
+  float f[kValues];
+  load_block8<kSigned>(codes + i, scales[i / kBlock8], left, wide, f);
+  store4(out + i, left, wide, f);
+}
+
+// ------------------------------------------------------------------ norm
+
+// Squares are summed in double: memory bound all the same, and the result
+// does not depend on the order to any bit of the fp32 norm that matters.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void square_sum_kernel(
+    TableNorm t, double* partial) {
+  const int k = find_tensor(t, blockIdx.x);
+  const long at = (long)(blockIdx.x - t.first[k]) * kChunk +
+                  threadIdx.x * kValues;
+  const T* g = static_cast<const T*>(t.g[k]);
+  const bool wide = ((unsigned long)g & 15) == 0;
+  double s = 0.0;
+  for (int pass = 0; pass < kPasses; ++pass) {
+    const long i = at + (long)pass * kPass, left = t.n[k] - i;
+    if (left <= 0) break;
+    float f[kValues];
+    load4(g + i, left, wide, f);
+#pragma unroll
+    for (int j = 0; j < kValues; ++j) s += (double)f[j] * (double)f[j];
+  }
+  for (int d = 32; d >= 1; d >>= 1) s += __shfl_xor(s, d, 64);
+  __shared__ double waves[kThreads / 64];
+  if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kThreads / 64; ++w) s += waves[w];
+    partial[blockIdx.x] = s;
+  }
+}
+
+__global__ __launch_bounds__(1024) void norm_kernel(const double* partial,
+                                                    int count, float* out) {
+  double s = 0.0;
+  for (int i = threadIdx.x; i < count; i += 1024) s += partial[i];
+  for (int d = 32; d >= 1; d >>= 1) s += __shfl_xor(s, d, 64);
+  __shared__ double waves[16];
+  if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 16; ++w) s += waves[w];
+    *out = (float)sqrt(s);
+  }
+}
+
+int chunks(long n) { return (int)((n + kChunk - 1) / kChunk); }
+
+}  // namespace
+
+template <typename Table>
+static int fill(Table& t, const AdamWTensors& a, int from, int most) {
+  int wg = 0;
+  t.count = 0;
+  for (int i = from; i < a.count && t.count < most; ++i) {
+    const int k = t.count++;
+    t.p[k] = a.p[i];
+    t.g[k] = a.g[i];
+    t.m[k] = a.m[i];
+    t.v[k] = a.v[i];
+    t.n[k] = a.n[i];
+    t.first[k] = wg;
+    wg += chunks(a.n[i]);
+  }
+  return wg;
+}
+
+extern "C" hipError_t adamw_launch(const AdamWTensors* a,
+                                   const AdamWScalars* s, int type,
+                                   hipStream_t stream) {
+  const Hyper h{s->beta1, s->one_minus_beta1, s->beta2, s->one_minus_beta2,
+                s->eps, s->decay, s->rate, s->inv_bc2, s->max_norm, s->norm};
+  for (int from = 0; from < a->count;) {
+    if (a->ms == nullptr) {
+      Table32<kTensors32> t;
+      const int wg = fill(t, *a, from, kTensors32);
+      from += t.count;
+      switch (type) {
+        case kElemF32: adamw32_kernel<float><<<wg, kThreads, 0, stream>>>(t, h); break;
+        case kElemBF16: adamw32_kernel<bf16_t><<<wg, kThreads, 0, stream>>>(t, h); break;
+        default: adamw32_kernel<fp16_t><<<wg, kThreads, 0, stream>>>(t, h);
+      }
+    } else {
+      Table8<kTensors8> t;
+      const int wg = fill(t, *a, from, kTensors8);
+      for (int k = 0; k < t.count; ++k) {
+        t.ms[k] = a->ms[from + k];
+        t.vs[k] = a->vs[from + k];
+      }
+      from += t.count;
+      switch (type) {
+        case kElemF32: adamw8_kernel<float><<<wg, kThreads, 0, stream>>>(t, h); break;
+        case kElemBF16: adamw8_kernel<bf16_t><<<wg, kThreads, 0, stream>>>(t, h); break;
+        default: adamw8_kernel<fp16_t><<<wg, kThreads, 0, stream>>>(t, h);
+      }
+    }
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+extern "C" int adamw_chunk() { return kChunk; }
+
+extern "C" hipError_t square_sum_launch(const void* const* g, const long* n,
+                                        int count, int type, double* partial,
+                                        hipStream_t stream) {
+  for (int from = 0; from < count;) {
+    TableNorm t;
+    int wg = 0;
+    for (t.count = 0; from < count && t.count < kTensorsNorm; ++from) {
+      const int k = t.count++;
+      t.g[k] = g[from];
+      t.n[k] = n[from];
+      t.first[k] = wg;
+      wg += chunks(n[from]);
+    }
+    switch (type) {
+      case kElemF32: square_sum_kernel<float><<<wg, kThreads, 0, stream>>>(t, partial); break;
+      case kElemBF16: square_sum_kernel<bf16_t><<<wg, kThreads, 0, stream>>>(t, partial); break;
+      default: square_sum_kernel<fp16_t><<<wg, kThreads, 0, stream>>>(t, partial);
+    }
+    partial += wg;
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+extern "C" hipError_t norm_launch(const double* partial, int count, float* out,
+                                  hipStream_t stream) {
+  norm_kernel<<<1, 1024, 0, stream>>>(partial, count, out);
+  return hipGetLastError();
+}
+
+extern "C" hipError_t pack8_launch(const float* x, unsigned char* codes,
+                                   unsigned char* scales, long n,
+                                   bool is_signed, hipStream_t stream) {
+  const unsigned wg = (unsigned)((n + kPass - 1) / kPass);
+  if (is_signed)
+    pack8_kernel<true><<<wg, kThreads, 0, stream>>>(x, codes, scales, n);
+  else
+    pack8_kernel<false><<<wg, kThreads, 0, stream>>>(x, codes, scales, n);
+  return hipGetLastError();
+}
+
+template <bool kSigned>
+static void unpack8(const unsigned char* codes, const unsigned char* scales,
+                    void* out, long n, int type, hipStream_t stream) {
+  const unsigned wg = (unsigned)((n + kPass - 1) / kPass);
+  switch (type) {
+    case kElemF32: unpack8_kernel<kSigned, float><<<wg, kThreads, 0, stream>>>(codes, scales, (float*)out, n); break;
+    case kElemBF16: unpack8_kernel<kSigned, bf16_t><<<wg, kThreads, 0, stream>>>(codes, scales, (bf16_t*)out, n); break;
+    default: unpack8_kernel<kSigned, fp16_t><<<wg, kThreads, 0, stream>>>(codes, scales, (fp16_t*)out, n);
+  }
+}
+
+extern "C" hipError_t unpack8_launch(const unsigned char* codes,
+                                     const unsigned char* scales, void* out,
+                                     long n, bool is_signed, int type,
+                                     hipStream_t stream) {
+  if (is_signed) unpack8<true>(codes, scales, out, n, type, stream);
+  else unpack8<false>(codes, scales, out, n, type, stream);
+  return hipGetLastError();
+}

@@ -1,0 +1,450 @@
+// Layer norm over the last dimension: forward, and the backward with the
+// reduction of the weight's and bias's gradients.
+//
+//   mu = mean(x)   var = mean((x - mu)^2)   r = 1 / sqrt(var + eps)
+//   xh = (x - mu) r           y = xh w + b
+//   d = dy w       dx = r (d - mean(d) - xh mean(d xh))
+//   dw = sum over rows of dy xh       db = sum over rows of dy
+//
+// Memory bound: x (and dy) are read once and stay in registers between the
+// statistics and the result; the variance is taken from the differences to
+// the mean, in fp32. A row belongs to a team of kTeam lanes (a part of a
+// wave up to 64, a workgroup above), each holding kVecs packets of kWidth
+// consecutive values (16 bytes where rows are aligned for it, else 1 value).
+// In the backward each lane also keeps its columns' sums of dy xh and dy
+// over all rows it sees; they leave once per workgroup as one row of
+// partial sums and a second launch adds the rows up in a fixed order, so
+// the gradients do not change from run to run.
+#include <hip/hip_runtime.h>
+
+#include "train_ops.h"
+#include "typed.h"
+
+namespace {
+
+// Sum over a team: within a wave by exchange, across waves through LDS.
+// `lds` holds two floats a wave; the caller keeps calls apart with `slot`.
+template <int kTeam>
+__device__ inline float team_sum(float s, float* lds) {
+  constexpr int in_wave = kTeam < 64 ? kTeam : 64;
+#pragma unroll
+  for (int d = in_wave / 2; d >= 1; d >>= 1) s += __shfl_xor(s, d, 64);
+  if constexpr (kTeam > 64) {
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s;
+    __syncthreads();
+    s = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kTeam / 64; ++w) s += lds[w];
+  }
+  return s;
+}
+
+template <int kTeam>
+__device__ inline void team_sum2(float& a, float& b, float* lds) {
+  constexpr int in_wave = kTeam < 64 ? kTeam : 64;
+#pragma unroll
+  for (int d = in_wave / 2; d >= 1; d >>= 1) {
+    a += __shfl_xor(a, d, 64);
+    b += __shfl_xor(b, d, 64);
+  }
+  if constexpr (kTeam > 64) {
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) {
+      lds[threadIdx.x >> 6] = a;
+      lds[16 + (threadIdx.x >> 6)] = b;
+    }
+    __syncthreads();
+    a = b = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kTeam / 64; ++w) {
+      a += lds[w];
+      b += lds[16 + w];
+    }
+  }
+}
+
+template <int kTeam>
+constexpr int threads_of() { return kTeam < 256 ? 256 : kTeam; }
+
+// T: x and y; W: weight and bias (null: 1 and 0).
+template <typename T, typename W, int kTeam, int kVecs, int kWidth>
+__global__ __launch_bounds__(threads_of<kTeam>()) void norm_fwd_kernel(
+    const T* x, const W* w, const W* b, T* y, float* mean, float* rstd,
+    long rows, int width, long x_stride, float eps) {
+  constexpr int kRows = threads_of<kTeam>() / kTeam;   // of one workgroup
+  __shared__ float lds[32];
+  const long row = (long)blockIdx.x * kRows + threadIdx.x / kTeam;
+  const int lane = threadIdx.x % kTeam;
+  if (row >= rows) return;    // a whole team; above 64 lanes never part of one
+  x += row * x_stride;
+  y += row * (long)width;
+  float v[kVecs][kWidth];
+  float s = 0.0f;
+#pragma unroll
+  for (int k = 0; k < kVecs; ++k) {
+    const int c = (k * kTeam + lane) * kWidth;
+    if (c < width) {
+      load_f32<T, kWidth>(x + c, v[k]);
+#pragma unroll
+      for (int i = 0; i < kWidth; ++i) s += v[k][i];
+    }
+  }
+  const float inv = 1.0f / (float)width;
+  const float mu = team_sum<kTeam>(s, lds) * inv;
+  s = 0.0f;
+#pragma unroll
+  for (int k = 0; k < kVecs; ++k) {
+    const int c = (k * kTeam + lane) * kWidth;
+    if (c < width) {
+#pragma unroll
+      for (int i = 0; i < kWidth; ++i) {
+        v[k][i] -= mu;
+        s += v[k][i] * v[k][i];
+      }
+    }
+  }
+  const float r = 1.0f / sqrtf(team_sum<kTeam>(s, lds) * inv + eps);
+#pragma unroll
+  for (int k = 0; k < kVecs; ++k) {
+    const int c = (k * kTeam + lane) * kWidth;
+    if (c < width) {
+      float wf[kWidth], bf[kWidth];
+#pragma unroll
+      for (int i = 0; i < kWidth; ++i) { wf[i] = 1.0f; bf[i] = 0.0f; }
+      if (w != nullptr) load_f32<W, kWidth>(w + c, wf);
+      if (b != nullptr) load_f32<W, kWidth>(b + c, bf);
+#pragma unroll
+      for (int i = 0; i < kWidth; ++i) v[k][i] = v[k][i] * r * wf[i] + bf[i];
+      store_f32<T, kWidth>(y + c, v[k]);
+    }
+  }
+  if (mean != nullptr && lane == 0) {
+    mean[row] = mu;
+    rstd[row] = r;
+  }
+}
+
+// `part`: gridDim.x rows of 2 * width sums (dy xh, then dy); null: no
+// weight gradients wanted. `dx` may be null too.
+template <typename T, typename W, int kTeam, int kVecs, int kWidth>
+__global__ __launch_bounds__(threads_of<kTeam>()) void norm_bwd_kernel(
+    const T* dy, const T* x, const W* w, const float* mean, const float* rstd,
+    T* dx, float* part, long rows, int width, long dy_stride, long x_stride) {
+  constexpr int kThreads = threads_of<kTeam>();
+  constexpr int kRows = kThreads / kTeam;
+  constexpr int kCols = kTeam * kVecs * kWidth;
+  __shared__ float lds[32];
+  __shared__ float sums[kRows > 1 ? 2 * kRows * kCols : 1];
+  const int lane = threadIdx.x % kTeam, team = threadIdx.x / kTeam;
+  float wf[kVecs][kWidth], dw[kVecs][kWidth], db[kVecs][kWidth];
+#pragma unroll
+  for (int k = 0; k < kVecs; ++k) {
+    const int c = (k * kTeam + lane) * kWidth;
+#pragma unroll
+    for (int i = 0; i < kWidth; ++i) {
+      wf[k][i] = 1.0f;
+      dw[k][i] = db[k][i] = 0.0f;
+    }
+    if (w != nullptr && c < width) load_f32<W, kWidth>(w + c, wf[k]);
+  }
+  const float inv = 1.0f / (float)width;
+  for (long row = (long)blockIdx.x * kRows + team; row < rows;
+       row += (long)gridDim.x * kRows) {
+    const float mu = mean[row], r = rstd[row];
+    const T* xr = x + row * x_stride;
+    const T* dyr = dy + row * dy_stride;
+    float d[kVecs][kWidth], xh[kVecs][kWidth];
+    float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kVecs; ++k) {
+      const int c = (k * kTeam + lane) * kWidth;
+      if (c < width) {
+        load_f32<T, kWidth>(xr + c, xh[k]);
+        load_f32<T, kWidth>(dyr + c, d[k]);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kVecs; ++k) {
+      const int c = (k * kTeam + lane) * kWidth;
+      if (c < width) {
+#pragma unroll
+        for (int i = 0; i < kWidth; ++i) {
+          xh[k][i] = (xh[k][i] - mu) * r;
+          dw[k][i] += d[k][i] * xh[k][i];
+          db[k][i] += d[k][i];
+          d[k][i] *= wf[k][i];
+          s1 += d[k][i];
+          s2 += d[k][i] * xh[k][i];
+        }
+      }
+    }
+    if (dx == nullptr) continue;
+    team_sum2<kTeam>(s1, s2, lds);
+    s1 *= inv;
+    s2 *= inv;
+    T* dxr = dx + row * (long)width;
+#pragma unroll
+    for (int k = 0; k < kVecs; ++k) {
+      const int c = (k * kTeam + lane) * kWidth;
+      if (c < width) {
+#pragma unroll
+        for (int i = 0; i < kWidth; ++i)
+          d[k][i] = r * (d[k][i] - s1 - xh[k][i] * s2);
+        store_f32<T, kWidth>(dxr + c, d[k]);
+      }
+    }
+  }
+  if (part == nullptr) return;
+  part += (long)blockIdx.x * 2 * width;
+  if constexpr (kRows == 1) {
+#pragma unroll
+    for (int k = 0; k < kVecs; ++k) {
+      const int c = (k * kTeam + lane) * kWidth;
+      if (c < width) {
+        store_f32<float, kWidth>(part + c, dw[k]);
+        store_f32<float, kWidth>(part + width + c, db[k]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < kVecs; ++k) {
+      const int c = (k * kTeam + lane) * kWidth;
+#pragma unroll
+      for (int i = 0; i < kWidth; ++i) {
+        sums[team * kCols + c + i] = dw[k][i];
+        sums[(kRows + team) * kCols + c + i] = db[k][i];
+      }
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < width; c += kThreads) {
+      float a = 0.0f, b = 0.0f;
+#pragma unroll
+      for (int t = 0; t < kRows; ++t) {
+        a += sums[t * kCols + c];
+        b += sums[(kRows + t) * kCols + c];
+      }
+      part[c] = a;
+      part[width + c] = b;
+    }
+  }
+}
+
+// ------------------------------------------- rows too wide for registers
+
+constexpr int kWide = 1024;   // threads of one row
+
+template <typename T, typename W>
+__global__ __launch_bounds__(kWide) void norm_fwd_wide_kernel(
+    const T* x, const W* w, const W* b, T* y, float* mean, float* rstd,
+    int width, long x_stride, float eps) {
+  __shared__ float lds[32];
+  const long row = blockIdx.x;
+  x += row * x_stride;
+  y += row * (long)width;
+  float s = 0.0f;
+  for (int c = threadIdx.x; c < width; c += kWide) s += (float)x[c];
+  const float mu = team_sum<kWide>(s, lds) / (float)width;
+  s = 0.0f;
+  for (int c = threadIdx.x; c < width; c += kWide) {
+    const float v = (float)x[c] - mu;
+    s += v * v;
+  }
+  const float r = 1.0f / sqrtf(team_sum<kWide>(s, lds) / (float)width + eps);
+  for (int c = threadIdx.x; c < width; c += kWide)
+    y[c] = (T)(((float)x[c] - mu) * r * (w ? (float)w[c] : 1.0f) +
+               (b ? (float)b[c] : 0.0f));
+  if (mean != nullptr && threadIdx.x == 0) {
+    mean[row] = mu;
+    rstd[row] = r;
+  }
+}
+
+template <typename T, typename W>
+__global__ __launch_bounds__(kWide) void norm_dx_wide_kernel(
+    const T* dy, const T* x, const W* w, const float* mean, const float* rstd,
+    T* dx, int width, long dy_stride, long x_stride) {
+  __shared__ float lds[32];
+  const long row = blockIdx.x;
+  const float mu = mean[row], r = rstd[row];
+  x += row * x_stride;
+  dy += row * dy_stride;
+  dx += row * (long)width;
+  float s1 = 0.0f, s2 = 0.0f;
+  for (int c = threadIdx.x; c < width; c += kWide) {
+    const float d = (float)dy[c] * (w ? (float)w[c] : 1.0f);
+    s1 += d;
+    s2 += d * (((float)x[c] - mu) * r);
+  }
+  team_sum2<kWide>(s1, s2, lds);
+  s1 /= (float)width;
+  s2 /= (float)width;
+  for (int c = threadIdx.x; c < width; c += kWide) {
+    const float d = (float)dy[c] * (w ? (float)w[c] : 1.0f);
+    dx[c] = (T)(r * (d - s1 - ((float)x[c] - mu) * r * s2));
+  }
+}
+
+// One column a thread, gridDim.y strips of rows.
+template <typename T>
+__global__ __launch_bounds__(256) void norm_dw_wide_kernel(
+    const T* dy, const T* x, const float* mean, const float* rstd,
+    float* part, long rows, int width, long dy_stride, long x_stride) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= width) return;
+  float a = 0.0f, b = 0.0f;
+  for (long row = blockIdx.y; row < rows; row += gridDim.y) {
+    const float d = (float)dy[row * dy_stride + c];
+    a += d * (((float)x[row * x_stride + c] - mean[row]) * rstd[row]);
+    b += d;
+  }
+  part += (long)blockIdx.y * 2 * width;
+  part[c] = a;
+  part[width + c] = b;
+}
+
+// --------------------------------------------------- partial sums' sum
+
+// part: `count` rows of `width` sums -> out[0:split] and out2[0:width-split]
+// (either may be null). A workgroup takes 32 columns, 8 strips of rows.
+template <typename W>
+__global__ __launch_bounds__(256) void sum_rows_kernel(
+    const float* part, int count, int width, int split, W* out, W* out2) {
+  __shared__ float lds[8][33];
+  const int col = blockIdx.x * 32 + (threadIdx.x & 31);
+  const int strip = threadIdx.x >> 5;
+  float s = 0.0f;
+  if (col < width)
+    for (int i = strip; i < count; i += 8) s += part[(long)i * width + col];
+  lds[strip][threadIdx.x & 31] = s;
+  __syncthreads();
+  if (strip == 0 && col < width) {
+    s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += lds[i][threadIdx.x];
+    if (col < split) {
+      if (out != nullptr) out[col] = (W)s;
+    } else if (out2 != nullptr) {
+      out2[col - split] = (W)s;
+    }
+  }
+}
+
+}  // namespace
+
+namespace {
+
+template <typename T, typename W, int kTeam, int kVecs, int kWidth>
+void run_team(const NormArgs& a, bool backward, hipStream_t s) {
+  constexpr int threads = threads_of<kTeam>(), per = threads / kTeam;
+  if (!backward) {
+    const unsigned grid = (unsigned)((a.rows + per - 1) / per);
+    norm_fwd_kernel<T, W, kTeam, kVecs, kWidth><<<grid, threads, 0, s>>>(
+        (const T*)a.x, (const W*)a.w, (const W*)a.b, (T*)a.y, a.mean, a.rstd,
+        a.rows, a.width, a.x_stride, a.eps);
+  } else {
+    norm_bwd_kernel<T, W, kTeam, kVecs, kWidth><<<a.parts, threads, 0, s>>>(
+        (const T*)a.dy, (const T*)a.x, (const W*)a.w, a.mean, a.rstd,
+        (T*)a.dx, a.part, a.rows, a.width, a.dy_stride, a.x_stride);
+  }
+}
+
+// Rows that one workgroup has in hand at a time.
+int rows_at_once(int packets) {
+  return packets <= 8 ? 32 : packets <= 16 ? 16 : packets <= 32 ? 8
+         : packets <= 128 ? 4 : 1;
+}
+
+// A team is as small as its row allows, with few packets a lane: the
+// exchange takes fewer steps and more rows are in flight.
+template <typename T, typename W, int kWidth>
+bool run_width(const NormArgs& a, bool backward, hipStream_t s) {
+  const int packets = (a.width + kWidth - 1) / kWidth;
+  if (packets <= 8) run_team<T, W, 8, 1, kWidth>(a, backward, s);
+  else if (packets <= 16) run_team<T, W, 16, 1, kWidth>(a, backward, s);
+  else if (packets <= 32) run_team<T, W, 32, 1, kWidth>(a, backward, s);
+  else if (packets <= 64) run_team<T, W, 64, 1, kWidth>(a, backward, s);
+  else if (packets <= 128) run_team<T, W, 64, 2, kWidth>(a, backward, s);
+  else if (packets <= 256) run_team<T, W, 256, 1, kWidth>(a, backward, s);
+  else if (packets <= 512) run_team<T, W, 256, 2, kWidth>(a, backward, s);
+  else if (packets <= 1024) run_team<T, W, 256, 4, kWidth>(a, backward, s);
+  else if (packets <= 2048) run_team<T, W, 512, 4, kWidth>(a, backward, s);
+  else if (packets <= 4096) {
+    // 1024 lanes have 128 registers each: the backward's four arrays of 32
+    // values do not fit, so such rows go to the wide kernels.
+    if constexpr (kWidth < 8) {
+      run_team<T, W, 1024, 4, kWidth>(a, backward, s);
+    } else {
+      return false;
+    }
+  } else {
+    return false;
+  }
+  return true;
+}
+
+template <typename T, typename W>
+void run_types(const NormArgs& a, bool backward, hipStream_t s) {
+  constexpr int full = 16 / sizeof(T);
+  if (a.aligned ? run_width<T, W, full>(a, backward, s)
+                : run_width<T, W, 1>(a, backward, s))
+    return;
+  if (!backward) {
+    norm_fwd_wide_kernel<T, W><<<(unsigned)a.rows, kWide, 0, s>>>(
+        (const T*)a.x, (const W*)a.w, (const W*)a.b, (T*)a.y, a.mean, a.rstd,
+        a.width, a.x_stride, a.eps);
+    return;
+  }
+  if (a.dx != nullptr)
+    norm_dx_wide_kernel<T, W><<<(unsigned)a.rows, kWide, 0, s>>>(
+        (const T*)a.dy, (const T*)a.x, (const W*)a.w, a.mean, a.rstd,
+        (T*)a.dx, a.width, a.dy_stride, a.x_stride);
+  if (a.part != nullptr)
+    norm_dw_wide_kernel<T>
+        <<<dim3((a.width + 255) / 256, a.parts), 256, 0, s>>>(
+            (const T*)a.dy, (const T*)a.x, a.mean, a.rstd, a.part, a.rows,
+            a.width, a.dy_stride, a.x_stride);
+}
+
+hipError_t run_norm(const NormArgs& a, int type, int wtype, bool backward,
+                    hipStream_t s) {
+  if (type == kElemF32) run_types<float, float>(a, backward, s);
+  else if (type == kElemBF16 && wtype == kElemF32) run_types<bf16_t, float>(a, backward, s);
+  else if (type == kElemBF16) run_types<bf16_t, bf16_t>(a, backward, s);
+  else if (wtype == kElemF32) run_types<fp16_t, float>(a, backward, s);
+  else run_types<fp16_t, fp16_t>(a, backward, s);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+// Rows of partial sums that the backward writes: a workgroup for each set of
+// rows up to four a CU, so that many rows share one row of sums.
+extern "C" int layer_norm_parts(long rows, int width, int type, bool aligned) {
+  const int per = aligned ? (type == kElemF32 ? 4 : 8) : 1;
+  const int at_once = rows_at_once((width + per - 1) / per);
+  const long sets = (rows + at_once - 1) / at_once;
+  return (int)(sets < 1024 ? sets : 1024);
+}
+
+extern "C" hipError_t layer_norm_fwd_launch(const NormArgs* a, int type,
+                                            int wtype, hipStream_t s) {
+  return run_norm(*a, type, wtype, false, s);
+}
+
+extern "C" hipError_t layer_norm_bwd_launch(const NormArgs* a, int type,
+                                            int wtype, hipStream_t s) {
+  return run_norm(*a, type, wtype, true, s);
+}
+
+extern "C" hipError_t sum_rows_launch(const float* part, int count, int width,
+                                      int split, void* out, void* out2,
+                                      int type, hipStream_t s) {
+  const unsigned grid = (unsigned)((width + 31) / 32);
+  switch (type) {
+    case kElemF32: sum_rows_kernel<float><<<grid, 256, 0, s>>>(part, count, width, split, (float*)out, (float*)out2); break;
+    case kElemBF16: sum_rows_kernel<bf16_t><<<grid, 256, 0, s>>>(part, count, width, split, (bf16_t*)out, (bf16_t*)out2); break;
+    default: sum_rows_kernel<fp16_t><<<grid, 256, 0, s>>>(part, count, width, split, (fp16_t*)out, (fp16_t*)out2);
+  }
+  return hipGetLastError();
+}

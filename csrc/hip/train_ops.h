@@ -1,0 +1,69 @@
+// Arguments and launchers of the training operators, shared by their
+// kernels (csrc/hip) and their bindings (csrc/train_ops.cpp).
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+// Host views of the tensors of one type; `ms` and `vs` are null with fp32
+// states.
+struct AdamWTensors {
+  int count;
+  void* const* p;
+  const void* const* g;
+  void* const* m;
+  void* const* v;
+  unsigned char* const* ms;
+  unsigned char* const* vs;
+  const long* n;
+};
+
+struct AdamWScalars {
+  float beta1, one_minus_beta1, beta2, one_minus_beta2;
+  float eps;
+  float decay;         // 1 - lr * weight_decay
+  float rate;          // lr / (1 - beta1^step)
+  float inv_bc2;       // 1 / sqrt(1 - beta2^step)
+  float max_norm;
+  const float* norm;   // null: no clipping
+};
+
+struct NormArgs {
+  const void *dy, *x, *w, *b;     // w, b: null for 1 and 0
+  void *y, *dx;
+  float *mean, *rstd;
+  float* part;         // `parts` rows of 2 * width sums
+  long rows, x_stride, dy_stride;
+  int width;
+  int parts;           // the backward's grid
+  bool aligned;        // rows of all operands begin at multiples of 16 bytes
+  float eps;
+};
+
+extern "C" {
+hipError_t adamw_launch(const AdamWTensors*, const AdamWScalars*, int type,
+                        hipStream_t);
+// Values that one workgroup of the step and of the norm takes.
+int adamw_chunk();
+// `partial` has a double for every chunk of every tensor.
+hipError_t square_sum_launch(const void* const* g, const long* n, int count,
+                             int type, double* partial, hipStream_t);
+hipError_t norm_launch(const double* partial, int count, float* out,
+                       hipStream_t);
+hipError_t pack8_launch(const float* x, unsigned char* codes,
+                        unsigned char* scales, long n, bool is_signed,
+                        hipStream_t);
+hipError_t unpack8_launch(const unsigned char* codes,
+                          const unsigned char* scales, void* out, long n,
+                          bool is_signed, int type, hipStream_t);
+
+// Rows of partial sums that the norm's backward writes.
+int layer_norm_parts(long rows, int width, int type, bool aligned);
+hipError_t layer_norm_fwd_launch(const NormArgs*, int type, int wtype,
+                                 hipStream_t);
+hipError_t layer_norm_bwd_launch(const NormArgs*, int type, int wtype,
+                                 hipStream_t);
+// `count` rows of `width` fp32 sums -> out[0:split], out2[0:width - split];
+// either may be null.
+hipError_t sum_rows_launch(const float* part, int count, int width, int split,
+                           void* out, void* out2, int type, hipStream_t);
+}

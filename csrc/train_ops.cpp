@@ -1,0 +1,396 @@
+// PyTorch bindings of the training operators: layer norm, the AdamW step
+// with the gradient norm, and packed 8-bit optimizer states.
+
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/extension.h>
+
+#include <algorithm>
+#include <cmath>
+#include <optional>
+#include <vector>
+
+#include "hip/train_ops.h"
+
+namespace {
+
+using torch::Tensor;
+using Tensors = std::vector<Tensor>;
+
+hipStream_t current() { return c10::hip::getCurrentHIPStream().stream(); }
+
+void launched(hipError_t e, const char* what) {
+  TORCH_CHECK(e == hipSuccess, what, ": ", hipGetErrorString(e));
+}
+
+int elem_type(const Tensor& t, const char* what) {
+  switch (t.scalar_type()) {
+    case torch::kFloat: return 0;
+    case torch::kBFloat16: return 1;
+    case torch::kHalf: return 2;
+    default:
+      TORCH_CHECK(false, what, ": float32, bfloat16 or float16, not ",
+                  t.scalar_type());
+  }
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// ------------------------------------------------------------ layer norm
+
+// x as rows of consecutive values; a copy only where its strides need one.
+Tensor as_rows(const Tensor& x, int64_t width) {
+  if (x.dim() == 2 && (x.stride(1) == 1 || width == 1) &&
+      (x.stride(0) >= width || x.stride(0) == 0))
+    return x;
+  return x.contiguous().view({-1, width});
+}
+
+bool norm_aligned(const Tensor& rows) {
+  const int64_t e = rows.element_size(), full = 16 / e;
+  return rows.size(1) % full == 0 && rows.stride(0) % full == 0 &&
+         aligned16(rows.data_ptr());
+}
+
+void check_norm(const Tensor& x, const std::optional<Tensor>& w,
+                const char* name) {
+  if (!w) return;
+  TORCH_CHECK(w->device() == x.device(), "layer_norm: ", name,
+              " is on another device than x");
+  TORCH_CHECK(w->dim() == 1 && w->size(0) == x.size(-1), "layer_norm: ", name,
+              " must be [", x.size(-1), "]");
+  TORCH_CHECK(w->scalar_type() == x.scalar_type() ||
+                  w->scalar_type() == torch::kFloat,
+              "layer_norm: ", name, " must have x's type or float32");
+}
+
+void check_norm(const Tensor& x, const std::optional<Tensor>& w,
+                const std::optional<Tensor>& b) {
+  TORCH_CHECK(x.is_cuda(), "layer_norm: x must be on GPU");
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= (1 << 24),
+              "layer_norm: the last dimension must have 1 to 2^24 values");
+  check_norm(x, w, "weight");
+  check_norm(x, b, "bias");
+  TORCH_CHECK(!w || !b || w->scalar_type() == b->scalar_type(),
+              "layer_norm: weight and bias must have one type");
+}
+
+std::vector<Tensor> layer_norm_fwd(const Tensor& x, std::optional<Tensor> w,
+                                   std::optional<Tensor> b, double eps,
+                                   bool stats) {
+  check_norm(x, w, b);
+  const int type = elem_type(x, "layer_norm");
+  const c10::DeviceGuard guard(x.device());
+  const int64_t width = x.size(-1), rows = x.numel() / width;
+  Tensor y = torch::empty(x.sizes(), x.options().memory_format(
+                                         at::MemoryFormat::Contiguous));
+  Tensor st;
+  if (stats) st = torch::empty({2, rows}, x.options().dtype(torch::kFloat));
+  if (rows > 0) {
+    const Tensor xr = as_rows(x, width);
+    if (w) w = w->contiguous();
+    if (b) b = b->contiguous();
+    NormArgs a{};
+    a.x = xr.data_ptr();
+    a.w = w ? w->data_ptr() : nullptr;
+    a.b = b ? b->data_ptr() : nullptr;
+    a.y = y.data_ptr();
+    if (stats) {
+      a.mean = st.data_ptr<float>();
+      a.rstd = a.mean + rows;
+    }
+    a.rows = rows;
+    a.width = (int)width;
+    a.x_stride = rows > 1 ? xr.stride(0) : width;
+    a.aligned = norm_aligned(xr) && aligned16(a.w) && aligned16(a.b);
+    a.eps = (float)eps;
+    launched(layer_norm_fwd_launch(
+                 &a, type, w ? elem_type(*w, "layer_norm")
+                             : b ? elem_type(*b, "layer_norm") : type,
+                 current()),
+             "layer_norm");
+  }
+  return {y, st};
+}
+
+// Returns dx, dw, db; undefined where not wanted.
+std::vector<Tensor> layer_norm_bwd(const Tensor& dy, const Tensor& x,
+                                   std::optional<Tensor> w,
+                                   torch::ScalarType wtype, const Tensor& st,
+                                   bool want_dx, bool want_dw, bool want_db) {
+  TORCH_CHECK(dy.sizes() == x.sizes() && dy.scalar_type() == x.scalar_type() &&
+                  dy.device() == x.device(),
+              "layer_norm: the output's gradient does not match x");
+  const int type = elem_type(x, "layer_norm");
+  const c10::DeviceGuard guard(x.device());
+  const int64_t width = x.size(-1), rows = x.numel() / width;
+  const auto wopts = x.options().dtype(wtype);
+  Tensor dx, dw, db;
+  if (want_dx)
+    dx = torch::empty(x.sizes(), x.options().memory_format(
+                                     at::MemoryFormat::Contiguous));
+  if (want_dw)
+    dw = rows ? torch::empty({width}, wopts) : torch::zeros({width}, wopts);
+  if (want_db)
+    db = rows ? torch::empty({width}, wopts) : torch::zeros({width}, wopts);
+  if (rows > 0) {
+    const Tensor xr = as_rows(x, width), dyr = as_rows(dy, width);
+    if (w) w = w->contiguous();
+    NormArgs a{};
+    a.dy = dyr.data_ptr();
+    a.x = xr.data_ptr();
+    a.w = w ? w->data_ptr() : nullptr;
+    a.dx = want_dx ? dx.data_ptr() : nullptr;
+    a.mean = st.data_ptr<float>();
+    a.rstd = a.mean + rows;
+    a.rows = rows;
+    a.width = (int)width;
+    a.x_stride = rows > 1 ? xr.stride(0) : width;
+    a.dy_stride = rows > 1 ? dyr.stride(0) : width;
+    a.aligned = norm_aligned(xr) && norm_aligned(dyr) && aligned16(a.w);
+    a.parts = layer_norm_parts(rows, (int)width, type, a.aligned);
+    Tensor part;
+    if (want_dw || want_db) {
+      part = torch::empty({a.parts, 2 * width},
+                          x.options().dtype(torch::kFloat));
+      a.part = part.data_ptr<float>();
+    }
+    const int wt = wtype == torch::kFloat ? 0 : type;
+    launched(layer_norm_bwd_launch(&a, type, wt, current()),
+             "layer_norm backward");
+    if (a.part != nullptr)
+      launched(sum_rows_launch(a.part, a.parts, (int)(2 * width), (int)width,
+                               want_dw ? dw.data_ptr() : nullptr,
+                               want_db ? db.data_ptr() : nullptr, wt,
+                               current()),
+               "layer_norm backward");
+  }
+  return {dx, dw, db};
+}
+
+// ----------------------------------------------------------------- AdamW
+
+// Written ranges of memory: sorted, they must not meet.
+struct Written {
+  std::vector<std::pair<uintptr_t, uintptr_t>> ranges;
+  void add(const Tensor& t) {
+    const auto a = (uintptr_t)t.data_ptr();
+    ranges.emplace_back(a, a + (uintptr_t)t.numel() * t.element_size());
+  }
+  void check(const char* what) {
+    std::sort(ranges.begin(), ranges.end());
+    for (size_t i = 1; i < ranges.size(); ++i)
+      TORCH_CHECK(ranges[i].first >= ranges[i - 1].second, what,
+                  ": two of the tensors to write share memory");
+  }
+};
+
+constexpr int64_t kBlock8 = 256;
+
+void adamw_step(const Tensors& p, const Tensors& g, const Tensors& m,
+                const Tensors& v, const std::optional<Tensors>& ms,
+                const std::optional<Tensors>& vs,
+                const std::optional<Tensor>& norm, double max_norm,
+                double step, double lr, double beta1, double beta2,
+                double eps, double weight_decay) {
+  const size_t count = p.size();
+  TORCH_CHECK(g.size() == count && m.size() == count && v.size() == count &&
+                  ms.has_value() == vs.has_value() &&
+                  (!ms || (ms->size() == count && vs->size() == count)),
+              "adamw_step: the lists have different lengths");
+  if (count == 0) return;
+  const auto device = p[0].device();
+  TORCH_CHECK(device.is_cuda(), "adamw_step: parameters must be on GPU");
+  const auto state_type = ms ? torch::kByte : torch::kFloat;
+  if (norm)
+    TORCH_CHECK(norm->device() == device && norm->numel() == 1 &&
+                    norm->scalar_type() == torch::kFloat,
+                "adamw_step: grad_norm must be one float32 on the "
+                "parameters' device");
+  const c10::DeviceGuard guard(device);
+  const hipStream_t stream = current();
+  hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
+  launched(hipStreamIsCapturing(stream, &capturing), "adamw_step");
+  TORCH_CHECK(capturing == hipStreamCaptureStatusNone,
+              "adamw_step: the step's number and rate are the host's and "
+              "would stay the same in every replay of a captured graph");
+
+  Written written;
+  written.ranges.reserve(count * (ms ? 5 : 3));
+  Tensors copies;               // gradients laid out like their parameter
+  std::vector<const void*> grads(count);
+  for (size_t i = 0; i < count; ++i) {
+    TORCH_CHECK(p[i].device() == device && g[i].device() == device &&
+                    m[i].device() == device && v[i].device() == device,
+                "adamw_step: tensor ", i, " is on another device");
+    TORCH_CHECK(!g[i].is_sparse(), "adamw_step: gradient ", i, " is sparse");
+    TORCH_CHECK(g[i].scalar_type() == p[i].scalar_type() &&
+                    m[i].scalar_type() == state_type &&
+                    v[i].scalar_type() == state_type,
+                "adamw_step: tensor ", i,
+                ": the gradient must have the parameter's type and the "
+                "states must be ", state_type);
+    TORCH_CHECK(g[i].sizes() == p[i].sizes() && m[i].sizes() == p[i].sizes() &&
+                    v[i].sizes() == p[i].sizes(),
+                "adamw_step: tensor ", i, ": sizes differ");
+    TORCH_CHECK(p[i].is_non_overlapping_and_dense(), "adamw_step: parameter ",
+                i, " must be dense");
+    elem_type(p[i], "adamw_step");
+    const bool plain = p[i].is_contiguous();
+    const auto laid_out = [&](const Tensor& t) {
+      return plain ? t.is_contiguous() : t.strides() == p[i].strides();
+    };
+    TORCH_CHECK(laid_out(m[i]) && laid_out(v[i]), "adamw_step: the states of "
+                "tensor ", i, " must have the parameter's strides");
+    if (laid_out(g[i])) {
+      grads[i] = g[i].data_ptr();
+    } else {
+      copies.push_back(torch::empty_strided(p[i].sizes(), p[i].strides(),
+                                            p[i].options()).copy_(g[i]));
+      grads[i] = copies.back().data_ptr();
+    }
+    written.add(p[i]);
+    written.add(m[i]);
+    written.add(v[i]);
+    if (ms) {
+      const int64_t blocks = (p[i].numel() + kBlock8 - 1) / kBlock8;
+      for (const Tensor* s : {&(*ms)[i], &(*vs)[i]}) {
+        TORCH_CHECK(s->device() == device &&
+                        s->scalar_type() == torch::kByte &&
+                        s->is_contiguous() && s->numel() == blocks,
+                    "adamw_step: the scales of tensor ", i, " must be ",
+                    blocks, " contiguous bytes");
+        written.add(*s);
+      }
+    }
+  }
+  written.check("adamw_step");
+
+  AdamWScalars s{};
+  s.beta1 = (float)beta1;
+  s.one_minus_beta1 = (float)(1.0 - beta1);
+  s.beta2 = (float)beta2;
+  s.one_minus_beta2 = (float)(1.0 - beta2);
+  s.eps = (float)eps;
+  s.decay = (float)(1.0 - lr * weight_decay);
+  s.rate = (float)(lr / (1.0 - std::pow(beta1, step)));
+  s.inv_bc2 = (float)(1.0 / std::sqrt(1.0 - std::pow(beta2, step)));
+  s.max_norm = (float)max_norm;
+  s.norm = norm ? norm->data_ptr<float>() : nullptr;
+
+  // One launch takes tensors of one type.
+  for (int type = 0; type < 3; ++type) {
+    std::vector<void*> tp, tm, tv;
+    std::vector<const void*> tg;
+    std::vector<unsigned char*> tms, tvs;
+    std::vector<long> tn;
+    for (size_t i = 0; i < count; ++i) {
+      if (p[i].numel() == 0 || elem_type(p[i], "adamw_step") != type) continue;
+      tp.push_back(p[i].data_ptr());
+      tg.push_back(grads[i]);
+      tm.push_back(m[i].data_ptr());
+      tv.push_back(v[i].data_ptr());
+      if (ms) {
+        tms.push_back((*ms)[i].data_ptr<uint8_t>());
+        tvs.push_back((*vs)[i].data_ptr<uint8_t>());
+      }
+      tn.push_back(p[i].numel());
+    }
+    if (tp.empty()) continue;
+    const AdamWTensors a{(int)tp.size(), tp.data(), tg.data(), tm.data(),
+                         tv.data(), ms ? tms.data() : nullptr,
+                         ms ? tvs.data() : nullptr, tn.data()};
+    launched(adamw_launch(&a, &s, type, stream), "adamw_step");
+  }
+}
+
+Tensor grad_norm(const Tensors& g) {
+  TORCH_CHECK(!g.empty(), "grad_norm: no tensors");
+  const auto device = g[0].device();
+  TORCH_CHECK(device.is_cuda(), "grad_norm: tensors must be on GPU");
+  const c10::DeviceGuard guard(device);
+  Tensors dense;
+  std::vector<const void*> at[3];
+  std::vector<long> n[3];
+  long parts = 0;
+  for (const Tensor& t : g) {
+    TORCH_CHECK(t.device() == device,
+                "grad_norm: the tensors are on several devices");
+    const int type = elem_type(t, "grad_norm");
+    TORCH_CHECK(!t.is_sparse(), "grad_norm: a tensor is sparse");
+    if (t.numel() == 0) continue;
+    if (t.is_non_overlapping_and_dense()) {
+      at[type].push_back(t.data_ptr());
+    } else {
+      dense.push_back(t.contiguous());
+      at[type].push_back(dense.back().data_ptr());
+    }
+    n[type].push_back(t.numel());
+    parts += (t.numel() + adamw_chunk() - 1) / adamw_chunk();
+  }
+  const auto opts = torch::TensorOptions().device(device);
+  Tensor out = torch::empty({}, opts.dtype(torch::kFloat));
+  Tensor partial = torch::empty({parts}, opts.dtype(torch::kDouble));
+  double* next = parts ? partial.data_ptr<double>() : nullptr;
+  for (int type = 0; type < 3; ++type) {
+    if (at[type].empty()) continue;
+    launched(square_sum_launch(at[type].data(), n[type].data(),
+                               (int)at[type].size(), type, next, current()),
+             "grad_norm");
+    for (const long k : n[type]) next += (k + adamw_chunk() - 1) / adamw_chunk();
+  }
+  launched(norm_launch(parts ? partial.data_ptr<double>() : nullptr,
+                       (int)parts, out.data_ptr<float>(), current()),
+           "grad_norm");
+  return out;
+}
+
+std::tuple<Tensor, Tensor> pack_state8(const Tensor& x, bool is_signed) {
+  TORCH_CHECK(x.is_cuda() && x.scalar_type() == torch::kFloat &&
+                  x.is_non_overlapping_and_dense(),
+              "pack_state8: a dense float32 tensor on GPU");
+  const c10::DeviceGuard guard(x.device());
+  Tensor codes = torch::empty_strided(x.sizes(), x.strides(),
+                                      x.options().dtype(torch::kByte));
+  Tensor scales = torch::empty({(x.numel() + kBlock8 - 1) / kBlock8},
+                               x.options().dtype(torch::kByte));
+  if (x.numel())
+    launched(pack8_launch(x.data_ptr<float>(), codes.data_ptr<uint8_t>(),
+                          scales.data_ptr<uint8_t>(), x.numel(), is_signed,
+                          current()),
+             "pack_state8");
+  return {codes, scales};
+}
+
+Tensor unpack_state8(const Tensor& codes, const Tensor& scales,
+                     bool is_signed, torch::ScalarType dtype) {
+  TORCH_CHECK(codes.is_cuda() && codes.scalar_type() == torch::kByte &&
+                  codes.is_non_overlapping_and_dense(),
+              "unpack_state8: codes must be dense bytes on GPU");
+  TORCH_CHECK(scales.device() == codes.device() &&
+                  scales.scalar_type() == torch::kByte &&
+                  scales.is_contiguous() &&
+                  scales.numel() == (codes.numel() + kBlock8 - 1) / kBlock8,
+              "unpack_state8: scales must be one byte for 256 codes");
+  const c10::DeviceGuard guard(codes.device());
+  Tensor out = torch::empty_strided(codes.sizes(), codes.strides(),
+                                    codes.options().dtype(dtype));
+  const int type = elem_type(out, "unpack_state8");
+  if (codes.numel())
+    launched(unpack8_launch(codes.data_ptr<uint8_t>(),
+                            scales.data_ptr<uint8_t>(), out.data_ptr(),
+                            codes.numel(), is_signed, type, current()),
+             "unpack_state8");
+  return out;
+}
+
+}  // namespace
+
+void register_train_ops(pybind11::module_& m) {
+  m.def("layer_norm_fwd", &layer_norm_fwd, "layer norm forward (CDNA4)");
+  m.def("layer_norm_bwd", &layer_norm_bwd, "layer norm backward (CDNA4)");
+  m.def("adamw_step", &adamw_step, "AdamW step over many tensors (CDNA4)");
+  m.def("grad_norm", &grad_norm, "2-norm over many tensors (CDNA4)");
+  m.def("pack_state8", &pack_state8, "fp32 -> 8-bit optimizer state");
+  m.def("unpack_state8", &unpack_state8, "8-bit optimizer state -> values");
+}

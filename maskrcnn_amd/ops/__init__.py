@@ -1,4 +1,5 @@
-"""Compute ops: RoIAlign, NMS, detection post-processing.
+"""Compute ops: RoIAlign, NMS, detection post-processing, dense layers,
+layer norm and the optimizer step.
 
 Each op has a hand-written CDNA4 HIP kernel (csrc/hip/*) used on GPU and a
 pure-PyTorch reference used on CPU and as the numerics oracle in tests.
@@ -12,3 +13,7 @@ from .nms import (  # noqa: F401
 )
 from .fpn_fuse import fpn_fuse  # noqa: F401
 from .conv3x3 import conv3x3_bias_relu, conv3x3_bn_relu  # noqa: F401
+from .layer_norm import layer_norm, LayerNorm  # noqa: F401
+from .adamw import (  # noqa: F401
+    adamw_step, grad_norm, pack_state8, unpack_state8,
+)

@@ -1,0 +1,209 @@
+"""AdamW step over many tensors, with states in 32 or 8 bits.
+
+    c = min(1, max_grad_norm / (grad_norm + 1e-6))
+    m = beta1 m + (1 - beta1) c g       v = beta2 v + (1 - beta2) (c g)^2
+    p = p (1 - lr wd) - lr / (1 - beta1^t) * m / (sqrt(v / (1 - beta2^t)) + eps)
+
+GPU: csrc/hip/adamw.hip, a launch for some 60 to 90 tensors; the gradients
+are read, never rewritten, so the clipped norm costs no pass of its own over
+them. CPU: the same operations in plain torch (the numerics oracle; the two
+give the same bits).
+
+8-bit states: 256 values in memory order share a power of two, and a value
+is its ratio to it with 3 bits of mantissa (pack_state8, unpack_state8).
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+from ._ext import require_ext
+
+BLOCK8 = 256        # values of an 8-bit state that share one scale
+_MIN_EXP = 40       # keeps every power and step a normal fp32 number
+
+
+def _dense(t):
+    """A dense tensor's values in memory order, as a view."""
+    return t.as_strided((t.numel(),), (1,))
+
+
+def _is_dense(t):
+    return torch.ops.aten.is_non_overlapping_and_dense(t)
+
+
+def _pack_torch(x, signed):
+    low, top = (14, 127) if signed else (30, 255)
+    n = x.numel()
+    flat = torch.zeros(-(-n // BLOCK8) * BLOCK8, dtype=torch.float32)
+    flat[:n] = _dense(x)
+    bits = flat.view(torch.int32) & 0x7FFFFFFF
+    blocks = bits.view(-1, BLOCK8)
+    e = (blocks.amax(1) >> 23).clamp(min=_MIN_EXP) if n else \
+        torch.zeros(0, dtype=torch.int32)
+    inv = ((254 - e) << 23).view(torch.float32)
+    inv = torch.where(e == 255, torch.zeros_like(inv), inv)
+    r = (flat.abs().view(-1, BLOCK8) * inv[:, None]).view(-1)
+    rb = r.view(torch.int32)
+    code = ((rb + 0x7FFFF + ((rb >> 20) & 1)) >> 20) - ((126 - low) << 3)
+    small = r < 2.0 ** -low
+    code = torch.where(
+        small, torch.round(torch.where(small, r, torch.zeros_like(r)) *
+                           2.0 ** (low + 3)).to(torch.int32),
+        code.clamp(max=top))
+    if signed:
+        code = code | ((flat.view(torch.int32) < 0).to(torch.int32) << 7)
+    else:
+        code = torch.where((flat > 0) & (code == 0),
+                           torch.ones_like(code), code)
+    code = torch.where((e == 255).repeat_interleave(BLOCK8),
+                       torch.zeros_like(code), code)
+    codes = torch.empty_strided(x.shape, x.stride(), dtype=torch.uint8)
+    _dense(codes).copy_(code[:n])
+    return codes, e.to(torch.uint8)
+
+
+def _unpack_torch(codes, scales, signed, dtype):
+    low = 14 if signed else 30
+    c = _dense(codes).to(torch.int32)
+    mag = c & 127 if signed else c
+    r = torch.where(mag >= 8,
+                    ((mag + ((126 - low) << 3)) << 20).view(torch.float32),
+                    mag * 2.0 ** -(low + 3))
+    if signed:
+        r = torch.where(c > 127, -r, r)
+    e = scales.to(torch.int32)
+    one = (e << 23).view(torch.float32)
+    one = torch.where(e == 255, torch.full_like(one, math.nan), one)
+    out = torch.empty_strided(codes.shape, codes.stride(), dtype=dtype)
+    _dense(out).copy_(r * one.repeat_interleave(BLOCK8)[:c.numel()])
+    return out
+
+
+def pack_state8(x: torch.Tensor, signed: bool):
+    """fp32 values -> (codes, scales), both uint8.
+
+    signed: the first moment's code (sign, 4 bits of exponent, 3 of
+    mantissa), else the second's (5 bits of exponent), whose values above
+    zero never get the code of zero. codes has x's shape and strides,
+    scales one value for 256 of x in memory order. A block with an infinity
+    or NaN stands for NaN.
+    """
+    if x.is_cuda:
+        return require_ext().pack_state8(x, signed)
+    if x.dtype != torch.float32 or not _is_dense(x):
+        raise RuntimeError("pack_state8: a dense float32 tensor")
+    return _pack_torch(x, signed)
+
+
+def unpack_state8(codes: torch.Tensor, scales: torch.Tensor, signed: bool,
+                  dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The values that codes and scales stand for; bfloat16 holds them
+    exactly."""
+    if codes.is_cuda:
+        return require_ext().unpack_state8(codes, scales, signed, dtype)
+    if codes.dtype != torch.uint8 or not _is_dense(codes):
+        raise RuntimeError("unpack_state8: codes must be dense bytes")
+    if scales.dtype != torch.uint8 or scales.dim() != 1 or \
+            scales.numel() != -(-codes.numel() // BLOCK8):
+        raise RuntimeError("unpack_state8: scales must be one byte for 256 "
+                           "codes")
+    return _unpack_torch(codes, scales, signed, dtype)
+
+
+def grad_norm(tensors) -> torch.Tensor:
+    """2-norm over all values of a list of tensors, as one fp32 value on
+    their device. Squares are summed in 64 bits."""
+    tensors = list(tensors)
+    if not tensors:
+        raise RuntimeError("grad_norm: no tensors")
+    if tensors[0].is_cuda:
+        return require_ext().grad_norm(tensors)
+    return torch.stack([t.double().square().sum()
+                        for t in tensors]).sum().sqrt().float()
+
+
+def _step_torch(p, g, m, v, clip, beta1, beta2, eps, decay, rate, inv_bc2):
+    """One tensor's step; m and v are fp32 and changed in place. The root
+    goes through 64 bits, as torch's own in fp32 on the CPU is not always
+    the nearest."""
+    gf = g.float()
+    if clip is not None:
+        gf = gf * clip
+    m.copy_(m * beta1 + gf * (1.0 - beta1))
+    v.copy_(v * beta2 + (gf * gf) * (1.0 - beta2))
+    p.copy_(p.float() * decay - m /
+            (torch.sqrt(v.double()).float() * inv_bc2 + eps) * rate)
+
+
+@torch.no_grad()
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *,
+               exp_avg_scales=None, exp_avg_sq_scales=None, step: int,
+               lr: float, betas=(0.9, 0.999), eps: float = 1e-8,
+               weight_decay: float = 0.0, grad_norm=None,
+               max_grad_norm: float = 0.0) -> None:
+    """Updates params and their states in place.
+
+    params: float32, bfloat16 or float16, dense, in any mixture; grads: in
+    their parameter's type and shape. exp_avgs, exp_avg_sqs: float32 in the
+    parameter's shape and strides; or uint8 codes in that layout with
+    exp_avg_scales and exp_avg_sq_scales, one byte for 256 values (zeros in
+    both for a state that begins). step: the number of this step, from 1.
+    grad_norm: one float32 on the device (of grad_norm()); the gradients
+    count as scaled to max_grad_norm where it is above that.
+
+    step and lr are the host's, so the call is refused while a stream is
+    captured into a graph. No two tensors to write may share memory.
+    """
+    beta1, beta2 = betas
+    if not 0.0 <= beta1 < 1.0 or not 0.0 <= beta2 < 1.0:
+        raise ValueError(f"adamw_step: betas {betas} outside [0, 1)")
+    if step < 1:
+        raise ValueError(f"adamw_step: step {step} below 1")
+    if grad_norm is not None and not max_grad_norm > 0.0:
+        raise ValueError("adamw_step: grad_norm without a max_grad_norm "
+                         "above 0")
+    if params and params[0].is_cuda:
+        require_ext().adamw_step(
+            params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales,
+            exp_avg_sq_scales, grad_norm, max_grad_norm, step, lr, beta1,
+            beta2, eps, weight_decay)
+        return
+    eight = exp_avg_scales is not None
+    if eight != (exp_avg_sq_scales is not None) or not (
+            len(params) == len(grads) == len(exp_avgs) == len(exp_avg_sqs)) \
+            or eight and not (len(params) == len(exp_avg_scales) ==
+                              len(exp_avg_sq_scales)):
+        raise RuntimeError("adamw_step: the lists have different lengths")
+    clip = None
+    if grad_norm is not None:
+        clip = (torch.full_like(grad_norm, max_grad_norm) /
+                (grad_norm + 1e-6)).clamp(max=1.0)
+    scalars = (clip, beta1, beta2, eps, 1.0 - lr * weight_decay,
+               lr / (1.0 - beta1 ** step),
+               1.0 / math.sqrt(1.0 - beta2 ** step))
+    for i, (p, g, m, v) in enumerate(zip(params, grads, exp_avgs,
+                                         exp_avg_sqs)):
+        want = torch.uint8 if eight else torch.float32
+        if p.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+            raise RuntimeError(f"adamw_step: parameter {i} is {p.dtype}")
+        if g.dtype != p.dtype or m.dtype != want or v.dtype != want:
+            raise RuntimeError(f"adamw_step: tensor {i}: the gradient must "
+                               "have the parameter's type and the states "
+                               f"must be {want}")
+        if not g.shape == m.shape == v.shape == p.shape:
+            raise RuntimeError(f"adamw_step: tensor {i}: sizes differ")
+        if not eight:
+            _step_torch(p, g, m, v, *scalars)
+            continue
+        mf = unpack_state8(m, exp_avg_scales[i], True)
+        vf = unpack_state8(v, exp_avg_sq_scales[i], False)
+        _step_torch(p, g, mf, vf, *scalars)
+        for codes, scales, x, signed in (
+                (m, exp_avg_scales[i], mf, True),
+                (v, exp_avg_sq_scales[i], vf, False)):
+            new, exps = pack_state8(x, signed)
+            codes.copy_(new)
+            scales.copy_(exps)
