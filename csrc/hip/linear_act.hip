@@ -1,0 +1,565 @@
+// Matrix products of dense layers, with bias, activation and residual in the
+// epilogue, and their gradients.
+//
+//   z = x W^T + b      y = act(z) + r      slope = act'(z)
+//   dz = dy slope      dx = dz W           dW = dz^T x      db = sum dz
+//
+// The derivative is kept for the backward, not z: it is formed where z is
+// still in fp32, so ReLU's is exact in any type and no erf or exp is
+// computed twice; GELU's and SiLU's are rounded once to the tensors' type,
+// like dz, which the matrix cores take in that type.
+//
+// All three products are one kernel, D[m][n] = sum_k X(m,k) Y(n,k), where
+// either operand may lie with k consecutive or with its own index
+// consecutive:
+//   forward X = x, Y = W;  dx: X = dz, Y = W (n consecutive);
+//   dW: X = dz, Y = x (both with their own index consecutive).
+//
+// A workgroup computes a kBM x kBN tile, waves in a grid over it. Each step
+// takes 128 bytes of k from both operands through LDS (two buffers): memory
+// to LDS directly, 16 bytes a lane, the next step's loads in flight during
+// this step's products. The bounds are the buffer descriptor's: rows and
+// columns past the end read as 0. Lanes of one load go to consecutive LDS
+// addresses, so what would be a column of equal banks is spread by choosing
+// which 16 bytes a lane fetches (an exclusive or with the row's bits).
+// Operands with k consecutive are read from LDS 16 bytes a lane; with 16-bit
+// types the others go through the transposing LDS read, 4 values of k a
+// lane. Y is the matrix instruction's row operand, so that a lane ends up
+// with 4 consecutive columns of one row of D.
+//
+// Few tiles: the k axis is split, partial sums go to memory in fp32 and a
+// second kernel adds them in order and applies the epilogue.
+#include <hip/hip_runtime.h>
+
+#include "train_ops.h"
+#include "typed.h"
+
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
+typedef fp16_t fp16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) char lds_char;
+
+constexpr int kRow = 128;                 // bytes of k in one step
+constexpr unsigned kOutside = 0x80000000u;  // above any descriptor's range
+
+// One packet of 16 bytes an operand; the products of all its values.
+__device__ inline void mma(f32x4& acc, i32x4 a, i32x4 b, bf16_t) {
+  acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+      __builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), acc, 0, 0,
+      0);
+}
+__device__ inline void mma(f32x4& acc, i32x4 a, i32x4 b, fp16_t) {
+  acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+      __builtin_bit_cast(fp16x8, a), __builtin_bit_cast(fp16x8, b), acc, 0, 0,
+      0);
+}
+__device__ inline void mma(f32x4& acc, i32x4 a, i32x4 b, float) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__int_as_float(a[j]),
+                                               __int_as_float(b[j]), acc, 0,
+                                               0, 0);
+}
+
+// 16 bytes a lane from memory to LDS at `to` + 16 * lane. In assembly, as
+// the compiler would wait for it before every transposing LDS read; there is
+// no output register, and the waits are the caller's.
+__device__ inline void load_lds(i32x4 desc, unsigned from, unsigned to) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\ts_nop 0\n\t"
+      "buffer_load_dwordx4 %1, %2, 0 offen lds"
+      :
+      : "s"(to), "v"(from), "s"(desc)
+      : "memory");
+}
+
+// Every load into LDS has arrived and every read of it is done, in all waves.
+__device__ inline void all_arrived() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+__device__ inline i32x4 descriptor(const char* base, long bytes) {
+  const unsigned long a = (unsigned long)base;
+  const long range = bytes < 0 ? 0 : bytes < 0x7fffffff ? bytes : 0x7fffffff;
+  i32x4 d;
+  d[0] = __builtin_amdgcn_readfirstlane((int)a);
+  d[1] = __builtin_amdgcn_readfirstlane((int)(a >> 32) & 0xffff);
+  d[2] = __builtin_amdgcn_readfirstlane((int)range);
+  d[3] = 0x00020000;
+  return d;
+}
+
+// One operand's tile of kR rows (its own index) and 128 bytes of k.
+template <typename T, bool kTrans, int kR, int kWaves>
+struct Operand {
+  static constexpr int kPer = 16 / sizeof(T);           // values of a packet
+  static constexpr int kK = kRow / sizeof(T);           // k of one step
+  static constexpr int kBytes = kR * kRow;
+  static constexpr int kLoads = kBytes / (1024 * kWaves);
+  static_assert(kLoads * 1024 * kWaves == kBytes, "whole loads for each wave");
+  // With its own index consecutive: packets of one row of k, and how many
+  // packets the 16 indices of a matrix operand take.
+  static constexpr int kPackets = kR / kPer;
+  static constexpr int kUnit = 16 / kPer;
+  static constexpr int kUnits = kPackets / kUnit;
+
+  const char* base;     // at the tile's first row, k = 0
+  long ld;              // bytes
+  int extent;           // rows left from the tile's first
+  int k;                // k altogether
+  unsigned from[kLoads];
+
+  static __device__ int twist(int r) {
+    if constexpr (!kTrans) return (r >> 1) & 7;
+    // The rows of k that one read takes fall on different banks: 8 g + 0..3
+    // for 16-bit types, 4 g for fp32.
+    const int f = sizeof(T) == 2 ? (r & 3) | ((r >> 3) & 1) << 2
+                                 : (r >> 2) & 3;
+    return f & (kUnits - 1);
+  }
+
+  __device__ void init(const void* p, long ld_values, int first, int total,
+                       int k_total, int wave, int lane) {
+    ld = ld_values * (long)sizeof(T);
+    k = k_total;
+    extent = total - first;
+    base = (const char*)p + (kTrans ? first * (long)sizeof(T) : first * ld);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int at = (wave * kLoads + i) * 64 + lane;    // packet in LDS
+      if constexpr (!kTrans) {
+        const int r = at >> 3, c = (at & 7) ^ twist(r);
+        from[i] = (unsigned)(r * (int)ld + c * 16);
+      } else {
+        const int r = at / kPackets, s = at % kPackets;
+        const int c = ((s / kUnit) ^ twist(r)) * kUnit + s % kUnit;
+        from[i] = (unsigned)(r * (int)ld + c * 16);
+      }
+    }
+  }
+
+  // The step's loads; `to`: LDS address of the tile.
+  __device__ void load(int step, unsigned to, int wave, int lane) const {
+    const int k0 = step * kK;
+    const char* p;
+    long bytes;
+    if constexpr (!kTrans) {
+      p = base + (long)step * kRow;
+      bytes = (extent - 1) * ld + (long)(k - k0) * (long)sizeof(T);
+    } else {
+      p = base + k0 * ld;
+      bytes = (k - k0 - 1) * ld + (long)extent * (long)sizeof(T);
+    }
+    const i32x4 d = descriptor(p, bytes);
+    to += wave * kLoads * 1024;
+    if (!kTrans && k - k0 < kK) {
+      // The last step of a ragged k: packets past it would be the next
+      // row's.
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int at = (wave * kLoads + i) * 64 + lane;
+        const int c = (at & 7) ^ twist(at >> 3);
+        load_lds(d, c * kPer < k - k0 ? from[i] : kOutside, to + i * 1024);
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) load_lds(d, from[i], to + i * 1024);
+  }
+
+  // The packet of rows r0 + lane % 16 and k-group lane / 16 of half `h`.
+  static __device__ i32x4 read(const char* tile, int r0, int h, int lane) {
+    const int g = (lane >> 4) + 4 * h, i = lane & 15;
+    if constexpr (!kTrans) {
+      const int r = r0 + i;
+      return *(const i32x4*)(tile + r * kRow + ((g ^ twist(r)) << 4));
+    } else if constexpr (sizeof(T) == 2) {
+      i32x4 out;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int r = g * 8 + q * 4 + (i >> 2);
+        const char* p = tile + r * (kR * 2) +
+                        (((r0 >> 4) ^ twist(r)) << 5) + ((i & 3) << 3);
+        const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) s16x4*)p);
+        const long two = __builtin_bit_cast(long, v);
+        out[2 * q] = (int)two;
+        out[2 * q + 1] = (int)(two >> 32);
+      }
+      return out;
+    } else {
+      i32x4 out;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = g * 4 + j;
+        out[j] = *(const int*)(tile + r * (kR * 4) +
+                               (((r0 >> 4) ^ twist(r)) << 6) + (i << 2));
+      }
+      return out;
+    }
+  }
+};
+
+// ---------------------------------------------------------------- epilogue
+
+__device__ inline void activate(int act, float z, float& y, float& slope) {
+  switch (act) {
+    case kActRelu:
+      y = z < 0.0f ? 0.0f : z;            // NaN stays
+      slope = z > 0.0f ? 1.0f : 0.0f;
+      break;
+    case kActGelu: {
+      const float cdf = 0.5f * (1.0f + erff(z * 0.70710678f));
+      y = z * cdf;
+      slope = cdf + z * (0.39894228f * __expf(-0.5f * z * z));
+      break;
+    }
+    case kActSilu: {
+      const float s = 1.0f / (1.0f + __expf(-z));
+      y = z * s;
+      slope = s * (1.0f + z * (1.0f - s));
+      break;
+    }
+    default:
+      y = z;
+      slope = 1.0f;
+  }
+}
+
+constexpr int kOut = 8;       // consecutive columns that a lane finishes
+
+// Columns n .. n + 7 of row m.
+template <typename T>
+__device__ inline void finish(const LinearEpilogue& e, long m, int n, int N,
+                              float (&z)[kOut]) {
+  float s[kOut];
+  const T* bias = (const T*)e.bias;
+  const T* res = (const T*)e.residual + m * e.ld_residual;
+  T* out = (T*)e.y + m * (long)N;
+  T* slope = e.slope ? (T*)e.slope + m * (long)N : nullptr;
+  if (e.wide) {      // then N % 8 == 0
+    float b[kOut] = {}, r[kOut] = {};
+    if (bias) load_f32<T, kOut>(bias + n, b);
+    if (e.residual) load_f32<T, kOut>(res + n, r);
+#pragma unroll
+    for (int i = 0; i < kOut; ++i) {
+      activate(e.act, z[i] + b[i], z[i], s[i]);
+      z[i] += r[i];
+    }
+    store_f32<T, kOut>(out + n, z);
+    if (slope) store_f32<T, kOut>(slope + n, s);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < kOut; ++i) {
+    if (n + i >= N) return;
+    activate(e.act, z[i] + (bias ? (float)bias[n + i] : 0.0f), z[i], s[i]);
+    if (e.residual) z[i] += (float)res[n + i];
+    out[n + i] = (T)z[i];
+    if (slope) slope[n + i] = (T)s[i];
+  }
+}
+
+// ------------------------------------------------------------------ kernel
+
+template <typename T, bool kXT, bool kYT, int kBM, int kBN, int kWM, int kWN>
+__global__ __launch_bounds__(kWM * kWN * 64) void product_kernel(
+    LinearProduct a) {
+  constexpr int kWaves = kWM * kWN;
+  using X = Operand<T, kXT, kBM, kWaves>;
+  using Y = Operand<T, kYT, kBN, kWaves>;
+  constexpr int kMI = kBM / kWM / 16, kNI = kBN / kWN / 16;
+  constexpr int kStage = X::kBytes + Y::kBytes;
+  __shared__ __attribute__((aligned(1024))) char lds[2][kStage];
+
+  // Workgroups go round the 8 chiplets; each gets a consecutive run of
+  // tiles, columns fastest, so that its L2 keeps the rows of X.
+  const int tiles_n = (a.n + kBN - 1) / kBN, tiles_m = (a.m + kBM - 1) / kBM;
+  const int total = gridDim.x, xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
+  const int big = total >> 3, rest = total & 7;
+  const int id = xcd * big + (xcd < rest ? xcd : rest) + at;
+  const int split = id / (tiles_m * tiles_n), tile = id % (tiles_m * tiles_n);
+  const int m0 = tile / tiles_n * kBM, n0 = tile % tiles_n * kBN;
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / kWN, wn = wave % kWN;
+  X x;
+  Y y;
+  x.init(a.x, a.ldx, m0, a.ext_x, a.kx, wave, lane);
+  y.init(a.y, a.ldy, n0, a.ext_y, a.ky, wave, lane);
+
+  const int steps = (a.kx + X::kK - 1) / X::kK;
+  const int first = split * a.steps_per_split;
+  const int last = first + a.steps_per_split < steps
+                       ? first + a.steps_per_split : steps;
+  const unsigned at_lds = (unsigned)(unsigned long)(lds_char*)&lds[0][0];
+
+  f32x4 acc[kMI][kNI] = {};
+  x.load(first, at_lds, wave, lane);
+  y.load(first, at_lds + X::kBytes, wave, lane);
+  for (int s = first; s < last; ++s) {
+    const int b = (s - first) & 1;
+    all_arrived();
+    if (s + 1 < last) {
+      const unsigned next = at_lds + (b ^ 1) * kStage;
+      x.load(s + 1, next, wave, lane);
+      y.load(s + 1, next + X::kBytes, wave, lane);
+    }
+    const char* xt = lds[b];
+    const char* yt = lds[b] + X::kBytes;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      i32x4 xf[kMI], yf[kNI];
+#pragma unroll
+      for (int i = 0; i < kMI; ++i)
+        xf[i] = X::read(xt, wm * (kBM / kWM) + i * 16, h, lane);
+#pragma unroll
+      for (int j = 0; j < kNI; ++j)
+        yf[j] = Y::read(yt, wn * (kBN / kWN) + j * 16, h, lane);
+#pragma unroll
+      for (int i = 0; i < kMI; ++i)
+#pragma unroll
+        for (int j = 0; j < kNI; ++j) mma(acc[i][j], yf[j], xf[i], T{});
+    }
+  }
+
+  // A lane holds row lane % 16 and columns 4 (lane / 16) .. + 3 of each
+  // 16 x 16 part. The parts go through the wave's share of LDS (packets of a
+  // row in an order that spreads the banks), from where a lane takes 8
+  // consecutive columns: full-width accesses, and one copy of the epilogue's
+  // code.
+  constexpr int kCols = kBN / kWN, kQuads = kCols / 4;
+  constexpr int kShare = 2 * kStage / kWaves;            // bytes of a wave
+  constexpr int kParts = kShare / (16 * kCols * 4) < kMI
+                             ? kShare / (16 * kCols * 4) : kMI;
+  static_assert(kMI % kParts == 0, "whole rounds");
+  all_arrived();
+  char* mine = &lds[0][0] + wave * kShare;
+  for (int round = 0; round < kMI / kParts; ++round) {
+#pragma unroll
+    for (int i = 0; i < kMI; ++i) {
+      if (i / kParts != round) continue;
+      const int r = (i % kParts) * 16 + (lane & 15);
+#pragma unroll
+      for (int j = 0; j < kNI; ++j) {
+        const int q = (j * 4 + (lane >> 4)) ^ (r & (kQuads - 1));
+        *(f32x4*)(mine + (r * kQuads + q) * 16) = acc[i][j];
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+    constexpr int kLanes = kCols / kOut;                 // of one row
+#pragma unroll 1
+    for (int r = lane / kLanes; r < kParts * 16; r += 64 / kLanes) {
+      const int c = lane % kLanes, m = m0 + wm * (kBM / kWM) +
+                                       round * kParts * 16 + r;
+      const int n = n0 + wn * kCols + c * kOut;
+      if (m >= a.m || n >= a.n) continue;
+      float z[kOut];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int q = (c * 2 + h) ^ (r & (kQuads - 1));
+        const f32x4 v = *(const f32x4*)(mine + (r * kQuads + q) * 16);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) z[h * 4 + i] = v[i];
+      }
+      if (a.part != nullptr)
+        store_f32<float, kOut>(
+            a.part + ((long)split * a.m + m) * a.ld_part + n, z);
+      else
+        finish<T>(a.e, m, n, a.n, z);
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// Adds the splits' sums and finishes; one thread has 8 columns of a row.
+template <typename T>
+__global__ __launch_bounds__(256) void join_kernel(LinearProduct a) {
+  const int across = a.ld_part / kOut;
+  const long at = (long)blockIdx.x * 256 + threadIdx.x;
+  if (at >= (long)a.m * across) return;
+  const long m = at / across;
+  const int n = (int)(at % across) * kOut;
+  const float* p = a.part + m * a.ld_part + n;
+  float z[kOut];
+  load_f32<float, kOut>(p, z);
+  for (int s = 1; s < a.splits; ++s) {
+    float t[kOut];
+    load_f32<float, kOut>(p + (long)s * a.m * a.ld_part, t);
+#pragma unroll
+    for (int i = 0; i < kOut; ++i) z[i] += t[i];
+  }
+  finish<T>(a.e, m, n, a.n, z);
+}
+
+// --------------------------------------------------- dz, db and alignment
+
+// dz = dy * slope (slope null: 1) with rows of ld_dz values, zeros past n;
+// part: a row of column sums of the unrounded dz for each blockIdx.y. A
+// thread has 8 columns, 32 threads a row, 8 rows a pass.
+template <typename T>
+__global__ __launch_bounds__(256) void dz_kernel(
+    const T* dy, const T* slope, T* dz, float* part, int m, int n, long ld_dy,
+    int ld_dz, int rows, bool wide) {
+  __shared__ float lds[8][256 + 8];
+  const int c = blockIdx.x * 256 + (threadIdx.x & 31) * 8;
+  const int r0 = blockIdx.y * rows, r1 = r0 + rows < m ? r0 + rows : m;
+  float sum[8] = {};
+  for (int r = r0 + (threadIdx.x >> 5); r < r1; r += 8) {
+    float g[8], s[8];
+    const T* p = dy + r * ld_dy + c;
+    const T* q = slope + (long)r * n + c;
+    if (wide && c < n) {
+      load_f32<T, 8>(p, g);
+      if (slope) load_f32<T, 8>(q, s);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        g[i] = c + i < n ? (float)p[i] : 0.0f;
+        s[i] = slope && c + i < n ? (float)q[i] : 0.0f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (slope) g[i] *= s[i];
+      sum[i] += g[i];
+    }
+    if (dz) {
+      T* o = dz + (long)r * ld_dz + c;
+      if (c + 8 <= ld_dz) {
+        store_f32<T, 8>(o, g);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (c + i < ld_dz) o[i] = (T)g[i];
+      }
+    }
+  }
+  if (part == nullptr) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    lds[threadIdx.x >> 5][(threadIdx.x & 31) * 8 + i] = sum[i];
+  __syncthreads();
+  const int col = blockIdx.x * 256 + threadIdx.x;
+  if (col < n) {
+    float t = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t += lds[i][threadIdx.x];
+    part[(long)blockIdx.y * n + col] = t;
+  }
+}
+
+// Rows of `width` values at any stride -> rows of `ld` values, zeros behind.
+template <typename T>
+__global__ __launch_bounds__(256) void pad_kernel(const T* from, T* to,
+                                                  int rows, int width,
+                                                  long stride, int ld) {
+  const long total = (long)rows * ld;
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total;
+       i += (long)gridDim.x * 256) {
+    const long r = i / ld;
+    const int c = (int)(i % ld);
+    to[i] = c < width ? from[r * stride + c] : (T)0.0f;
+  }
+}
+
+template <typename T, bool kXT, bool kYT>
+void run_tiles(const LinearProduct& a, hipStream_t s) {
+  const unsigned grid = (unsigned)(((a.m + a.tile - 1) / a.tile) *
+                                   ((a.n + a.tile - 1) / a.tile) * a.splits);
+  if (a.tile == 256)
+    product_kernel<T, kXT, kYT, 256, 256, 2, 4><<<grid, 512, 0, s>>>(a);
+  else if (a.tile == 128)
+    product_kernel<T, kXT, kYT, 128, 128, 2, 2><<<grid, 256, 0, s>>>(a);
+  else
+    product_kernel<T, kXT, kYT, 64, 64, 2, 2><<<grid, 256, 0, s>>>(a);
+}
+
+template <typename T>
+hipError_t run_product(const LinearProduct& a, hipStream_t s) {
+  if (a.x_trans) run_tiles<T, true, true>(a, s);
+  else if (a.y_trans) run_tiles<T, false, true>(a, s);
+  else run_tiles<T, false, false>(a, s);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.part == nullptr) return e;
+  const long threads = (long)a.m * (a.ld_part / kOut);
+  join_kernel<T><<<(unsigned)((threads + 255) / 256), 256, 0, s>>>(a);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t run_pad(const void* from, void* to, int rows, int width,
+                   long stride, int ld, hipStream_t s) {
+  const long blocks = ((long)rows * ld + 1023) / 1024;
+  pad_kernel<T><<<(unsigned)(blocks < 65536 ? blocks : 65536), 256, 0, s>>>(
+      (const T*)from, (T*)to, rows, width, stride, ld);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+extern "C" void linear_plan(LinearProduct* a, int type) {
+  const long tiles256 = (long)((a->m + 255) / 256) * ((a->n + 255) / 256);
+  const long tiles128 = (long)((a->m + 127) / 128) * ((a->n + 127) / 128);
+  a->tile = type != kElemF32 && tiles256 >= 192 ? 256
+            : tiles128 >= 16 ? 128 : 64;
+  const long tiles = (long)((a->m + a->tile - 1) / a->tile) *
+                     ((a->n + a->tile - 1) / a->tile);
+  const int per = type == kElemF32 ? 32 : 64;
+  const int steps = a->kx > per ? (a->kx + per - 1) / per : 1;
+  int splits = 1;
+  while (tiles * splits < 256 && steps / (splits * 2) >= 4) splits *= 2;
+  a->steps_per_split = (steps + splits - 1) / splits;
+  a->splits = (steps + a->steps_per_split - 1) / a->steps_per_split;
+  a->ld_part = (a->n + kOut - 1) / kOut * kOut;
+}
+
+extern "C" hipError_t linear_product_launch(const LinearProduct* a, int type,
+                                            hipStream_t s) {
+  switch (type) {
+    case kElemF32: return run_product<float>(*a, s);
+    case kElemBF16: return run_product<bf16_t>(*a, s);
+    default: return run_product<fp16_t>(*a, s);
+  }
+}
+
+extern "C" int linear_dz_strips(int m, int n) {
+  const int across = (n + 255) / 256;
+  int strips = 1024 / across;
+  if (strips > (m + 31) / 32) strips = (m + 31) / 32;
+  return strips < 1 ? 1 : strips;
+}
+
+template <typename T>
+static hipError_t run_dz(const LinearDz& a, hipStream_t s) {
+  const int rows = (a.m + a.strips - 1) / a.strips;
+  const int cols = a.dz && a.ld_dz > a.n ? a.ld_dz : a.n;
+  dz_kernel<T><<<dim3((cols + 255) / 256, a.strips), 256, 0, s>>>(
+      (const T*)a.dy, (const T*)a.slope, (T*)a.dz, a.part, a.m, a.n, a.ld_dy,
+      a.ld_dz, rows, a.wide);
+  return hipGetLastError();
+}
+
+extern "C" hipError_t linear_dz_launch(const LinearDz* a, int type,
+                                       hipStream_t s) {
+  switch (type) {
+    case kElemF32: return run_dz<float>(*a, s);
+    case kElemBF16: return run_dz<bf16_t>(*a, s);
+    default: return run_dz<fp16_t>(*a, s);
+  }
+}
+
+extern "C" hipError_t linear_pad_launch(const void* from, void* to, int rows,
+                                        int width, long stride, int ld,
+                                        int type, hipStream_t s) {
+  switch (type) {
+    case kElemF32: return run_pad<float>(from, to, rows, width, stride, ld, s);
+    case kElemBF16: return run_pad<bf16_t>(from, to, rows, width, stride, ld, s);
+    default: return run_pad<fp16_t>(from, to, rows, width, stride, ld, s);
+  }
+}

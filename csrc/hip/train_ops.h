@@ -39,7 +39,52 @@ struct NormArgs {
   float eps;
 };
 
+enum LinearAct : int { kActNone = 0, kActRelu, kActGelu, kActSilu };
+
+struct LinearEpilogue {
+  const void* bias;        // null: 0
+  const void* residual;    // null: 0
+  void* y;                 // rows of n values
+  void* slope;             // act'(z), rows of n values; null: not wanted
+  long ld_residual;
+  int act;
+  bool wide;               // 8 columns move as one access, and n % 8 == 0
+};
+
+// D[m][n] = sum over k of X(m, k) Y(n, k). Rows of both operands begin at
+// multiples of 16 bytes and their consecutive extent is a whole number of
+// 16 bytes.
+struct LinearProduct {
+  const void *x, *y;
+  long ldx, ldy;           // values between rows in memory
+  bool x_trans, y_trans;   // k is not the consecutive index
+  int m, n;                // of D
+  int ext_x, ext_y;        // of the operands in memory, m and n or padded
+  int kx, ky;              // likewise of k
+  // linear_plan()'s
+  int tile, splits, steps_per_split, ld_part;
+  float* part;             // splits * m * ld_part sums, or null (one split)
+  LinearEpilogue e;
+};
+
+struct LinearDz {
+  const void *dy, *slope;  // slope: null for 1
+  void* dz;                // null: sums alone
+  float* part;             // `strips` rows of n column sums, or null
+  long ld_dy;
+  int m, n, ld_dz, strips;
+  bool wide;               // 8 columns of dy and slope move as one access
+};
+
 extern "C" {
+void linear_plan(LinearProduct*, int type);
+hipError_t linear_product_launch(const LinearProduct*, int type, hipStream_t);
+int linear_dz_strips(int m, int n);
+hipError_t linear_dz_launch(const LinearDz*, int type, hipStream_t);
+// Rows of `width` values -> rows of `ld` values, zeros behind.
+hipError_t linear_pad_launch(const void* from, void* to, int rows, int width,
+                             long stride, int ld, int type, hipStream_t);
+
 hipError_t adamw_launch(const AdamWTensors*, const AdamWScalars*, int type,
                         hipStream_t);
 // Values that one workgroup of the step and of the norm takes.

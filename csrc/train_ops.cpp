@@ -1,5 +1,5 @@
-// PyTorch bindings of the training operators: layer norm, the AdamW step
-// with the gradient norm, and packed 8-bit optimizer states.
+// PyTorch bindings of the training operators: dense layers, layer norm, the
+// AdamW step with the gradient norm, and packed 8-bit optimizer states.
 
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -164,6 +164,228 @@ std::vector<Tensor> layer_norm_bwd(const Tensor& dy, const Tensor& x,
                                want_db ? db.data_ptr() : nullptr, wt,
                                current()),
                "layer_norm backward");
+  }
+  return {dx, dw, db};
+}
+
+// ---------------------------------------------------------- dense layers
+
+// A matrix as the product kernel takes it: rows that begin at multiples of
+// 16 bytes, of a whole number of 16 bytes. `t` is rows of consecutive
+// values; what does not fit is copied with zeros behind each row.
+struct Operand {
+  Tensor held;
+  int rows, width;      // width: in memory, a whole number of 16 bytes
+  long ld;
+  Operand(const Tensor& t, int type, hipStream_t stream) : held(t) {
+    const int64_t per = 16 / t.element_size();
+    rows = (int)t.size(0);
+    width = (int)((t.size(1) + per - 1) / per * per);
+    ld = rows > 1 ? t.stride(0) : std::max<int64_t>(t.stride(0), width);
+    if (rows <= 1) ld = (ld + per - 1) / per * per;
+    if (t.size(1) == width && ld % per == 0 && aligned16(t.data_ptr()))
+      return;
+    held = torch::empty({rows, width}, t.options());
+    ld = width;
+    if (rows > 0 && width > 0)
+      launched(linear_pad_launch(t.data_ptr(), held.data_ptr(), rows,
+                                 (int)t.size(1), t.stride(0), width, type,
+                                 stream),
+               "linear_act");
+  }
+};
+
+// Rows with a stride of their own, never overlapping.
+Tensor as_matrix(const Tensor& t, int64_t rows, int64_t width) {
+  if (t.dim() == 2 && (t.stride(1) == 1 || width <= 1) &&
+      (t.stride(0) >= width || t.size(0) <= 1))
+    return t;
+  return t.contiguous().view({rows, width});
+}
+
+constexpr int64_t kMostRows = 1LL << 30;
+
+// `a` with x, y, the extents and the epilogue set.
+void product(LinearProduct& a, int type, const Tensor& like,
+             hipStream_t stream) {
+  const int64_t row = std::max(a.ldx, a.ldy) * like.element_size();
+  TORCH_CHECK(row * 256 + 128 < (1LL << 31),
+              "linear_act: rows of ", row, " bytes are too far apart");
+  linear_plan(&a, type);
+  Tensor part;
+  if (a.splits > 1) {
+    part = torch::empty({a.splits, a.m, a.ld_part},
+                        like.options().dtype(torch::kFloat));
+    a.part = part.data_ptr<float>();
+  }
+  launched(linear_product_launch(&a, type, stream), "linear_act");
+}
+
+// Returns y and act'(z), which is undefined where not wanted.
+std::vector<Tensor> linear_fwd(const Tensor& x, const Tensor& w,
+                               const std::optional<Tensor>& bias, int64_t act,
+                               const std::optional<Tensor>& residual,
+                               bool want_slope) {
+  const int type = elem_type(x, "linear_act");
+  TORCH_CHECK(x.is_cuda(), "linear_act: x must be on GPU");
+  TORCH_CHECK(x.dim() >= 1 && w.dim() == 2 && w.size(1) == x.size(-1) &&
+                  w.size(0) >= 1,
+              "linear_act: x [..., K] and weight [N, K], N at least 1; got ",
+              x.sizes(), " and ", w.sizes());
+  const int64_t K = x.size(-1), N = w.size(0);
+  auto shape = x.sizes().vec();
+  shape.back() = N;
+  int64_t M = 1;
+  for (size_t i = 0; i + 1 < shape.size(); ++i) M *= shape[i];
+  TORCH_CHECK(M <= kMostRows && N <= kMostRows && K <= kMostRows,
+              "linear_act: more than 2^30 rows or columns");
+  const auto like_x = [&](const Tensor& t, const char* name) {
+    TORCH_CHECK(t.device() == x.device() &&
+                    t.scalar_type() == x.scalar_type(),
+                "linear_act: ", name, " must have x's type and device");
+  };
+  like_x(w, "weight");
+  if (bias) {
+    like_x(*bias, "bias");
+    TORCH_CHECK(bias->dim() == 1 && bias->size(0) == N,
+                "linear_act: bias must be [", N, "]");
+  }
+  if (residual) {
+    like_x(*residual, "residual");
+    TORCH_CHECK(residual->sizes() == at::IntArrayRef(shape),
+                "linear_act: residual must have the output's shape ", shape);
+  }
+  TORCH_CHECK(act >= kActNone && act <= kActSilu, "linear_act: activation");
+  const c10::DeviceGuard guard(x.device());
+  const hipStream_t stream = current();
+  Tensor y = torch::empty(shape, x.options().memory_format(
+                                     at::MemoryFormat::Contiguous));
+  Tensor slope;
+  if (want_slope && act != kActNone) slope = torch::empty_like(y);
+  if (M == 0) return {y, slope};
+
+  const Operand xo(as_matrix(x, M, K), type, stream);
+  const Operand wo(as_matrix(w, N, K), type, stream);
+  Tensor b, r;
+  LinearProduct a{};
+  a.x = xo.held.data_ptr();
+  a.y = wo.held.data_ptr();
+  a.ldx = xo.ld;
+  a.ldy = wo.ld;
+  a.m = a.ext_x = (int)M;
+  a.n = a.ext_y = (int)N;
+  a.kx = a.ky = xo.width;
+  a.e.act = (int)act;
+  a.e.y = y.data_ptr();
+  a.e.slope = slope.defined() ? slope.data_ptr() : nullptr;
+  a.e.wide = N % 8 == 0;
+  if (bias) {
+    b = bias->contiguous();
+    a.e.bias = b.data_ptr();
+    a.e.wide = a.e.wide && aligned16(a.e.bias);
+  }
+  if (residual) {
+    r = as_matrix(*residual, M, N);
+    a.e.residual = r.data_ptr();
+    a.e.ld_residual = M > 1 ? r.stride(0) : N;
+    a.e.wide = a.e.wide && aligned16(a.e.residual) && a.e.ld_residual % 8 == 0;
+  }
+  product(a, type, x, stream);
+  return {y, slope};
+}
+
+// Returns dx, dw, db; undefined where not wanted.
+std::vector<Tensor> linear_bwd(const Tensor& dy,
+                               const std::optional<Tensor>& slope,
+                               const Tensor& x, const Tensor& w, bool want_dx,
+                               bool want_dw, bool want_db) {
+  const int type = elem_type(x, "linear_act");
+  const int64_t K = x.size(-1), N = w.size(0);
+  const int64_t M = K ? x.numel() / K : dy.numel() / N;
+  TORCH_CHECK(dy.numel() == M * N && dy.scalar_type() == x.scalar_type() &&
+                  dy.device() == x.device(),
+              "linear_act: the output's gradient does not match");
+  const c10::DeviceGuard guard(x.device());
+  const hipStream_t stream = current();
+  const auto fresh = x.options().memory_format(at::MemoryFormat::Contiguous);
+  Tensor dx, dw, db;
+  if (want_dx) dx = torch::empty(x.sizes(), fresh);
+  if (want_dw) dw = M && K ? torch::empty({N, K}, fresh)
+                           : torch::zeros({N, K}, fresh);
+  if (want_db) db = M ? torch::empty({N}, fresh) : torch::zeros({N}, fresh);
+  if (M == 0) return {dx, dw, db};
+
+  // dz and the column sums in one pass; without an activation the products
+  // take dy itself where it is aligned for them.
+  const Tensor g = as_matrix(dy, M, N);
+  const int64_t per = 16 / x.element_size();
+  const int64_t Np = (N + per - 1) / per * per;
+  const long ldg = M > 1 ? g.stride(0) : Np;
+  const bool products = want_dx || want_dw;
+  const bool as_is = !slope && N == Np && ldg % per == 0 &&
+                     aligned16(g.data_ptr());
+  Tensor dz = g;
+  long ld_dz = ldg;
+  LinearDz z{};
+  if (products && !as_is) {
+    dz = torch::empty({M, Np}, fresh);
+    ld_dz = Np;
+    z.dz = dz.data_ptr();
+    z.ld_dz = (int)Np;
+  }
+  if (z.dz != nullptr || want_db) {
+    z.dy = g.data_ptr();
+    z.slope = slope ? slope->data_ptr() : nullptr;
+    z.ld_dy = ldg;
+    z.m = (int)M;
+    z.n = (int)N;
+    z.strips = linear_dz_strips(z.m, z.n);
+    z.wide = N % 8 == 0 && ldg % 8 == 0 && aligned16(z.dy);
+    Tensor part;
+    if (want_db) {
+      part = torch::empty({z.strips, N}, x.options().dtype(torch::kFloat));
+      z.part = part.data_ptr<float>();
+    }
+    launched(linear_dz_launch(&z, type, stream), "linear_act backward");
+    if (want_db)
+      launched(sum_rows_launch(z.part, z.strips, (int)N, (int)N,
+                               db.data_ptr(), nullptr, type, stream),
+               "linear_act backward");
+  }
+  if (K == 0) return {dx, dw, db};
+  if (want_dx) {
+    const Operand wo(as_matrix(w, N, K), type, stream);
+    LinearProduct a{};
+    a.x = dz.data_ptr();
+    a.ldx = ld_dz;
+    a.kx = (int)Np;
+    a.m = a.ext_x = (int)M;
+    a.y = wo.held.data_ptr();
+    a.ldy = wo.ld;
+    a.y_trans = true;
+    a.ky = (int)N;
+    a.n = (int)K;
+    a.ext_y = wo.width;
+    a.e.y = dx.data_ptr();
+    a.e.wide = K % 8 == 0;
+    product(a, type, x, stream);
+  }
+  if (want_dw) {
+    const Operand xo(as_matrix(x, M, K), type, stream);
+    LinearProduct a{};
+    a.x = dz.data_ptr();
+    a.ldx = ld_dz;
+    a.x_trans = a.y_trans = true;
+    a.kx = a.ky = (int)M;
+    a.m = (int)N;
+    a.ext_x = (int)Np;
+    a.y = xo.held.data_ptr();
+    a.ldy = xo.ld;
+    a.n = (int)K;
+    a.ext_y = xo.width;
+    a.e.y = dw.data_ptr();
+    a.e.wide = K % 8 == 0;
+    product(a, type, x, stream);
   }
   return {dx, dw, db};
 }
@@ -387,6 +609,9 @@ Tensor unpack_state8(const Tensor& codes, const Tensor& scales,
 }  // namespace
 
 void register_train_ops(pybind11::module_& m) {
+  m.def("linear_fwd", &linear_fwd,
+        "matrix product + bias + activation + residual (CDNA4 MFMA)");
+  m.def("linear_bwd", &linear_bwd, "its gradients (CDNA4 MFMA)");
   m.def("layer_norm_fwd", &layer_norm_fwd, "layer norm forward (CDNA4)");
   m.def("layer_norm_bwd", &layer_norm_bwd, "layer norm backward (CDNA4)");
   m.def("adamw_step", &adamw_step, "AdamW step over many tensors (CDNA4)");

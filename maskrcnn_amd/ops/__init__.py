@@ -13,6 +13,7 @@ from .nms import (  # noqa: F401
 )
 from .fpn_fuse import fpn_fuse  # noqa: F401
 from .conv3x3 import conv3x3_bias_relu, conv3x3_bn_relu  # noqa: F401
+from .linear_act import linear_act  # noqa: F401
 from .layer_norm import layer_norm, LayerNorm  # noqa: F401
 from .adamw import (  # noqa: F401
     adamw_step, grad_norm, pack_state8, unpack_state8,

@@ -1,0 +1,123 @@
+"""Dense layer with bias, activation and residual in one product.
+
+    y = act(x W^T + bias) + residual
+
+GPU: csrc/hip/linear_act.hip, the forward and both gradients' products on
+the matrix cores. CPU: the same formulas in plain torch (the numerics
+oracle).
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+from ._ext import require_ext
+
+ACTIVATIONS = ("none", "relu", "gelu", "silu")
+
+
+def _act_torch(z, act):
+    """The activation and its derivative."""
+    if act == "relu":
+        return z.clamp(min=0), (z > 0).to(z.dtype)
+    if act == "gelu":
+        cdf = 0.5 * (1.0 + torch.erf(z * math.sqrt(0.5)))
+        return z * cdf, cdf + z * torch.exp(-0.5 * z * z) / \
+            math.sqrt(2.0 * math.pi)
+    if act == "silu":
+        s = torch.sigmoid(z)
+        return z * s, s * (1.0 + z * (1.0 - s))
+    return z, torch.ones_like(z)
+
+
+def _fwd_torch(x, weight, bias, act, residual):
+    wide = torch.float64 if x.dtype == torch.float64 else torch.float32
+    z = x.to(wide) @ weight.to(wide).t()
+    if bias is not None:
+        z = z + bias.to(wide)
+    y, slope = _act_torch(z, act)
+    if residual is not None:
+        y = y + residual.to(wide)
+    return y.to(x.dtype), None if act == "none" else slope.to(x.dtype)
+
+
+def _bwd_torch(grad, slope, x, weight):
+    wide = torch.float64 if x.dtype == torch.float64 else torch.float32
+    n, k = weight.shape
+    dz = grad.to(wide).reshape(-1, n)
+    if slope is not None:
+        dz = dz * slope.to(wide).reshape(-1, n)
+    dx = (dz @ weight.to(wide)).reshape(x.shape)
+    dw = dz.t() @ x.to(wide).reshape(dz.shape[0], k)
+    return dx.to(x.dtype), dw.to(x.dtype), dz.sum(0).to(x.dtype)
+
+
+class _LinearActFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act):
+        if x.is_cuda:
+            y, slope = require_ext().linear_fwd(
+                x, weight, bias, ACTIVATIONS.index(act), residual, True)
+        else:
+            y, slope = _fwd_torch(x, weight, bias, act, residual)
+        ctx.save_for_backward(x, weight, slope)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        x, weight, slope = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        if not x.is_cuda:
+            grads = _bwd_torch(grad, slope, x, weight)
+            grads = [g if n else None for g, n in zip(grads, need)]
+        else:
+            grads = require_ext().linear_bwd(grad, slope, x, weight, need[0],
+                                             need[1], need[2])
+        return (*grads, grad if need[3] else None, None)
+
+
+def linear_act(x: torch.Tensor, weight: torch.Tensor,
+               bias: torch.Tensor = None, activation: str = "none",
+               residual: torch.Tensor = None) -> torch.Tensor:
+    """act(x @ weight.T + bias) + residual.
+
+    x: [..., K]; weight: [N, K] (nn.Linear's layout); bias: [N] or None;
+    residual: [..., N] or None. All in one type, float32, bfloat16 or
+    float16, of any strides; sums are in fp32. activation: "none", "relu",
+    "gelu" (by erf) or "silu". Returns a contiguous [..., N] in x's type.
+    In 16 bits the backward rounds act'(z) (ReLU's is exact) and the
+    gradient of z to that type.
+    """
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"linear_act: activation {activation!r}, not one "
+                         f"of {ACTIVATIONS}")
+    if not x.is_cuda:
+        if x.dim() < 1 or weight.dim() != 2 or not weight.shape[0] or \
+                weight.shape[1] != x.shape[-1]:
+            raise RuntimeError(
+                "linear_act: x [..., K] and weight [N, K], N at least 1; "
+                f"got {tuple(x.shape)} and {tuple(weight.shape)}")
+        shape = (*x.shape[:-1], weight.shape[0])
+        for name, t, want in (("weight", weight, weight.shape),
+                              ("bias", bias, shape[-1:]),
+                              ("residual", residual, shape)):
+            if t is None:
+                continue
+            if t.dtype != x.dtype or t.device != x.device:
+                raise RuntimeError(
+                    f"linear_act: {name} must have x's type and device")
+            if tuple(t.shape) != tuple(want):
+                raise RuntimeError(
+                    f"linear_act: {name} must be {list(want)}")
+    if torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad
+            for t in (x, weight, bias, residual)):
+        return _LinearActFn.apply(x, weight, bias, residual, activation)
+    if not x.is_cuda:
+        return _fwd_torch(x, weight, bias, activation, residual)[0]
+    return require_ext().linear_fwd(x, weight, bias,
+                                    ACTIVATIONS.index(activation), residual,
+                                    False)[0]
