@@ -1,13 +1,14 @@
 // Matrix products of dense layers, with bias, activation and residual in the
 // epilogue, and their gradients.
 //
-//   z = x W^T + b      y = act(z) + r      slope = act'(z)
-//   dz = dy slope      dx = dz W           dW = dz^T x      db = sum dz
+//   z = x W^T + b      y = act(z) + r
+//   dz = dy act'(z)    dx = dz W           dW = dz^T x      db = sum dz
 //
-// The derivative is kept for the backward, not z: it is formed where z is
-// still in fp32, so ReLU's is exact in any type and no erf or exp is
-// computed twice; GELU's and SiLU's are rounded once to the tensors' type,
-// like dz, which the matrix cores take in that type.
+// What is kept for the backward, in the tensors' type: ReLU's derivative,
+// taken where z is still in fp32 and so exact; z itself for GELU and SiLU,
+// because z act''(z) stays below 0.32, so that the rounding of z costs the
+// derivative a third of what its own rounding would. dz is rounded once, as
+// the matrix cores take it in that type; db sums it unrounded.
 //
 // All three products are one kernel, D[m][n] = sum_k X(m,k) Y(n,k), where
 // either operand may lie with k consecutive or with its own index
@@ -206,27 +207,32 @@ struct Operand {
 
 // ---------------------------------------------------------------- epilogue
 
-__device__ inline void activate(int act, float z, float& y, float& slope) {
+__device__ inline float activate(int act, float z) {
   switch (act) {
-    case kActRelu:
-      y = z < 0.0f ? 0.0f : z;            // NaN stays
-      slope = z > 0.0f ? 1.0f : 0.0f;
-      break;
-    case kActGelu: {
-      const float cdf = 0.5f * (1.0f + erff(z * 0.70710678f));
-      y = z * cdf;
-      slope = cdf + z * (0.39894228f * __expf(-0.5f * z * z));
-      break;
-    }
+    case kActRelu: return z < 0.0f ? 0.0f : z;             // NaN stays
+    case kActGelu: return z * (0.5f * (1.0f + erff(z * 0.70710678f)));
+    case kActSilu: return z / (1.0f + __expf(-z));
+    default: return z;
+  }
+}
+
+// What the backward needs of z.
+__device__ inline float kept_of(int act, float z) {
+  return act == kActRelu ? (z > 0.0f ? 1.0f : 0.0f) : z;
+}
+
+// act'(z) from that.
+__device__ inline float slope_of(int act, float kept) {
+  const float z = kept;
+  switch (act) {
+    case kActGelu:
+      return 0.5f * (1.0f + erff(z * 0.70710678f)) +
+             z * (0.39894228f * __expf(-0.5f * z * z));
     case kActSilu: {
       const float s = 1.0f / (1.0f + __expf(-z));
-      y = z * s;
-      slope = s * (1.0f + z * (1.0f - s));
-      break;
+      return s * (1.0f + z * (1.0f - s));
     }
-    default:
-      y = z;
-      slope = 1.0f;
+    default: return kept;
   }
 }
 
@@ -236,31 +242,31 @@ constexpr int kOut = 8;       // consecutive columns that a lane finishes
 template <typename T>
 __device__ inline void finish(const LinearEpilogue& e, long m, int n, int N,
                               float (&z)[kOut]) {
-  float s[kOut];
+  float kept[kOut];
   const T* bias = (const T*)e.bias;
   const T* res = (const T*)e.residual + m * e.ld_residual;
   T* out = (T*)e.y + m * (long)N;
-  T* slope = e.slope ? (T*)e.slope + m * (long)N : nullptr;
+  T* keep = e.kept ? (T*)e.kept + m * (long)N : nullptr;
   if (e.wide) {      // then N % 8 == 0
     float b[kOut] = {}, r[kOut] = {};
     if (bias) load_f32<T, kOut>(bias + n, b);
     if (e.residual) load_f32<T, kOut>(res + n, r);
 #pragma unroll
     for (int i = 0; i < kOut; ++i) {
-      activate(e.act, z[i] + b[i], z[i], s[i]);
-      z[i] += r[i];
+      kept[i] = kept_of(e.act, z[i] + b[i]);
+      z[i] = activate(e.act, z[i] + b[i]) + r[i];
     }
     store_f32<T, kOut>(out + n, z);
-    if (slope) store_f32<T, kOut>(slope + n, s);
+    if (keep) store_f32<T, kOut>(keep + n, kept);
     return;
   }
 #pragma unroll
   for (int i = 0; i < kOut; ++i) {
     if (n + i >= N) return;
-    activate(e.act, z[i] + (bias ? (float)bias[n + i] : 0.0f), z[i], s[i]);
-    if (e.residual) z[i] += (float)res[n + i];
-    out[n + i] = (T)z[i];
-    if (slope) slope[n + i] = (T)s[i];
+    const float v = z[i] + (bias ? (float)bias[n + i] : 0.0f);
+    out[n + i] = (T)(activate(e.act, v) +
+                     (e.residual ? (float)res[n + i] : 0.0f));
+    if (keep) keep[n + i] = (T)kept_of(e.act, v);
   }
 }
 
@@ -399,13 +405,13 @@ __global__ __launch_bounds__(256) void join_kernel(LinearProduct a) {
 
 // --------------------------------------------------- dz, db and alignment
 
-// dz = dy * slope (slope null: 1) with rows of ld_dz values, zeros past n;
+// dz = dy act'(z) (kept null: dy) with rows of ld_dz values, zeros past n;
 // part: a row of column sums of the unrounded dz for each blockIdx.y. A
 // thread has 8 columns, 32 threads a row, 8 rows a pass.
 template <typename T>
 __global__ __launch_bounds__(256) void dz_kernel(
-    const T* dy, const T* slope, T* dz, float* part, int m, int n, long ld_dy,
-    int ld_dz, int rows, bool wide) {
+    const T* dy, const T* kept, T* dz, float* part, int m, int n, long ld_dy,
+    int ld_dz, int rows, int act, bool wide) {
   __shared__ float lds[8][256 + 8];
   const int c = blockIdx.x * 256 + (threadIdx.x & 31) * 8;
   const int r0 = blockIdx.y * rows, r1 = r0 + rows < m ? r0 + rows : m;
@@ -413,20 +419,20 @@ __global__ __launch_bounds__(256) void dz_kernel(
   for (int r = r0 + (threadIdx.x >> 5); r < r1; r += 8) {
     float g[8], s[8];
     const T* p = dy + r * ld_dy + c;
-    const T* q = slope + (long)r * n + c;
+    const T* q = kept + (long)r * n + c;
     if (wide && c < n) {
       load_f32<T, 8>(p, g);
-      if (slope) load_f32<T, 8>(q, s);
+      if (kept) load_f32<T, 8>(q, s);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         g[i] = c + i < n ? (float)p[i] : 0.0f;
-        s[i] = slope && c + i < n ? (float)q[i] : 0.0f;
+        s[i] = kept && c + i < n ? (float)q[i] : 0.0f;
       }
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if (slope) g[i] *= s[i];
+      if (kept) g[i] *= slope_of(act, s[i]);
       sum[i] += g[i];
     }
     if (dz) {
@@ -540,8 +546,8 @@ static hipError_t run_dz(const LinearDz& a, hipStream_t s) {
   const int rows = (a.m + a.strips - 1) / a.strips;
   const int cols = a.dz && a.ld_dz > a.n ? a.ld_dz : a.n;
   dz_kernel<T><<<dim3((cols + 255) / 256, a.strips), 256, 0, s>>>(
-      (const T*)a.dy, (const T*)a.slope, (T*)a.dz, a.part, a.m, a.n, a.ld_dy,
-      a.ld_dz, rows, a.wide);
+      (const T*)a.dy, (const T*)a.kept, (T*)a.dz, a.part, a.m, a.n, a.ld_dy,
+      a.ld_dz, rows, a.act, a.wide);
   return hipGetLastError();
 }
 

@@ -45,7 +45,8 @@ struct LinearEpilogue {
   const void* bias;        // null: 0
   const void* residual;    // null: 0
   void* y;                 // rows of n values
-  void* slope;             // act'(z), rows of n values; null: not wanted
+  void* kept;              // for the backward, rows of n values, or null:
+                           // ReLU's derivative, else z
   long ld_residual;
   int act;
   bool wide;               // 8 columns move as one access, and n % 8 == 0
@@ -68,12 +69,12 @@ struct LinearProduct {
 };
 
 struct LinearDz {
-  const void *dy, *slope;  // slope: null for 1
+  const void *dy, *kept;   // kept: of the epilogue, null: no activation
   void* dz;                // null: sums alone
   float* part;             // `strips` rows of n column sums, or null
   long ld_dy;
-  int m, n, ld_dz, strips;
-  bool wide;               // 8 columns of dy and slope move as one access
+  int m, n, ld_dz, strips, act;
+  bool wide;               // 8 columns of dy and kept move as one access
 };
 
 extern "C" {

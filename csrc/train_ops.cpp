@@ -4,6 +4,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
+#include <torch/csrc/autograd/custom_function.h>
 
 #include <algorithm>
 #include <cmath>
@@ -221,11 +222,11 @@ void product(LinearProduct& a, int type, const Tensor& like,
   launched(linear_product_launch(&a, type, stream), "linear_act");
 }
 
-// Returns y and act'(z), which is undefined where not wanted.
+// Returns y and what the backward keeps (undefined where not wanted).
 std::vector<Tensor> linear_fwd(const Tensor& x, const Tensor& w,
                                const std::optional<Tensor>& bias, int64_t act,
                                const std::optional<Tensor>& residual,
-                               bool want_slope) {
+                               bool want_kept) {
   const int type = elem_type(x, "linear_act");
   TORCH_CHECK(x.is_cuda(), "linear_act: x must be on GPU");
   TORCH_CHECK(x.dim() >= 1 && w.dim() == 2 && w.size(1) == x.size(-1) &&
@@ -260,9 +261,9 @@ std::vector<Tensor> linear_fwd(const Tensor& x, const Tensor& w,
   const hipStream_t stream = current();
   Tensor y = torch::empty(shape, x.options().memory_format(
                                      at::MemoryFormat::Contiguous));
-  Tensor slope;
-  if (want_slope && act != kActNone) slope = torch::empty_like(y);
-  if (M == 0) return {y, slope};
+  Tensor kept;
+  if (want_kept && act != kActNone) kept = torch::empty_like(y);
+  if (M == 0) return {y, kept};
 
   const Operand xo(as_matrix(x, M, K), type, stream);
   const Operand wo(as_matrix(w, N, K), type, stream);
@@ -277,7 +278,7 @@ std::vector<Tensor> linear_fwd(const Tensor& x, const Tensor& w,
   a.kx = a.ky = xo.width;
   a.e.act = (int)act;
   a.e.y = y.data_ptr();
-  a.e.slope = slope.defined() ? slope.data_ptr() : nullptr;
+  a.e.kept = kept.defined() ? kept.data_ptr() : nullptr;
   a.e.wide = N % 8 == 0;
   if (bias) {
     b = bias->contiguous();
@@ -291,13 +292,13 @@ std::vector<Tensor> linear_fwd(const Tensor& x, const Tensor& w,
     a.e.wide = a.e.wide && aligned16(a.e.residual) && a.e.ld_residual % 8 == 0;
   }
   product(a, type, x, stream);
-  return {y, slope};
+  return {y, kept};
 }
 
 // Returns dx, dw, db; undefined where not wanted.
 std::vector<Tensor> linear_bwd(const Tensor& dy,
-                               const std::optional<Tensor>& slope,
-                               const Tensor& x, const Tensor& w, bool want_dx,
+                               const Tensor& kept, const Tensor& x,
+                               const Tensor& w, int64_t act, bool want_dx,
                                bool want_dw, bool want_db) {
   const int type = elem_type(x, "linear_act");
   const int64_t K = x.size(-1), N = w.size(0);
@@ -322,7 +323,7 @@ std::vector<Tensor> linear_bwd(const Tensor& dy,
   const int64_t Np = (N + per - 1) / per * per;
   const long ldg = M > 1 ? g.stride(0) : Np;
   const bool products = want_dx || want_dw;
-  const bool as_is = !slope && N == Np && ldg % per == 0 &&
+  const bool as_is = act == kActNone && N == Np && ldg % per == 0 &&
                      aligned16(g.data_ptr());
   Tensor dz = g;
   long ld_dz = ldg;
@@ -335,7 +336,8 @@ std::vector<Tensor> linear_bwd(const Tensor& dy,
   }
   if (z.dz != nullptr || want_db) {
     z.dy = g.data_ptr();
-    z.slope = slope ? slope->data_ptr() : nullptr;
+    z.kept = act == kActNone ? nullptr : kept.data_ptr();
+    z.act = (int)act;
     z.ld_dy = ldg;
     z.m = (int)M;
     z.n = (int)N;
@@ -388,6 +390,93 @@ std::vector<Tensor> linear_bwd(const Tensor& dy,
     product(a, type, x, stream);
   }
   return {dx, dw, db};
+}
+
+// The autograd nodes are in C++: small layers are bound by the host's time.
+class LinearActNode
+    : public torch::autograd::Function<LinearActNode> {
+ public:
+  static Tensor forward(torch::autograd::AutogradContext* ctx,
+                        const Tensor& x, const Tensor& w,
+                        const std::optional<Tensor>& bias,
+                        const std::optional<Tensor>& residual, int64_t act) {
+    auto out = linear_fwd(x, w, bias, act, residual, true);
+    ctx->save_for_backward({x, w, out[1]});
+    // The edges are the given tensors' alone: which there are goes with act.
+    ctx->saved_data["act"] = act | (bias ? 8 : 0) | (residual ? 16 : 0);
+    return out[0];
+  }
+
+  static torch::autograd::variable_list backward(
+      torch::autograd::AutogradContext* ctx,
+      torch::autograd::variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(),
+                "linear_act: its gradients have no gradient (create_graph)");
+    const auto saved = ctx->get_saved_variables();
+    const int64_t act = ctx->saved_data["act"].toInt();
+    const bool bias = act & 8, residual = act & 16;
+    auto g = linear_bwd(grads[0], saved[2], saved[0], saved[1], act & 7,
+                        ctx->needs_input_grad(0), ctx->needs_input_grad(1),
+                        bias && ctx->needs_input_grad(2));
+    const bool dr = residual && ctx->needs_input_grad(bias ? 3 : 2);
+    return {g[0], g[1], g[2], dr ? grads[0] : Tensor(), Tensor()};
+  }
+};
+
+bool wants_grad(const std::optional<Tensor>& t) {
+  return t && t->requires_grad();
+}
+
+Tensor linear_act(const Tensor& x, const Tensor& w,
+                  const std::optional<Tensor>& bias, int64_t act,
+                  const std::optional<Tensor>& residual) {
+  if (at::GradMode::is_enabled() &&
+      (x.requires_grad() || w.requires_grad() || wants_grad(bias) ||
+       wants_grad(residual)))
+    return LinearActNode::apply(x, w, bias, residual, act);
+  return linear_fwd(x, w, bias, act, residual, false)[0];
+}
+
+class LayerNormNode : public torch::autograd::Function<LayerNormNode> {
+ public:
+  static Tensor forward(torch::autograd::AutogradContext* ctx,
+                        const Tensor& x, const std::optional<Tensor>& w,
+                        const std::optional<Tensor>& b, double eps) {
+    auto out = layer_norm_fwd(x, w, b, eps, true);
+    ctx->save_for_backward({x, w ? *w : Tensor(), out[1]});
+    // The edges are the given tensors' alone: which there are goes with the
+    // parameters' type.
+    ctx->saved_data["given"] =
+        (int64_t)(w ? w->scalar_type()
+                    : b ? b->scalar_type() : x.scalar_type()) |
+        (w ? 256 : 0) | (b ? 512 : 0);
+    return out[0];
+  }
+
+  static torch::autograd::variable_list backward(
+      torch::autograd::AutogradContext* ctx,
+      torch::autograd::variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(),
+                "layer_norm: its gradients have no gradient (create_graph)");
+    const auto saved = ctx->get_saved_variables();
+    const int64_t given = ctx->saved_data["given"].toInt();
+    const bool weight = given & 256, bias = given & 512;
+    auto g = layer_norm_bwd(
+        grads[0], saved[0],
+        weight ? std::optional<Tensor>(saved[1]) : std::nullopt,
+        (torch::ScalarType)(given & 255), saved[2], ctx->needs_input_grad(0),
+        weight && ctx->needs_input_grad(1),
+        bias && ctx->needs_input_grad(weight ? 2 : 1));
+    return {g[0], g[1], g[2], Tensor()};
+  }
+};
+
+Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& w,
+                  const std::optional<Tensor>& b, double eps) {
+  if (at::GradMode::is_enabled() &&
+      (x.requires_grad() || wants_grad(w) || wants_grad(b)))
+    return LayerNormNode::apply(x, w, b, eps);
+  return layer_norm_fwd(x, w, b, eps, false)[0];
 }
 
 // ----------------------------------------------------------------- AdamW
@@ -609,11 +698,9 @@ Tensor unpack_state8(const Tensor& codes, const Tensor& scales,
 }  // namespace
 
 void register_train_ops(pybind11::module_& m) {
-  m.def("linear_fwd", &linear_fwd,
+  m.def("linear_act", &linear_act,
         "matrix product + bias + activation + residual (CDNA4 MFMA)");
-  m.def("linear_bwd", &linear_bwd, "its gradients (CDNA4 MFMA)");
-  m.def("layer_norm_fwd", &layer_norm_fwd, "layer norm forward (CDNA4)");
-  m.def("layer_norm_bwd", &layer_norm_bwd, "layer norm backward (CDNA4)");
+  m.def("layer_norm", &layer_norm, "layer norm (CDNA4)");
   m.def("adamw_step", &adamw_step, "AdamW step over many tensors (CDNA4)");
   m.def("grad_norm", &grad_norm, "2-norm over many tensors (CDNA4)");
   m.def("pack_state8", &pack_state8, "fp32 -> 8-bit optimizer state");

@@ -43,11 +43,7 @@ def _bwd_torch(grad, x, weight, wtype, stats):
 class _LayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        if x.is_cuda:
-            y, stats = require_ext().layer_norm_fwd(x, weight, bias, eps,
-                                                    True)
-        else:
-            y, stats = _fwd_torch(x, weight, bias, eps)
+        y, stats = _fwd_torch(x, weight, bias, eps)
         ctx.save_for_backward(x, weight, stats)
         given = weight if weight is not None else bias
         ctx.wtype = given.dtype if given is not None else x.dtype
@@ -57,13 +53,9 @@ class _LayerNormFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         x, weight, stats = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        if not x.is_cuda:
-            grads = _bwd_torch(grad, x, weight, ctx.wtype, stats)
-            return (*(g if n else None for g, n in zip(grads, need)), None)
-        dx, dw, db = require_ext().layer_norm_bwd(
-            grad, x, weight, ctx.wtype, stats, need[0], need[1], need[2])
-        return dx, dw, db, None
+        grads = _bwd_torch(grad, x, weight, ctx.wtype, stats)
+        return (*(g if n else None
+                  for g, n in zip(grads, ctx.needs_input_grad)), None)
 
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor = None,
@@ -74,20 +66,14 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor = None,
     one type. Returns a contiguous tensor of x's shape and type. x may be
     float32, bfloat16 or float16, of any strides.
     """
-    if not x.is_cuda:
-        if x.dim() < 1 or x.shape[-1] < 1:
-            raise RuntimeError("layer_norm: the last dimension is empty")
-        for name, t in (("weight", weight), ("bias", bias)):
-            if t is not None and tuple(t.shape) != (x.shape[-1],):
-                raise RuntimeError(
-                    f"layer_norm: {name} must be [{x.shape[-1]}]")
-    if torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in (x, weight, bias)):
-        return _LayerNormFn.apply(x, weight, bias, float(eps))
-    if not x.is_cuda:
-        return _fwd_torch(x, weight, bias, eps)[0]
-    return require_ext().layer_norm_fwd(x, weight, bias, float(eps),
-                                        False)[0]
+    if x.is_cuda:
+        return require_ext().layer_norm(x, weight, bias, eps)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise RuntimeError("layer_norm: the last dimension is empty")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None and tuple(t.shape) != (x.shape[-1],):
+            raise RuntimeError(f"layer_norm: {name} must be [{x.shape[-1]}]")
+    return _LayerNormFn.apply(x, weight, bias, float(eps))
 
 
 class LayerNorm(nn.Module):

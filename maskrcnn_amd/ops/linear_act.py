@@ -16,6 +16,7 @@ import torch
 from ._ext import require_ext
 
 ACTIVATIONS = ("none", "relu", "gelu", "silu")
+_INDEX = {name: i for i, name in enumerate(ACTIVATIONS)}   # of csrc's enum
 
 
 def _act_torch(z, act):
@@ -40,15 +41,19 @@ def _fwd_torch(x, weight, bias, act, residual):
     y, slope = _act_torch(z, act)
     if residual is not None:
         y = y + residual.to(wide)
-    return y.to(x.dtype), None if act == "none" else slope.to(x.dtype)
+    # For the backward: ReLU's derivative, else z, in x's type.
+    kept = None if act == "none" else \
+        (slope if act == "relu" else z).to(x.dtype)
+    return y.to(x.dtype), kept
 
 
-def _bwd_torch(grad, slope, x, weight):
+def _bwd_torch(grad, kept, x, weight, act):
     wide = torch.float64 if x.dtype == torch.float64 else torch.float32
     n, k = weight.shape
     dz = grad.to(wide).reshape(-1, n)
-    if slope is not None:
-        dz = dz * slope.to(wide).reshape(-1, n)
+    if kept is not None:
+        kept = kept.to(wide).reshape(-1, n)
+        dz = dz * (kept if act == "relu" else _act_torch(kept, act)[1])
     dx = (dz @ weight.to(wide)).reshape(x.shape)
     dw = dz.t() @ x.to(wide).reshape(dz.shape[0], k)
     return dx.to(x.dtype), dw.to(x.dtype), dz.sum(0).to(x.dtype)
@@ -57,26 +62,18 @@ def _bwd_torch(grad, slope, x, weight):
 class _LinearActFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act):
-        if x.is_cuda:
-            y, slope = require_ext().linear_fwd(
-                x, weight, bias, ACTIVATIONS.index(act), residual, True)
-        else:
-            y, slope = _fwd_torch(x, weight, bias, act, residual)
-        ctx.save_for_backward(x, weight, slope)
+        y, kept = _fwd_torch(x, weight, bias, act, residual)
+        ctx.save_for_backward(x, weight, kept)
+        ctx.act = act
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        x, weight, slope = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        if not x.is_cuda:
-            grads = _bwd_torch(grad, slope, x, weight)
-            grads = [g if n else None for g, n in zip(grads, need)]
-        else:
-            grads = require_ext().linear_bwd(grad, slope, x, weight, need[0],
-                                             need[1], need[2])
-        return (*grads, grad if need[3] else None, None)
+        x, weight, kept = ctx.saved_tensors
+        grads = (*_bwd_torch(grad, kept, x, weight, ctx.act), grad)
+        return (*(g if n else None
+                  for g, n in zip(grads, ctx.needs_input_grad)), None)
 
 
 def linear_act(x: torch.Tensor, weight: torch.Tensor,
@@ -88,36 +85,29 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor,
     residual: [..., N] or None. All in one type, float32, bfloat16 or
     float16, of any strides; sums are in fp32. activation: "none", "relu",
     "gelu" (by erf) or "silu". Returns a contiguous [..., N] in x's type.
-    In 16 bits the backward rounds act'(z) (ReLU's is exact) and the
-    gradient of z to that type.
+    In 16 bits z is kept for the backward in that type (ReLU's mask is
+    exact), and its gradient is rounded to it once.
     """
-    if activation not in ACTIVATIONS:
+    act = _INDEX.get(activation)
+    if act is None:
         raise ValueError(f"linear_act: activation {activation!r}, not one "
                          f"of {ACTIVATIONS}")
-    if not x.is_cuda:
-        if x.dim() < 1 or weight.dim() != 2 or not weight.shape[0] or \
-                weight.shape[1] != x.shape[-1]:
+    if x.is_cuda:
+        return require_ext().linear_act(x, weight, bias, act, residual)
+    if x.dim() < 1 or weight.dim() != 2 or not weight.shape[0] or \
+            weight.shape[1] != x.shape[-1]:
+        raise RuntimeError(
+            "linear_act: x [..., K] and weight [N, K], N at least 1; "
+            f"got {tuple(x.shape)} and {tuple(weight.shape)}")
+    shape = (*x.shape[:-1], weight.shape[0])
+    for name, t, want in (("weight", weight, weight.shape),
+                          ("bias", bias, shape[-1:]),
+                          ("residual", residual, shape)):
+        if t is None:
+            continue
+        if t.dtype != x.dtype or t.device != x.device:
             raise RuntimeError(
-                "linear_act: x [..., K] and weight [N, K], N at least 1; "
-                f"got {tuple(x.shape)} and {tuple(weight.shape)}")
-        shape = (*x.shape[:-1], weight.shape[0])
-        for name, t, want in (("weight", weight, weight.shape),
-                              ("bias", bias, shape[-1:]),
-                              ("residual", residual, shape)):
-            if t is None:
-                continue
-            if t.dtype != x.dtype or t.device != x.device:
-                raise RuntimeError(
-                    f"linear_act: {name} must have x's type and device")
-            if tuple(t.shape) != tuple(want):
-                raise RuntimeError(
-                    f"linear_act: {name} must be {list(want)}")
-    if torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad
-            for t in (x, weight, bias, residual)):
-        return _LinearActFn.apply(x, weight, bias, residual, activation)
-    if not x.is_cuda:
-        return _fwd_torch(x, weight, bias, activation, residual)[0]
-    return require_ext().linear_fwd(x, weight, bias,
-                                    ACTIVATIONS.index(activation), residual,
-                                    False)[0]
+                f"linear_act: {name} must have x's type and device")
+        if tuple(t.shape) != tuple(want):
+            raise RuntimeError(f"linear_act: {name} must be {list(want)}")
+    return _LinearActFn.apply(x, weight, bias, residual, activation)
