@@ -17,10 +17,11 @@
 //   dW: X = dz, Y = x (both with their own index consecutive).
 //
 // A workgroup computes a kBM x kBN tile, waves in a grid over it. Each step
-// takes 128 bytes of k from both operands through LDS (two buffers): memory
-// to LDS directly, 16 bytes a lane, the next step's loads in flight during
-// this step's products. The bounds are the buffer descriptor's: rows and
-// columns past the end read as 0. Lanes of one load go to consecutive LDS
+// takes 128 bytes of k from both operands through LDS (three buffers of X and
+// two of Y, all of a CU's LDS with the largest tile): memory to LDS directly,
+// 16 bytes a lane, loads in flight for one to two steps; the next half step's
+// fragments are read from LDS during this half's products. The bounds are the
+// buffer descriptor's: rows and columns past the end read as 0. Lanes of one load go to consecutive LDS
 // addresses, so what would be a column of equal banks is spread by choosing
 // which 16 bytes a lane fetches (an exclusive or with the row's bits).
 // Operands with k consecutive are read from LDS 16 bytes a lane; with 16-bit
@@ -31,6 +32,8 @@
 // Few tiles: the k axis is split, partial sums go to memory in fp32 and a
 // second kernel adds them in order and applies the epilogue.
 #include <hip/hip_runtime.h>
+
+#include <type_traits>
 
 #include "train_ops.h"
 #include "typed.h"
@@ -78,18 +81,20 @@ __device__ inline void load_lds(i32x4 desc, unsigned from, unsigned to) {
       : "memory");
 }
 
-// Every load into LDS has arrived and every read of it is done, in all waves.
-__device__ inline void all_arrived() {
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+// All but the latest kLater loads into LDS have arrived and every read of it
+// is done, in all waves.
+template <int kLater>
+__device__ inline void arrived() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLater)
+               : "memory");
 }
 
-__device__ inline i32x4 descriptor(const char* base, long bytes) {
+__device__ inline i32x4 descriptor(const char* base, int bytes) {
   const unsigned long a = (unsigned long)base;
-  const long range = bytes < 0 ? 0 : bytes < 0x7fffffff ? bytes : 0x7fffffff;
   i32x4 d;
   d[0] = __builtin_amdgcn_readfirstlane((int)a);
   d[1] = __builtin_amdgcn_readfirstlane((int)(a >> 32) & 0xffff);
-  d[2] = __builtin_amdgcn_readfirstlane((int)range);
+  d[2] = bytes;
   d[3] = 0x00020000;
   return d;
 }
@@ -109,10 +114,13 @@ struct Operand {
   static constexpr int kUnits = kPackets / kUnit;
 
   const char* base;     // at the tile's first row, k = 0
-  long ld;              // bytes
-  int extent;           // rows left from the tile's first
+  int ld;               // bytes
+  int rows;             // of this tile
   int k;                // k altogether
   unsigned from[kLoads];
+  int packet[2];        // k consecutive: the packet that a lane fetches in
+                        // even and odd loads
+  static_assert(kLoads % 2 == 0, "even loads for each wave");
 
   static __device__ int twist(int r) {
     if constexpr (!kTrans) return (r >> 1) & 7;
@@ -125,51 +133,49 @@ struct Operand {
 
   __device__ void init(const void* p, long ld_values, int first, int total,
                        int k_total, int wave, int lane) {
-    ld = ld_values * (long)sizeof(T);
+    ld = (int)(ld_values * (long)sizeof(T));
     k = k_total;
-    extent = total - first;
-    base = (const char*)p + (kTrans ? first * (long)sizeof(T) : first * ld);
+    rows = total - first < kR ? total - first : kR;
+    base = (const char*)p + (kTrans ? first * (long)sizeof(T)
+                                    : first * (long)ld);
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int at = (wave * kLoads + i) * 64 + lane;    // packet in LDS
       if constexpr (!kTrans) {
         const int r = at >> 3, c = (at & 7) ^ twist(r);
-        from[i] = (unsigned)(r * (int)ld + c * 16);
+        from[i] = (unsigned)(r * ld + c * 16);
+        packet[i & 1] = c;
       } else {
         const int r = at / kPackets, s = at % kPackets;
         const int c = ((s / kUnit) ^ twist(r)) * kUnit + s % kUnit;
-        from[i] = (unsigned)(r * (int)ld + c * 16);
+        from[i] = (unsigned)(r * ld + c * 16);
       }
     }
   }
 
-  // The step's loads; `to`: LDS address of the tile.
-  __device__ void load(int step, unsigned to, int wave, int lane) const {
-    const int k0 = step * kK;
-    const char* p;
-    long bytes;
-    if constexpr (!kTrans) {
-      p = base + (long)step * kRow;
-      bytes = (extent - 1) * ld + (long)(k - k0) * (long)sizeof(T);
-    } else {
-      p = base + k0 * ld;
-      bytes = (k - k0 - 1) * ld + (long)extent * (long)sizeof(T);
-    }
-    const i32x4 d = descriptor(p, bytes);
-    to += wave * kLoads * 1024;
-    if (!kTrans && k - k0 < kK) {
-      // The last step of a ragged k: packets past it would be the next
-      // row's.
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const int at = (wave * kLoads + i) * 64 + lane;
-        const int c = (at & 7) ^ twist(at >> 3);
-        load_lds(d, c * kPer < k - k0 ? from[i] : kOutside, to + i * 1024);
-      }
-      return;
-    }
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) load_lds(d, from[i], to + i * 1024);
+  struct Step {
+    i32x4 desc;
+    int left;           // k consecutive: packets left in the rows
+  };
+
+  // Step `step`'s part of the operand; from `end` on nothing is in range.
+  __device__ Step at_step(int step, int end) const {
+    const int k0 = step * kK, left = step < end ? k - k0 : 0;
+    if constexpr (!kTrans)
+      return {descriptor(base + (long)step * kRow, (rows - 1) * ld + kRow),
+              left / kPer};
+    const int rows_k = left < kK ? left : kK;
+    return {descriptor(base + (long)k0 * ld,
+                       rows_k > 0 ? (rows_k - 1) * ld + rows * (int)sizeof(T)
+                                  : 0),
+            0};
+  }
+
+  // Load i of the step; `to`: LDS address of the tile. In the last step of
+  // a ragged k the packets past it would be the next row's.
+  __device__ void load(const Step& s, int i, unsigned to, int wave) const {
+    const unsigned f = kTrans || packet[i & 1] < s.left ? from[i] : kOutside;
+    load_lds(s.desc, f, to + (wave * kLoads + i) * 1024);
   }
 
   // The packet of rows r0 + lane % 16 and k-group lane / 16 of half `h`.
@@ -238,62 +244,88 @@ __device__ inline float slope_of(int act, float kept) {
 
 constexpr int kOut = 8;       // consecutive columns that a lane finishes
 
-// Columns n .. n + 7 of row m.
+// The bias of columns n .. n + 7, zeros past N.
 template <typename T>
+__device__ inline void load_bias(const LinearEpilogue& e, int n, int N,
+                                 float (&b)[kOut]) {
+#pragma unroll
+  for (int i = 0; i < kOut; ++i)
+    b[i] = e.bias != nullptr && n + i < N ? (float)((const T*)e.bias)[n + i]
+                                          : 0.0f;
+}
+
+// Columns n .. n + 7 of row m.
+template <typename T, int kAct>
 __device__ inline void finish(const LinearEpilogue& e, long m, int n, int N,
-                              float (&z)[kOut]) {
+                              const float (&b)[kOut], float (&z)[kOut]) {
   float kept[kOut];
-  const T* bias = (const T*)e.bias;
   const T* res = (const T*)e.residual + m * e.ld_residual;
   T* out = (T*)e.y + m * (long)N;
   T* keep = e.kept ? (T*)e.kept + m * (long)N : nullptr;
   if (e.wide) {      // then N % 8 == 0
-    float b[kOut] = {}, r[kOut] = {};
-    if (bias) load_f32<T, kOut>(bias + n, b);
+    float r[kOut] = {};
     if (e.residual) load_f32<T, kOut>(res + n, r);
 #pragma unroll
     for (int i = 0; i < kOut; ++i) {
-      kept[i] = kept_of(e.act, z[i] + b[i]);
-      z[i] = activate(e.act, z[i] + b[i]) + r[i];
+      kept[i] = kept_of(kAct, z[i] + b[i]);
+      z[i] = activate(kAct, z[i] + b[i]) + r[i];
     }
     store_f32<T, kOut>(out + n, z);
-    if (keep) store_f32<T, kOut>(keep + n, kept);
+    if (kAct != kActNone && keep) store_f32<T, kOut>(keep + n, kept);
     return;
   }
 #pragma unroll
   for (int i = 0; i < kOut; ++i) {
     if (n + i >= N) return;
-    const float v = z[i] + (bias ? (float)bias[n + i] : 0.0f);
-    out[n + i] = (T)(activate(e.act, v) +
+    const float v = z[i] + b[i];
+    out[n + i] = (T)(activate(kAct, v) +
                      (e.residual ? (float)res[n + i] : 0.0f));
-    if (keep) keep[n + i] = (T)kept_of(e.act, v);
+    if (kAct != kActNone && keep) keep[n + i] = (T)kept_of(kAct, v);
+  }
+}
+
+// f(the activation as a constant)
+template <typename F>
+__device__ inline void with_act(int act, F f) {
+  switch (act) {
+    case kActRelu: f(std::integral_constant<int, kActRelu>{}); break;
+    case kActGelu: f(std::integral_constant<int, kActGelu>{}); break;
+    case kActSilu: f(std::integral_constant<int, kActSilu>{}); break;
+    default: f(std::integral_constant<int, kActNone>{});
   }
 }
 
 // ------------------------------------------------------------------ kernel
 
+// Two waves a SIMD have 256 registers each, which holds the sums in ordinary
+// ones: with more, the compiler moves hundreds of sums between the two kinds
+// in each step.
 template <typename T, bool kXT, bool kYT, int kBM, int kBN, int kWM, int kWN>
-__global__ __launch_bounds__(kWM * kWN * 64) void product_kernel(
+__global__ __launch_bounds__(kWM * kWN * 64, 2) void product_kernel(
     LinearProduct a) {
   constexpr int kWaves = kWM * kWN;
   using X = Operand<T, kXT, kBM, kWaves>;
   using Y = Operand<T, kYT, kBN, kWaves>;
   constexpr int kMI = kBM / kWM / 16, kNI = kBN / kWN / 16;
-  constexpr int kStage = X::kBytes + Y::kBytes;
-  __shared__ __attribute__((aligned(1024))) char lds[2][kStage];
+  constexpr int kYAt = 3 * X::kBytes, kLds = kYAt + 2 * Y::kBytes;
+  __shared__ __attribute__((aligned(1024))) char lds[kLds];
 
-  // Workgroups go round the 8 chiplets; each gets a consecutive run of
-  // tiles, columns fastest, so that its L2 keeps the rows of X.
+  // Workgroups go round the 8 chiplets; each gets a consecutive run of tiles,
+  // blocks of `group` rows of tiles by all columns, down the rows first, so
+  // that what runs at a time shares rows of X and of Y in the chiplet's L2.
   const int tiles_n = (a.n + kBN - 1) / kBN, tiles_m = (a.m + kBM - 1) / kBM;
   const int total = gridDim.x, xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
   const int big = total >> 3, rest = total & 7;
   const int id = xcd * big + (xcd < rest ? xcd : rest) + at;
   const int split = id / (tiles_m * tiles_n), tile = id % (tiles_m * tiles_n);
-  const int m0 = tile / tiles_n * kBM, n0 = tile % tiles_n * kBN;
+  const int block = tile / (a.group * tiles_n), in = tile % (a.group * tiles_n);
+  const int deep = tiles_m - block * a.group < a.group
+                       ? tiles_m - block * a.group : a.group;
+  const int m0 = (block * a.group + in % deep) * kBM, n0 = in / deep * kBN;
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave / kWN, wn = wave % kWN;
+  const int xr = wave / kWN * (kBM / kWM), yr = wave % kWN * (kBN / kWN);
   X x;
   Y y;
   x.init(a.x, a.ldx, m0, a.ext_x, a.kx, wave, lane);
@@ -303,35 +335,77 @@ __global__ __launch_bounds__(kWM * kWN * 64) void product_kernel(
   const int first = split * a.steps_per_split;
   const int last = first + a.steps_per_split < steps
                        ? first + a.steps_per_split : steps;
-  const unsigned at_lds = (unsigned)(unsigned long)(lds_char*)&lds[0][0];
+  const unsigned at_lds = (unsigned)(unsigned long)(lds_char*)&lds[0];
 
   f32x4 acc[kMI][kNI] = {};
-  x.load(first, at_lds, wave, lane);
-  y.load(first, at_lds + X::kBytes, wave, lane);
+  i32x4 xf[2][kMI], yf[2][kNI];
+  const auto load_x = [&](int step, unsigned to) {
+    const auto s = x.at_step(step, last);
+#pragma unroll
+    for (int i = 0; i < X::kLoads; ++i) x.load(s, i, at_lds + to, wave);
+  };
+  const auto load_y = [&](int step, unsigned to) {
+    const auto s = y.at_step(step, last);
+#pragma unroll
+    for (int i = 0; i < Y::kLoads; ++i) y.load(s, i, at_lds + to, wave);
+  };
+  // Fragment r of a half step: one of X, all of Y, the rest of X, the order
+  // in which the products need them.
+  const auto read = [&](int r, int h, int xat, int yat) {
+    if (r >= 1 && r <= kNI)
+      yf[h][r - 1] = Y::read(lds + yat, yr + (r - 1) * 16, h, lane);
+    else if (r < kMI + kNI)
+      xf[h][r ? r - kNI : 0] =
+          X::read(lds + xat, xr + (r ? r - kNI : 0) * 16, h, lane);
+  };
+
+  // X's buffers: of this step, the next and the one after; Y's: of this step
+  // and the next.
+  int x0 = 0, x1 = X::kBytes, x2 = 2 * X::kBytes;
+  int y0 = kYAt, y1 = kYAt + Y::kBytes;
+  load_x(first, x0);
+  load_y(first, y0);
+  load_x(first + 1, x1);
+  load_y(first + 1, y1);
+  arrived<X::kLoads + Y::kLoads>();
+#pragma unroll
+  for (int r = 0; r < kMI + kNI; ++r) read(r, 0, x0, y0);
+  // A half step: its products, row of fragments by row; the reads of the next
+  // half's fragments, all but the last rows' time ahead of their use; and
+  // loads of a later step, spread evenly, as four at a time on a CU's four
+  // SIMDs would queue. The barrier is in the middle of the step: behind it
+  // the next step has arrived and no wave still reads this one.
+  constexpr int kReads = (kMI + kNI + kMI - 1) / kMI < 2
+                             ? 2 : (kMI + kNI + kMI - 1) / kMI;
   for (int s = first; s < last; ++s) {
-    const int b = (s - first) & 1;
-    all_arrived();
-    if (s + 1 < last) {
-      const unsigned next = at_lds + (b ^ 1) * kStage;
-      x.load(s + 1, next, wave, lane);
-      y.load(s + 1, next + X::kBytes, wave, lane);
+    const auto xs = x.at_step(s + 2, last);
+#pragma unroll
+    for (int i = 0; i < kMI; ++i) {
+#pragma unroll
+      for (int l = i * X::kLoads / kMI; l < (i + 1) * X::kLoads / kMI; ++l)
+        x.load(xs, l, at_lds + x2, wave);
+#pragma unroll
+      for (int r = i * kReads; r < (i + 1) * kReads; ++r) read(r, 1, x0, y0);
+#pragma unroll
+      for (int j = 0; j < kNI; ++j) mma(acc[i][j], yf[0][j], xf[0][i], T{});
+      __builtin_amdgcn_sched_barrier(0);
     }
-    const char* xt = lds[b];
-    const char* yt = lds[b] + X::kBytes;
+    arrived<X::kLoads>();
+    const auto ys = y.at_step(s + 2, last);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      i32x4 xf[kMI], yf[kNI];
+    for (int i = 0; i < kMI; ++i) {
 #pragma unroll
-      for (int i = 0; i < kMI; ++i)
-        xf[i] = X::read(xt, wm * (kBM / kWM) + i * 16, h, lane);
+      for (int l = i * Y::kLoads / kMI; l < (i + 1) * Y::kLoads / kMI; ++l)
+        y.load(ys, l, at_lds + y0, wave);
 #pragma unroll
-      for (int j = 0; j < kNI; ++j)
-        yf[j] = Y::read(yt, wn * (kBN / kWN) + j * 16, h, lane);
+      for (int r = i * kReads; r < (i + 1) * kReads; ++r) read(r, 0, x1, y1);
 #pragma unroll
-      for (int i = 0; i < kMI; ++i)
-#pragma unroll
-        for (int j = 0; j < kNI; ++j) mma(acc[i][j], yf[j], xf[i], T{});
+      for (int j = 0; j < kNI; ++j) mma(acc[i][j], yf[1][j], xf[1][i], T{});
+      __builtin_amdgcn_sched_barrier(0);
     }
+    const int t = x0, u = y0;
+    x0 = x1, x1 = x2, x2 = t;
+    y0 = y1, y1 = u;
   }
 
   // A lane holds row lane % 16 and columns 4 (lane / 16) .. + 3 of each
@@ -340,47 +414,59 @@ __global__ __launch_bounds__(kWM * kWN * 64) void product_kernel(
   // consecutive columns: full-width accesses, and one copy of the epilogue's
   // code.
   constexpr int kCols = kBN / kWN, kQuads = kCols / 4;
-  constexpr int kShare = 2 * kStage / kWaves;            // bytes of a wave
-  constexpr int kParts = kShare / (16 * kCols * 4) < kMI
-                             ? kShare / (16 * kCols * 4) : kMI;
-  static_assert(kMI % kParts == 0, "whole rounds");
-  all_arrived();
-  char* mine = &lds[0][0] + wave * kShare;
-  for (int round = 0; round < kMI / kParts; ++round) {
+  constexpr int kFit = kLds / kWaves / (16 * kCols * 4);   // parts down
+  constexpr int kParts = kFit >= kMI ? kMI : kFit >= kMI / 2 ? kMI / 2
+                                                             : kMI / 4;
+  static_assert(kParts > 0 && kParts <= kFit, "a wave's share of LDS");
+  constexpr int kLanes = kCols / kOut;                     // of one row
+  arrived<0>();
+  char* mine = lds + wave * (kParts * 16 * kCols * 4);
+  const int c = lane % kLanes, n = n0 + yr + c * kOut;
+  const auto rows = [&](auto store) {
 #pragma unroll
-    for (int i = 0; i < kMI; ++i) {
-      if (i / kParts != round) continue;
-      const int r = (i % kParts) * 16 + (lane & 15);
+    for (int round = 0; round < kMI / kParts; ++round) {
 #pragma unroll
-      for (int j = 0; j < kNI; ++j) {
-        const int q = (j * 4 + (lane >> 4)) ^ (r & (kQuads - 1));
-        *(f32x4*)(mine + (r * kQuads + q) * 16) = acc[i][j];
+      for (int i = 0; i < kParts; ++i) {
+        const int r = i * 16 + (lane & 15);
+#pragma unroll
+        for (int j = 0; j < kNI; ++j) {
+          const int q = (j * 4 + (lane >> 4)) ^ (r & (kQuads - 1));
+          *(f32x4*)(mine + (r * kQuads + q) * 16) =
+              acc[round * kParts + i][j];
+        }
       }
-    }
-    __builtin_amdgcn_wave_barrier();
-    constexpr int kLanes = kCols / kOut;                 // of one row
-#pragma unroll 1
-    for (int r = lane / kLanes; r < kParts * 16; r += 64 / kLanes) {
-      const int c = lane % kLanes, m = m0 + wm * (kBM / kWM) +
-                                       round * kParts * 16 + r;
-      const int n = n0 + wn * kCols + c * kOut;
-      if (m >= a.m || n >= a.n) continue;
-      float z[kOut];
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll 2
+      for (int r = lane / kLanes; r < kParts * 16; r += 64 / kLanes) {
+        const int m = m0 + xr + round * kParts * 16 + r;
+        if (m >= a.m || n >= a.n) continue;
+        float z[kOut];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int q = (c * 2 + h) ^ (r & (kQuads - 1));
-        const f32x4 v = *(const f32x4*)(mine + (r * kQuads + q) * 16);
+        for (int h = 0; h < 2; ++h) {
+          const int q = (c * 2 + h) ^ (r & (kQuads - 1));
+          const f32x4 v = *(const f32x4*)(mine + (r * kQuads + q) * 16);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) z[h * 4 + i] = v[i];
+          for (int i = 0; i < 4; ++i) z[h * 4 + i] = v[i];
+        }
+        store(m, z);
       }
-      if (a.part != nullptr)
-        store_f32<float, kOut>(
-            a.part + ((long)split * a.m + m) * a.ld_part + n, z);
-      else
-        finish<T>(a.e, m, n, a.n, z);
+      __builtin_amdgcn_wave_barrier();
     }
-    __builtin_amdgcn_wave_barrier();
+  };
+  if (a.part != nullptr) {
+    rows([&](int m, float (&z)[kOut]) {
+      store_f32<float, kOut>(
+          a.part + ((long)split * a.m + m) * a.ld_part + n, z);
+    });
+    return;
   }
+  float b[kOut];
+  load_bias<T>(a.e, n, a.n, b);
+  with_act(a.e.act, [&](auto act) {
+    rows([&](int m, float (&z)[kOut]) {
+      finish<T, act>(a.e, m, n, a.n, b, z);
+    });
+  });
 }
 
 // Adds the splits' sums and finishes; one thread has 8 columns of a row.
@@ -392,7 +478,8 @@ __global__ __launch_bounds__(256) void join_kernel(LinearProduct a) {
   const long m = at / across;
   const int n = (int)(at % across) * kOut;
   const float* p = a.part + m * a.ld_part + n;
-  float z[kOut];
+  float z[kOut], b[kOut];
+  load_bias<T>(a.e, n, a.n, b);
   load_f32<float, kOut>(p, z);
   for (int s = 1; s < a.splits; ++s) {
     float t[kOut];
@@ -400,7 +487,8 @@ __global__ __launch_bounds__(256) void join_kernel(LinearProduct a) {
 #pragma unroll
     for (int i = 0; i < kOut; ++i) z[i] += t[i];
   }
-  finish<T>(a.e, m, n, a.n, z);
+  with_act(a.e.act,
+           [&](auto act) { finish<T, act>(a.e, m, n, a.n, b, z); });
 }
 
 // --------------------------------------------------- dz, db and alignment
@@ -478,9 +566,13 @@ template <typename T, bool kXT, bool kYT>
 void run_tiles(const LinearProduct& a, hipStream_t s) {
   const unsigned grid = (unsigned)(((a.m + a.tile - 1) / a.tile) *
                                    ((a.n + a.tile - 1) / a.tile) * a.splits);
-  if (a.tile == 256)
-    product_kernel<T, kXT, kYT, 256, 256, 2, 4><<<grid, 512, 0, s>>>(a);
-  else if (a.tile == 128)
+  if constexpr (sizeof(T) == 2) {
+    if (a.tile == 256) {
+      product_kernel<T, kXT, kYT, 256, 256, 2, 4><<<grid, 512, 0, s>>>(a);
+      return;
+    }
+  }
+  if (a.tile == 128)
     product_kernel<T, kXT, kYT, 128, 128, 2, 2><<<grid, 256, 0, s>>>(a);
   else
     product_kernel<T, kXT, kYT, 64, 64, 2, 2><<<grid, 256, 0, s>>>(a);
@@ -512,6 +604,7 @@ hipError_t run_pad(const void* from, void* to, int rows, int width,
 extern "C" void linear_plan(LinearProduct* a, int type) {
   const long tiles256 = (long)((a->m + 255) / 256) * ((a->n + 255) / 256);
   const long tiles128 = (long)((a->m + 127) / 128) * ((a->n + 127) / 128);
+  // fp32 products are bound by their instructions: small tiles do.
   a->tile = type != kElemF32 && tiles256 >= 192 ? 256
             : tiles128 >= 16 ? 128 : 64;
   const long tiles = (long)((a->m + a->tile - 1) / a->tile) *
@@ -522,6 +615,7 @@ extern "C" void linear_plan(LinearProduct* a, int type) {
   while (tiles * splits < 256 && steps / (splits * 2) >= 4) splits *= 2;
   a->steps_per_split = (steps + splits - 1) / splits;
   a->splits = (steps + a->steps_per_split - 1) / a->steps_per_split;
+  a->group = (a->n + a->tile - 1) / a->tile > 4 ? 4 : 1;
   a->ld_part = (a->n + kOut - 1) / kOut * kOut;
 }
 

@@ -63,7 +63,7 @@ struct LinearProduct {
   int ext_x, ext_y;        // of the operands in memory, m and n or padded
   int kx, ky;              // likewise of k
   // linear_plan()'s
-  int tile, splits, steps_per_split, ld_part;
+  int tile, group, splits, steps_per_split, ld_part;
   float* part;             // splits * m * ld_part sums, or null (one split)
   LinearEpilogue e;
 };
