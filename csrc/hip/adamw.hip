@@ -5,9 +5,12 @@
 //   v = b2 v + (1 - b2) (c g)^2
 //   p = p (1 - lr wd) - lr / bc1 * m / (sqrt(v) / sqrt(bc2) + eps)
 //
-// All of it in fp32 with every product and sum rounded by itself (no
-// contraction), so that a plain elementwise program gets the same bits; the
-// scalars are formed in double on the host.
+// All of it in fp32; the scalars are formed in double on the host. Every
+// product and sum of the states is rounded by itself (no contraction), so
+// that a plain elementwise program gets the same states to the bit, and with
+// them the same 8-bit codes. The update's root and quotient are the
+// instructions' (1 unit in the last place each): 3 units of an update that is
+// itself a small part of p, for a fifth of the 8-bit kernel's instructions.
 //
 // 8-bit states: 256 consecutive values of a tensor share a power of two
 // 2^(E-127), the exponent of the largest magnitude among them, kept as one
@@ -37,8 +40,9 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kValues = 4;                       // consecutive, per thread
 constexpr int kPass = kThreads * kValues;        // values of one pass
-constexpr int kPasses = 4;
-constexpr int kChunk = kPass * kPasses;          // values of one workgroup
+constexpr int kPasses = 4;                       // of one workgroup, or 1
+constexpr int kNormPasses = 16;                  // the same of the norm's
+constexpr int kNormChunk = kPass * kNormPasses;
 constexpr int kBlock8 = 256;                     // values sharing a scale
 static_assert(kPass % kBlock8 == 0 && kBlock8 == 64 * kValues,
               "a wave holds one block of an 8-bit state");
@@ -55,7 +59,7 @@ struct Table32 {
   void* v[N];
   long n[N];
   int first[N];     // first workgroup of the tensor
-  int count;
+  int count, passes;
 };
 
 template <int N>
@@ -94,13 +98,22 @@ __device__ inline float clip_factor(const Hyper& h) {
   return c > 1.0f ? 1.0f : c;                    // NaN stays NaN
 }
 
+// The root, 0 and subnormal arguments (which the instruction takes for 0)
+// too.
+__device__ inline float root(float v) {
+  const bool tiny = v < 0x1p-96f;
+  const float s = __builtin_amdgcn_sqrtf(tiny ? v * 0x1p64f : v);
+  return tiny ? s * 0x1p-32f : s;
+}
+
 __device__ inline void update(const Hyper& h, float c, float g, float& p,
                               float& m, float& v) {
 #pragma clang fp contract(off)
   g = g * c;
   m = m * h.beta1 + g * h.one_minus_beta1;
   v = v * h.beta2 + (g * g) * h.one_minus_beta2;
-  const float step = m / (sqrtf(v) * h.inv_bc2 + h.eps);
+  const float step =
+      m * __builtin_amdgcn_rcpf(root(v) * h.inv_bc2 + h.eps);
   p = p * h.decay - step * h.rate;
 }
 
@@ -134,11 +147,19 @@ __device__ inline bool aligned16(const void* a, const void* b, const void* c,
            (unsigned long)d) & 15) == 0;
 }
 
+// Workgroups go through the tensors from the end: the norm, if there is one,
+// has just read the gradients from the beginning, and the last of them are
+// still in the memory-side cache.
+template <typename Table>
+__device__ inline int turned(const Table&) {
+  return gridDim.x - 1 - blockIdx.x;
+}
+
 template <typename T>
 __global__ __launch_bounds__(kThreads) void adamw32_kernel(
     Table32<kTensors32> t, Hyper h) {
-  const int k = find_tensor(t, blockIdx.x);
-  const long at = (long)(blockIdx.x - t.first[k]) * kChunk +
+  const int wg = turned(t), k = find_tensor(t, wg);
+  const long at = (long)(wg - t.first[k]) * t.passes * kPass +
                   threadIdx.x * kValues;
   const long n = t.n[k];
   T* p = static_cast<T*>(t.p[k]);
@@ -147,7 +168,7 @@ __global__ __launch_bounds__(kThreads) void adamw32_kernel(
   float* v = static_cast<float*>(t.v[k]);
   const bool wide = aligned16(p, g, m, v);
   const float c = clip_factor(h);
-  for (int pass = 0; pass < kPasses; ++pass) {
+  for (int pass = 0; pass < t.passes; ++pass) {
     const long i = at + (long)pass * kPass, left = n - i;
     if (left <= 0) return;
     float pf[kValues], gf[kValues], mf[kValues], vf[kValues];
@@ -176,14 +197,21 @@ template <> struct Code8<false> { static constexpr int low = 30, top = 255; };
 
 constexpr int kMinExp = 40;  // keeps 2^(E-127) and every step a normal fp32
 
+// 2^(E - 127), NaN for E = 255.
+__device__ inline float scale8(int e) {
+  return e == 255 ? __int_as_float(0x7fc00000) : pow2_biased(e);
+}
+
+// A code in the place of an fp32 number's exponent and first 3 bits is its
+// value times a power of two, the codes below the smallest normal one being
+// subnormal there too.
 template <bool kSigned>
-__device__ inline float decode8(unsigned code, int e) {
+__device__ inline float decode8(unsigned code, float scale) {
   constexpr int low = Code8<kSigned>::low;
-  const unsigned mag = kSigned ? code & 127u : code;
-  float r = mag >= 8 ? __int_as_float((mag + ((126 - low) << 3)) << 20)
-                     : (float)mag * pow2_biased(127 - low - 3);
-  if (kSigned && code > 127) r = -r;
-  return e == 255 ? __int_as_float(0x7fc00000) : r * pow2_biased(e);
+  const float r =
+      __uint_as_float((kSigned ? code & 127u : code) << 20) *
+      pow2_biased(127 + 126 - low) * scale;
+  return kSigned && code > 127 ? -r : r;
 }
 
 // `inv` = 2^(127 - E).
@@ -192,16 +220,16 @@ __device__ inline unsigned encode8(float x, float inv) {
   constexpr int low = Code8<kSigned>::low;
   const float r = fabsf(x) * inv;
   const int b = __float_as_int(r);
-  int code;
-  if (r >= pow2_biased(127 - low)) {
-    code = ((b + 0x7ffff + ((b >> 20) & 1)) >> 20) - ((126 - low) << 3);
-    code = code > Code8<kSigned>::top ? Code8<kSigned>::top : code;
-  } else {
-    code = (int)rintf(r * pow2_biased(127 + low + 3));
-    if (!kSigned && x > 0.0f && code == 0) code = 1;
+  int code = ((b + 0x7ffff + ((b >> 20) & 1)) >> 20) - ((126 - low) << 3);
+  code = code > Code8<kSigned>::top ? Code8<kSigned>::top : code;
+  const bool small = r < pow2_biased(127 - low);
+  if (__any(small)) {                  // rare but for zeros
+    int c = (int)rintf(r * pow2_biased(127 + low + 3));
+    if (!kSigned && x > 0.0f && c == 0) c = 1;   // also where r is 0
+    code = small ? c : code;
   }
-  if (kSigned && __float_as_int(x) < 0) code |= 128;
-  return (unsigned)code & 255u;
+  if (kSigned) code |= (int)(__float_as_uint(x) >> 24) & 128;
+  return (unsigned)code;
 }
 
 // The block's biased exponent from the largest magnitude's bits: as an
@@ -227,11 +255,12 @@ __device__ inline void store_block8(unsigned char* codes, unsigned char* scale,
                                     long left, bool wide,
                                     const float (&x)[kValues]) {
   const int e = block_exponent(x);
-  const float inv = e == 255 ? 0.0f : pow2_biased(254 - e);
-  unsigned c[kValues];
+  unsigned c[kValues] = {};
+  if (e < 255) {                       // of the whole wave
+    const float inv = __int_as_float(e < 254 ? (254 - e) << 23 : 0x400000);
 #pragma unroll
-  for (int j = 0; j < kValues; ++j)
-    c[j] = e == 255 ? 0u : encode8<kSigned>(x[j], inv);
+    for (int j = 0; j < kValues; ++j) c[j] = encode8<kSigned>(x[j], inv);
+  }
   if (wide && left >= kValues) {
     *reinterpret_cast<unsigned*>(codes) =
         c[0] | (c[1] << 8) | (c[2] << 16) | (c[3] << 24);
@@ -243,54 +272,75 @@ __device__ inline void store_block8(unsigned char* codes, unsigned char* scale,
   if ((threadIdx.x & 63) == 0 && left > 0) *scale = (unsigned char)e;
 }
 
-template <bool kSigned>
-__device__ inline void load_block8(const unsigned char* codes, int e,
-                                   long left, bool wide,
-                                   float (&x)[kValues]) {
-  unsigned c[kValues] = {};
-  if (wide && left >= kValues) {
-    const unsigned w = *reinterpret_cast<const unsigned*>(codes);
-#pragma unroll
-    for (int j = 0; j < kValues; ++j) c[j] = (w >> (8 * j)) & 255u;
-  } else {
-#pragma unroll
-    for (int j = 0; j < kValues; ++j) c[j] = j < left ? codes[j] : 0u;
-  }
+// Four codes as they lie in memory, zeros past the end.
+__device__ inline unsigned load_codes(const unsigned char* codes, long left,
+                                      bool wide) {
+  if (wide && left >= kValues) return *reinterpret_cast<const unsigned*>(codes);
+  unsigned w = 0;
 #pragma unroll
   for (int j = 0; j < kValues; ++j)
-    x[j] = j < left ? decode8<kSigned>(c[j], e) : 0.0f;
+    if (j < left) w |= (unsigned)codes[j] << (8 * j);
+  return w;
 }
 
+template <bool kSigned>
+__device__ inline void decode_block8(unsigned w, int e, float (&x)[kValues]) {
+  const float scale = scale8(e);
+#pragma unroll
+  for (int j = 0; j < kValues; ++j)
+    x[j] = decode8<kSigned>((w >> (8 * j)) & 255u, scale);
+}
+
+// Two passes at a time, so that the loads of both are in flight.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void adamw8_kernel(
     Table8<kTensors8> t, Hyper h) {
-  const int k = find_tensor(t, blockIdx.x);
-  const long at = (long)(blockIdx.x - t.first[k]) * kChunk +
+  constexpr int kDeep = 2;
+  const int wg = turned(t), k = find_tensor(t, wg);
+  const long at = (long)(wg - t.first[k]) * t.passes * kPass +
                   threadIdx.x * kValues;
   const long n = t.n[k];
   T* p = static_cast<T*>(t.p[k]);
   const T* g = static_cast<const T*>(t.g[k]);
   unsigned char* m = static_cast<unsigned char*>(t.m[k]);
   unsigned char* v = static_cast<unsigned char*>(t.v[k]);
+  unsigned char* ms = t.ms[k];
+  unsigned char* vs = t.vs[k];
   const bool wide = aligned16(p, g, m, v);
   const float c = clip_factor(h);
-  for (int pass = 0; pass < kPasses; ++pass) {
-    const long i = at + (long)pass * kPass, left = n - i;
-    const long b = i / kBlock8;
-    if (b * kBlock8 >= n) return;    // the whole wave is past the end
-    float pf[kValues], gf[kValues], mf[kValues], vf[kValues];
-    load4(p + i, left, wide, pf);
-    load4(g + i, left, wide, gf);
-    load_block8<true>(m + i, t.ms[k][b], left, wide, mf);
-    load_block8<false>(v + i, t.vs[k][b], left, wide, vf);
+  for (int pass = 0; pass < t.passes; pass += kDeep) {
+    float pf[kDeep][kValues], gf[kDeep][kValues];
+    unsigned mc[kDeep], vc[kDeep], me[kDeep], ve[kDeep];
 #pragma unroll
-    for (int j = 0; j < kValues; ++j) {
-      update(h, c, gf[j], pf[j], mf[j], vf[j]);
-      if (j >= left) mf[j] = vf[j] = 0.0f;   // no part in the maximum
+    for (int d = 0; d < kDeep; ++d) {
+      const long i = at + (long)(pass + d) * kPass, left = n - i;
+      const long b = i / kBlock8;
+      if (pass + d >= t.passes || b * kBlock8 >= n) continue;
+      load4(p + i, left, wide, pf[d]);
+      load4(g + i, left, wide, gf[d]);
+      mc[d] = load_codes(m + i, left, wide);
+      vc[d] = load_codes(v + i, left, wide);
+      me[d] = ms[b];
+      ve[d] = vs[b];
     }
-    store4(p + i, left, wide, pf);
-    store_block8<true>(m + i, t.ms[k] + b, left, wide, mf);
-    store_block8<false>(v + i, t.vs[k] + b, left, wide, vf);
+#pragma unroll
+    for (int d = 0; d < kDeep; ++d) {
+      const long i = at + (long)(pass + d) * kPass, left = n - i;
+      const long b = i / kBlock8;
+      // A wave is past its end as a whole: it has one block.
+      if (pass + d >= t.passes || b * kBlock8 >= n) return;
+      float mf[kValues], vf[kValues];
+      decode_block8<true>(mc[d], me[d], mf);
+      decode_block8<false>(vc[d], ve[d], vf);
+#pragma unroll
+      for (int j = 0; j < kValues; ++j) {
+        update(h, c, gf[d][j], pf[d][j], mf[j], vf[j]);
+        if (j >= left) mf[j] = vf[j] = 0.0f;   // no part in the maximum
+      }
+      store4(p + i, left, wide, pf[d]);
+      store_block8<true>(m + i, ms + b, left, wide, mf);
+      store_block8<false>(v + i, vs + b, left, wide, vf);
+    }
   }
 }
 
@@ -308,38 +358,64 @@ __global__ __launch_bounds__(kThreads) void pack8_kernel(
   store_block8<kSigned>(codes + i, scales + b, left, wide, f);
 }
 
+// 16 values a thread.
+constexpr int kUnpack = 16;
 template <bool kSigned, typename T>
 __global__ __launch_bounds__(kThreads) void unpack8_kernel(
     const unsigned char* codes, const unsigned char* scales, T* out, long n) {
-  const long i = ((long)blockIdx.x * kThreads + threadIdx.x) * kValues;
-  const long left = n - i;
-  if (left <= 0) return;
-  const bool wide = aligned16(codes, out, nullptr, nullptr);
-  float f[kValues];
-  load_block8<kSigned>(codes + i, scales[i / kBlock8], left, wide, f);
-  store4(out + i, left, wide, f);
+  const long i = ((long)blockIdx.x * kThreads + threadIdx.x) * kUnpack;
+  if (i >= n) return;
+  const float e = scale8(scales[i / kBlock8]);
+  if (i + kUnpack <= n && aligned16(codes, out, nullptr, nullptr)) {
+    const Pack<unsigned, 4> w =
+        *reinterpret_cast<const Pack<unsigned, 4>*>(codes + i);
+    constexpr int kStore = 16 / sizeof(T);       // values of 16 bytes
+    float f[kUnpack];
+#pragma unroll
+    for (int j = 0; j < kUnpack; ++j)
+      f[j] = decode8<kSigned>((w.v[j / 4] >> (8 * (j % 4))) & 255u, e);
+#pragma unroll
+    for (int j = 0; j < kUnpack; j += kStore) {
+      float o[kStore];
+#pragma unroll
+      for (int q = 0; q < kStore; ++q) o[q] = f[j + q];
+      store_f32<T, kStore>(out + i + j, o);
+    }
+    return;
+  }
+  for (int j = 0; j < kUnpack && i + j < n; ++j)
+    out[i + j] = (T)decode8<kSigned>(codes[i + j], e);
 }
 
 // ------------------------------------------------------------------ norm
 
 // Squares are summed in double: memory bound all the same, and the result
 // does not depend on the order to any bit of the fp32 norm that matters.
+// Four loads of a thread are in flight.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void square_sum_kernel(
     TableNorm t, double* partial) {
+  constexpr int kDeep = 4;
+  static_assert(kNormPasses % kDeep == 0, "whole rounds");
   const int k = find_tensor(t, blockIdx.x);
-  const long at = (long)(blockIdx.x - t.first[k]) * kChunk +
+  const long at = (long)(blockIdx.x - t.first[k]) * kNormChunk +
                   threadIdx.x * kValues;
+  const long n = t.n[k];
   const T* g = static_cast<const T*>(t.g[k]);
   const bool wide = ((unsigned long)g & 15) == 0;
   double s = 0.0;
-  for (int pass = 0; pass < kPasses; ++pass) {
-    const long i = at + (long)pass * kPass, left = t.n[k] - i;
-    if (left <= 0) break;
-    float f[kValues];
-    load4(g + i, left, wide, f);
+  for (int pass = 0; pass < kNormPasses; pass += kDeep) {
+    const long i = at + (long)pass * kPass;
+    if (i >= n) break;
+    float f[kDeep][kValues];
 #pragma unroll
-    for (int j = 0; j < kValues; ++j) s += (double)f[j] * (double)f[j];
+    for (int d = 0; d < kDeep; ++d)
+      load4(g + i + d * kPass, n - i - d * kPass, wide, f[d]);
+#pragma unroll
+    for (int d = 0; d < kDeep; ++d)
+#pragma unroll
+      for (int j = 0; j < kValues; ++j)
+        s += (double)f[d][j] * (double)f[d][j];
   }
   for (int d = 32; d >= 1; d >>= 1) s += __shfl_xor(s, d, 64);
   __shared__ double waves[kThreads / 64];
@@ -365,23 +441,26 @@ __global__ __launch_bounds__(1024) void norm_kernel(const double* partial,
   }
 }
 
-int chunks(long n) { return (int)((n + kChunk - 1) / kChunk); }
+int chunks(long n, long each) { return (int)((n + each - 1) / each); }
 
 }  // namespace
 
+// Tensors from .. to - 1; returns the number of workgroups.
 template <typename Table>
-static int fill(Table& t, const AdamWTensors& a, int from, int most) {
+static int fill(Table& t, const AdamWTensors& a, int from, int to,
+                int passes) {
   int wg = 0;
-  t.count = 0;
-  for (int i = from; i < a.count && t.count < most; ++i) {
-    const int k = t.count++;
+  t.count = to - from;
+  t.passes = passes;
+  for (int i = from; i < to; ++i) {
+    const int k = i - from;
     t.p[k] = a.p[i];
     t.g[k] = a.g[i];
     t.m[k] = a.m[i];
     t.v[k] = a.v[i];
     t.n[k] = a.n[i];
     t.first[k] = wg;
-    wg += chunks(a.n[i]);
+    wg += chunks(a.n[i], (long)passes * kPass);
   }
   return wg;
 }
@@ -391,11 +470,17 @@ extern "C" hipError_t adamw_launch(const AdamWTensors* a,
                                    hipStream_t stream) {
   const Hyper h{s->beta1, s->one_minus_beta1, s->beta2, s->one_minus_beta2,
                 s->eps, s->decay, s->rate, s->inv_bc2, s->max_norm, s->norm};
-  for (int from = 0; from < a->count;) {
+  // Four passes a workgroup amortise its search for the tensor; few values
+  // are spread over more workgroups instead.
+  long values = 0;
+  for (int i = 0; i < a->count; ++i) values += a->n[i];
+  const int passes = values >= 1024L * kPasses * kPass ? kPasses : 1;
+  const int most = a->ms == nullptr ? kTensors32 : kTensors8;
+  for (int to = a->count; to > 0;) {
+    const int from = to > most ? to - most : 0;
     if (a->ms == nullptr) {
       Table32<kTensors32> t;
-      const int wg = fill(t, *a, from, kTensors32);
-      from += t.count;
+      const int wg = fill(t, *a, from, to, passes);
       switch (type) {
         case kElemF32: adamw32_kernel<float><<<wg, kThreads, 0, stream>>>(t, h); break;
         case kElemBF16: adamw32_kernel<bf16_t><<<wg, kThreads, 0, stream>>>(t, h); break;
@@ -403,25 +488,25 @@ extern "C" hipError_t adamw_launch(const AdamWTensors* a,
       }
     } else {
       Table8<kTensors8> t;
-      const int wg = fill(t, *a, from, kTensors8);
-      for (int k = 0; k < t.count; ++k) {
-        t.ms[k] = a->ms[from + k];
-        t.vs[k] = a->vs[from + k];
+      const int wg = fill(t, *a, from, to, passes);
+      for (int i = from; i < to; ++i) {
+        t.ms[i - from] = a->ms[i];
+        t.vs[i - from] = a->vs[i];
       }
-      from += t.count;
       switch (type) {
         case kElemF32: adamw8_kernel<float><<<wg, kThreads, 0, stream>>>(t, h); break;
         case kElemBF16: adamw8_kernel<bf16_t><<<wg, kThreads, 0, stream>>>(t, h); break;
         default: adamw8_kernel<fp16_t><<<wg, kThreads, 0, stream>>>(t, h);
       }
     }
+    to = from;
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
   return hipSuccess;
 }
 
-extern "C" int adamw_chunk() { return kChunk; }
+extern "C" int square_sum_chunk() { return kNormChunk; }
 
 extern "C" hipError_t square_sum_launch(const void* const* g, const long* n,
                                         int count, int type, double* partial,
@@ -434,7 +519,7 @@ extern "C" hipError_t square_sum_launch(const void* const* g, const long* n,
       t.g[k] = g[from];
       t.n[k] = n[from];
       t.first[k] = wg;
-      wg += chunks(n[from]);
+      wg += chunks(n[from], kNormChunk);
     }
     switch (type) {
       case kElemF32: square_sum_kernel<float><<<wg, kThreads, 0, stream>>>(t, partial); break;
@@ -468,7 +553,7 @@ extern "C" hipError_t pack8_launch(const float* x, unsigned char* codes,
 template <bool kSigned>
 static void unpack8(const unsigned char* codes, const unsigned char* scales,
                     void* out, long n, int type, hipStream_t stream) {
-  const unsigned wg = (unsigned)((n + kPass - 1) / kPass);
+  const unsigned wg = (unsigned)chunks(n, kUnpack * kThreads);
   switch (type) {
     case kElemF32: unpack8_kernel<kSigned, float><<<wg, kThreads, 0, stream>>>(codes, scales, (float*)out, n); break;
     case kElemBF16: unpack8_kernel<kSigned, bf16_t><<<wg, kThreads, 0, stream>>>(codes, scales, (bf16_t*)out, n); break;

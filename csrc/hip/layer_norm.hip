@@ -125,7 +125,7 @@ __global__ __launch_bounds__(threads_of<kTeam>()) void norm_fwd_kernel(
   }
 }
 
-// `part`: gridDim.x rows of 2 * width sums (dy xh, then dy); null: no
+// `part`: gridDim.x rows of two halves of sums (dy xh, then dy); null: no
 // weight gradients wanted. `dx` may be null too.
 template <typename T, typename W, int kTeam, int kVecs, int kWidth>
 __global__ __launch_bounds__(threads_of<kTeam>()) void norm_bwd_kernel(
@@ -196,14 +196,15 @@ __global__ __launch_bounds__(threads_of<kTeam>()) void norm_bwd_kernel(
     }
   }
   if (part == nullptr) return;
-  part += (long)blockIdx.x * 2 * width;
+  const int pad = norm_part_half(width);
+  part += (long)blockIdx.x * 2 * pad;
   if constexpr (kRows == 1) {
 #pragma unroll
     for (int k = 0; k < kVecs; ++k) {
       const int c = (k * kTeam + lane) * kWidth;
       if (c < width) {
         store_f32<float, kWidth>(part + c, dw[k]);
-        store_f32<float, kWidth>(part + width + c, db[k]);
+        store_f32<float, kWidth>(part + pad + c, db[k]);
       }
     }
   } else {
@@ -225,7 +226,7 @@ __global__ __launch_bounds__(threads_of<kTeam>()) void norm_bwd_kernel(
         b += sums[(kRows + t) * kCols + c];
       }
       part[c] = a;
-      part[width + c] = b;
+      part[pad + c] = b;
     }
   }
 }
@@ -298,36 +299,56 @@ __global__ __launch_bounds__(256) void norm_dw_wide_kernel(
     a += d * (((float)x[row * x_stride + c] - mean[row]) * rstd[row]);
     b += d;
   }
-  part += (long)blockIdx.y * 2 * width;
+  const int pad = norm_part_half(width);
+  part += (long)blockIdx.y * 2 * pad;
   part[c] = a;
-  part[width + c] = b;
+  part[pad + c] = b;
 }
 
 // --------------------------------------------------- partial sums' sum
 
-// part: `count` rows of `width` sums -> out[0:split] and out2[0:width-split]
-// (either may be null). A workgroup takes 32 columns, 8 strips of rows.
+// part: `count` rows of `cols` sums, cols % 4 == 0; columns 0 .. n - 1 go to
+// out, split .. split + n - 1 to out2 (either may be null). A workgroup takes
+// 64 columns, 16 lanes with 4 each; its 64 groups of lanes take every 64th
+// row, four of them in flight. The order of the sums is fixed.
 template <typename W>
-__global__ __launch_bounds__(256) void sum_rows_kernel(
-    const float* part, int count, int width, int split, W* out, W* out2) {
-  __shared__ float lds[8][33];
-  const int col = blockIdx.x * 32 + (threadIdx.x & 31);
-  const int strip = threadIdx.x >> 5;
-  float s = 0.0f;
-  if (col < width)
-    for (int i = strip; i < count; i += 8) s += part[(long)i * width + col];
-  lds[strip][threadIdx.x & 31] = s;
-  __syncthreads();
-  if (strip == 0 && col < width) {
-    s = 0.0f;
+__global__ __launch_bounds__(1024) void sum_rows_kernel(
+    const float* part, int count, int cols, int split, int n, W* out,
+    W* out2) {
+  __shared__ float lds[16][64];
+  const int lane = threadIdx.x & 15, strip = threadIdx.x >> 4;
+  const int col = blockIdx.x * 64 + lane * 4;
+  float s[4] = {};
+  if (col < cols) {
+    for (int i = strip; i < count; i += 256) {
+      float t[4][4] = {};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s += lds[i][threadIdx.x];
-    if (col < split) {
-      if (out != nullptr) out[col] = (W)s;
-    } else if (out2 != nullptr) {
-      out2[col - split] = (W)s;
+      for (int k = 0; k < 4; ++k)
+        if (i + 64 * k < count)
+          load_f32<float, 4>(part + (long)(i + 64 * k) * cols + col, t[k]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[j] += t[k][j];
     }
   }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    s[j] += __shfl_xor(s[j], 16, 64);
+    s[j] += __shfl_xor(s[j], 32, 64);
+  }
+  if ((threadIdx.x & 63) < 16) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) lds[threadIdx.x >> 6][lane * 4 + j] = s[j];
+  }
+  __syncthreads();
+  if (threadIdx.x >= 64) return;
+  float sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) sum += lds[i][threadIdx.x];
+  const int c = blockIdx.x * 64 + threadIdx.x;
+  if (c < n && out != nullptr) out[c] = (W)sum;
+  if (c >= split && c - split < n && out2 != nullptr) out2[c - split] = (W)sum;
 }
 
 }  // namespace
@@ -437,14 +458,14 @@ extern "C" hipError_t layer_norm_bwd_launch(const NormArgs* a, int type,
   return run_norm(*a, type, wtype, true, s);
 }
 
-extern "C" hipError_t sum_rows_launch(const float* part, int count, int width,
-                                      int split, void* out, void* out2,
+extern "C" hipError_t sum_rows_launch(const float* part, int count, int cols,
+                                      int split, int n, void* out, void* out2,
                                       int type, hipStream_t s) {
-  const unsigned grid = (unsigned)((width + 31) / 32);
+  const unsigned grid = (unsigned)((cols + 63) / 64);
   switch (type) {
-    case kElemF32: sum_rows_kernel<float><<<grid, 256, 0, s>>>(part, count, width, split, (float*)out, (float*)out2); break;
-    case kElemBF16: sum_rows_kernel<bf16_t><<<grid, 256, 0, s>>>(part, count, width, split, (bf16_t*)out, (bf16_t*)out2); break;
-    default: sum_rows_kernel<fp16_t><<<grid, 256, 0, s>>>(part, count, width, split, (fp16_t*)out, (fp16_t*)out2);
+    case kElemF32: sum_rows_kernel<float><<<grid, 1024, 0, s>>>(part, count, cols, split, n, (float*)out, (float*)out2); break;
+    case kElemBF16: sum_rows_kernel<bf16_t><<<grid, 1024, 0, s>>>(part, count, cols, split, n, (bf16_t*)out, (bf16_t*)out2); break;
+    default: sum_rows_kernel<fp16_t><<<grid, 1024, 0, s>>>(part, count, cols, split, n, (fp16_t*)out, (fp16_t*)out2);
   }
   return hipGetLastError();
 }

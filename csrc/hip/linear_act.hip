@@ -213,33 +213,62 @@ struct Operand {
 
 // ---------------------------------------------------------------- epilogue
 
-__device__ inline float activate(int act, float z) {
-  switch (act) {
-    case kActRelu: return z < 0.0f ? 0.0f : z;             // NaN stays
-    case kActGelu: return z * (0.5f * (1.0f + erff(z * 0.70710678f)));
-    case kActSilu: return z / (1.0f + __expf(-z));
-    default: return z;
+// The normal distribution at z: its density's exponential and its integral.
+// fp32 tensors take erf; for 16-bit ones the integral is Abramowitz and
+// Stegun's 7.1.26, off by 7.5e-8 at most and a fifth of erf's instructions,
+// which took 10 us of a 25 us forward of 3999x1024x1024.
+template <typename T>
+__device__ inline void normal(float z, float& e, float& cdf) {
+  e = __expf(-0.5f * z * z);
+  if constexpr (sizeof(T) == 4) {
+    cdf = 0.5f * (1.0f + erff(z * 0.70710678f));
+  } else {
+    const float t =
+        __builtin_amdgcn_rcpf(1.0f + 0.3275911f * 0.70710678f * fabsf(z));
+    const float p =
+        t * (0.254829592f +
+             t * (-0.284496736f +
+                  t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+    const float tail = 0.5f * p * e;
+    cdf = z < 0.0f ? tail : 1.0f - tail;
   }
+}
+
+__device__ inline float sigmoid(float z) {
+  return __builtin_amdgcn_rcpf(1.0f + __expf(-z));
+}
+
+template <typename T, int kAct>
+__device__ inline float activate(float z) {
+  if constexpr (kAct == kActRelu) return z < 0.0f ? 0.0f : z;   // NaN stays
+  if constexpr (kAct == kActSilu) return z * sigmoid(z);
+  if constexpr (kAct == kActGelu) {
+    float e, cdf;
+    normal<T>(z, e, cdf);
+    return z * cdf;
+  }
+  return z;
 }
 
 // What the backward needs of z.
-__device__ inline float kept_of(int act, float z) {
-  return act == kActRelu ? (z > 0.0f ? 1.0f : 0.0f) : z;
+template <int kAct>
+__device__ inline float kept_of(float z) {
+  return kAct == kActRelu ? (z > 0.0f ? 1.0f : 0.0f) : z;
 }
 
 // act'(z) from that.
-__device__ inline float slope_of(int act, float kept) {
-  const float z = kept;
-  switch (act) {
-    case kActGelu:
-      return 0.5f * (1.0f + erff(z * 0.70710678f)) +
-             z * (0.39894228f * __expf(-0.5f * z * z));
-    case kActSilu: {
-      const float s = 1.0f / (1.0f + __expf(-z));
-      return s * (1.0f + z * (1.0f - s));
-    }
-    default: return kept;
+template <typename T, int kAct>
+__device__ inline float slope_of(float z) {
+  if constexpr (kAct == kActSilu) {
+    const float s = sigmoid(z);
+    return s * (1.0f + z * (1.0f - s));
   }
+  if constexpr (kAct == kActGelu) {
+    float e, cdf;
+    normal<T>(z, e, cdf);
+    return cdf + z * (0.39894228f * e);
+  }
+  return z;
 }
 
 constexpr int kOut = 8;       // consecutive columns that a lane finishes
@@ -254,39 +283,59 @@ __device__ inline void load_bias(const LinearEpilogue& e, int n, int N,
                                           : 0.0f;
 }
 
-// Columns n .. n + 7 of row m.
+// 8 columns of a row as they lie in memory.
+template <typename T>
+struct Raw {
+  i32x4 q[sizeof(T) * kOut / 16];
+};
+
+// The residual's columns n .. n + 7 of row m, where 8 move as one access.
+template <typename T>
+__device__ inline Raw<T> load_residual(const LinearEpilogue& e, long m,
+                                       int n) {
+  Raw<T> r = {};
+  if (e.residual == nullptr || !e.wide) return r;
+  const i32x4* p =
+      (const i32x4*)((const T*)e.residual + m * e.ld_residual + n);
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(T) * kOut / 16); ++i) r.q[i] = p[i];
+  return r;
+}
+
+// Columns n .. n + 7 of row m; `raw` is load_residual()'s.
 template <typename T, int kAct>
 __device__ inline void finish(const LinearEpilogue& e, long m, int n, int N,
-                              const float (&b)[kOut], float (&z)[kOut]) {
-  float kept[kOut];
-  const T* res = (const T*)e.residual + m * e.ld_residual;
-  T* out = (T*)e.y + m * (long)N;
-  T* keep = e.kept ? (T*)e.kept + m * (long)N : nullptr;
+                              const float (&b)[kOut], Raw<T> raw,
+                              float (&z)[kOut]) {
+  T* out = (T*)e.y + m * (long)N + n;
+  T* keep = e.kept ? (T*)e.kept + m * (long)N + n : nullptr;
   if (e.wide) {      // then N % 8 == 0
-    float r[kOut] = {};
-    if (e.residual) load_f32<T, kOut>(res + n, r);
+    typedef T Res __attribute__((ext_vector_type(kOut)));
+    const Res r = __builtin_bit_cast(Res, raw);
+    float kept[kOut];
 #pragma unroll
     for (int i = 0; i < kOut; ++i) {
-      kept[i] = kept_of(kAct, z[i] + b[i]);
-      z[i] = activate(kAct, z[i] + b[i]) + r[i];
+      kept[i] = kept_of<kAct>(z[i] + b[i]);
+      z[i] = activate<T, kAct>(z[i] + b[i]) + (float)r[i];
     }
-    store_f32<T, kOut>(out + n, z);
-    if (kAct != kActNone && keep) store_f32<T, kOut>(keep + n, kept);
+    store_f32<T, kOut>(out, z);
+    if (kAct != kActNone && keep) store_f32<T, kOut>(keep, kept);
     return;
   }
+  const T* res = (const T*)e.residual + m * e.ld_residual + n;
 #pragma unroll
   for (int i = 0; i < kOut; ++i) {
-    if (n + i >= N) return;
+    if (n + i >= N) continue;
     const float v = z[i] + b[i];
-    out[n + i] = (T)(activate(kAct, v) +
-                     (e.residual ? (float)res[n + i] : 0.0f));
-    if (kAct != kActNone && keep) keep[n + i] = (T)kept_of(kAct, v);
+    out[i] = (T)(activate<T, kAct>(v) +
+                 (e.residual ? (float)res[i] : 0.0f));
+    if (kAct != kActNone && keep) keep[i] = (T)kept_of<kAct>(v);
   }
 }
 
 // f(the activation as a constant)
 template <typename F>
-__device__ inline void with_act(int act, F f) {
+__host__ __device__ inline void with_act(int act, F f) {
   switch (act) {
     case kActRelu: f(std::integral_constant<int, kActRelu>{}); break;
     case kActGelu: f(std::integral_constant<int, kActGelu>{}); break;
@@ -422,7 +471,10 @@ __global__ __launch_bounds__(kWM * kWN * 64, 2) void product_kernel(
   arrived<0>();
   char* mine = lds + wave * (kParts * 16 * kCols * 4);
   const int c = lane % kLanes, n = n0 + yr + c * kOut;
-  const auto rows = [&](auto store) {
+  constexpr int kTurns = kParts * 16 * kLanes / 64;        // of 64 lanes
+  constexpr int kAhead = kTurns < 4 ? kTurns : 4;
+  const int r_of_lane = lane / kLanes;
+  const auto rows = [&](auto fetch, auto store) {
 #pragma unroll
     for (int round = 0; round < kMI / kParts; ++round) {
 #pragma unroll
@@ -436,25 +488,38 @@ __global__ __launch_bounds__(kWM * kWN * 64, 2) void product_kernel(
         }
       }
       __builtin_amdgcn_wave_barrier();
-#pragma unroll 2
-      for (int r = lane / kLanes; r < kParts * 16; r += 64 / kLanes) {
-        const int m = m0 + xr + round * kParts * 16 + r;
-        if (m >= a.m || n >= a.n) continue;
-        float z[kOut];
+#pragma unroll 1
+      for (int t0 = 0; t0 < kTurns; t0 += kAhead) {
+        // What four rows need from memory is in flight before its first use.
+        const int r0 = r_of_lane + t0 * (64 / kLanes);
+        const int first_m = m0 + xr + round * kParts * 16 + r0;
+        decltype(fetch(0)) fetched[kAhead];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int q = (c * 2 + h) ^ (r & (kQuads - 1));
-          const f32x4 v = *(const f32x4*)(mine + (r * kQuads + q) * 16);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) z[h * 4 + i] = v[i];
+        for (int t = 0; t < kAhead; ++t) {
+          const int m = first_m + t * (64 / kLanes);
+          if (m < a.m && n < a.n) fetched[t] = fetch(m);
         }
-        store(m, z);
+#pragma unroll
+        for (int t = 0; t < kAhead; ++t) {
+          const int r = r0 + t * (64 / kLanes);
+          const int m = first_m + t * (64 / kLanes);
+          if (m >= a.m || n >= a.n) continue;
+          float z[kOut];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int q = (c * 2 + h) ^ (r & (kQuads - 1));
+            const f32x4 v = *(const f32x4*)(mine + (r * kQuads + q) * 16);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) z[h * 4 + i] = v[i];
+          }
+          store(m, fetched[t], z);
+        }
       }
       __builtin_amdgcn_wave_barrier();
     }
   };
   if (a.part != nullptr) {
-    rows([&](int m, float (&z)[kOut]) {
+    rows([](int) { return 0; }, [&](int m, int, float (&z)[kOut]) {
       store_f32<float, kOut>(
           a.part + ((long)split * a.m + m) * a.ld_part + n, z);
     });
@@ -463,9 +528,10 @@ __global__ __launch_bounds__(kWM * kWN * 64, 2) void product_kernel(
   float b[kOut];
   load_bias<T>(a.e, n, a.n, b);
   with_act(a.e.act, [&](auto act) {
-    rows([&](int m, float (&z)[kOut]) {
-      finish<T, act>(a.e, m, n, a.n, b, z);
-    });
+    rows([&](int m) { return load_residual<T>(a.e, m, n); },
+         [&](int m, Raw<T> r, float (&z)[kOut]) {
+           finish<T, act>(a.e, m, n, a.n, b, r, z);
+         });
   });
 }
 
@@ -480,7 +546,9 @@ __global__ __launch_bounds__(256) void join_kernel(LinearProduct a) {
   const float* p = a.part + m * a.ld_part + n;
   float z[kOut], b[kOut];
   load_bias<T>(a.e, n, a.n, b);
+  const Raw<T> r = load_residual<T>(a.e, m, n);
   load_f32<float, kOut>(p, z);
+#pragma unroll 4
   for (int s = 1; s < a.splits; ++s) {
     float t[kOut];
     load_f32<float, kOut>(p + (long)s * a.m * a.ld_part, t);
@@ -488,49 +556,64 @@ __global__ __launch_bounds__(256) void join_kernel(LinearProduct a) {
     for (int i = 0; i < kOut; ++i) z[i] += t[i];
   }
   with_act(a.e.act,
-           [&](auto act) { finish<T, act>(a.e, m, n, a.n, b, z); });
+           [&](auto act) { finish<T, act>(a.e, m, n, a.n, b, r, z); });
 }
 
 // --------------------------------------------------- dz, db and alignment
 
-// dz = dy act'(z) (kept null: dy) with rows of ld_dz values, zeros past n;
+// dz = dy act'(z) with rows of ld_dz values, zeros past n;
 // part: a row of column sums of the unrounded dz for each blockIdx.y. A
-// thread has 8 columns, 32 threads a row, 8 rows a pass.
-template <typename T>
+// thread has 8 columns, 32 threads a row; 8 rows at a time four deep, whose
+// loads are all in flight.
+template <typename T, int kAct>
 __global__ __launch_bounds__(256) void dz_kernel(
     const T* dy, const T* kept, T* dz, float* part, int m, int n, long ld_dy,
-    int ld_dz, int rows, int act, bool wide) {
+    int ld_dz, int rows, bool wide) {
+  constexpr int kDeep = 4;
   __shared__ float lds[8][256 + 8];
   const int c = blockIdx.x * 256 + (threadIdx.x & 31) * 8;
   const int r0 = blockIdx.y * rows, r1 = r0 + rows < m ? r0 + rows : m;
   float sum[8] = {};
-  for (int r = r0 + (threadIdx.x >> 5); r < r1; r += 8) {
-    float g[8], s[8];
-    const T* p = dy + r * ld_dy + c;
-    const T* q = kept + (long)r * n + c;
-    if (wide && c < n) {
-      load_f32<T, 8>(p, g);
-      if (kept) load_f32<T, 8>(q, s);
-    } else {
+  for (int r = r0 + (threadIdx.x >> 5); r < r1; r += 8 * kDeep) {
+    float g[kDeep][8], s[kDeep][8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        g[i] = c + i < n ? (float)p[i] : 0.0f;
-        s[i] = kept && c + i < n ? (float)q[i] : 0.0f;
+    for (int d = 0; d < kDeep; ++d) {
+      const int row = r + 8 * d;
+      const T* p = dy + row * ld_dy + c;
+      const T* q = kept + (long)row * n + c;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) g[d][i] = s[d][i] = 0.0f;
+      if (row >= r1) continue;
+      if (wide && c < n) {
+        load_f32<T, 8>(p, g[d]);
+        if (kAct != kActNone) load_f32<T, 8>(q, s[d]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (c + i >= n) continue;
+          g[d][i] = (float)p[i];
+          if (kAct != kActNone) s[d][i] = (float)q[i];
+        }
       }
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (kept) g[i] *= slope_of(act, s[i]);
-      sum[i] += g[i];
-    }
-    if (dz) {
-      T* o = dz + (long)r * ld_dz + c;
-      if (c + 8 <= ld_dz) {
-        store_f32<T, 8>(o, g);
-      } else {
+    for (int d = 0; d < kDeep; ++d) {
+      const int row = r + 8 * d;
+      if (row >= r1) continue;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (c + i < ld_dz) o[i] = (T)g[i];
+      for (int i = 0; i < 8; ++i) {
+        if (kAct != kActNone) g[d][i] *= slope_of<T, kAct>(s[d][i]);
+        sum[i] += g[d][i];
+      }
+      if (dz) {
+        T* o = dz + (long)row * ld_dz + c;
+        if (c + 8 <= ld_dz) {
+          store_f32<T, 8>(o, g[d]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (c + i < ld_dz) o[i] = (T)g[d][i];
+        }
       }
     }
   }
@@ -544,7 +627,7 @@ __global__ __launch_bounds__(256) void dz_kernel(
     float t = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) t += lds[i][threadIdx.x];
-    part[(long)blockIdx.y * n + col] = t;
+    part[(long)blockIdx.y * norm_part_half(n) + col] = t;
   }
 }
 
@@ -609,10 +692,11 @@ hipError_t run_pad(const void* from, void* to, int rows, int width,
 // tiles: 37 us, against 44 with 256-wide tiles in 12 splits and 43 with 3;
 // for 32000 rows 256-wide ones unsplit: 617 us, against 845 with 128.
 extern "C" void linear_plan(LinearProduct* a, int type) {
-  struct Shape { int tile; double step, rest; };
-  static const Shape kHalf[] = {{256, 1.55, 6.0}, {128, 0.55, 2.5},
-                                {64, 0.25, 1.0}};
-  static const Shape kFull[] = {{128, 1.8, 2.5}, {64, 0.5, 1.0}};
+  struct Shape { int tile; double step, alone, rest; };
+  static const Shape kHalf[] = {{256, 1.55, 1.55, 6.0},
+                                {128, 0.55, 0.55, 2.5},
+                                {64, 0.25, 0.40, 1.0}};
+  static const Shape kFull[] = {{128, 1.8, 1.8, 2.5}, {64, 0.5, 0.5, 1.0}};
   const Shape* shapes = type == kElemF32 ? kFull : kHalf;
   const int count = type == kElemF32 ? 2 : 3;
   const int per = type == kElemF32 ? 32 : 64;
@@ -624,9 +708,10 @@ extern "C" void linear_plan(LinearProduct* a, int type) {
     for (int s = 1; s <= 32 && (s == 1 || (s * 2 <= steps && tiles * s <= 2048));
          ++s) {
       const int each = (steps + s - 1) / s;
+      const long rounds = (tiles * s + 255) / 256;
       const double us =
-          (double)((tiles * s + 255) / 256) *
-              (each * shapes[i].step + shapes[i].rest) +
+          rounds * (each * (rounds == 1 ? shapes[i].alone : shapes[i].step) +
+                    shapes[i].rest) +
           (s > 1 ? 3.5 + (double)s * a->m * a->n * 8.0 / 4.5e6 : 0.0);
       if (best == 0.0 || us < best) {
         best = us;
@@ -662,9 +747,12 @@ template <typename T>
 static hipError_t run_dz(const LinearDz& a, hipStream_t s) {
   const int rows = (a.m + a.strips - 1) / a.strips;
   const int cols = a.dz && a.ld_dz > a.n ? a.ld_dz : a.n;
-  dz_kernel<T><<<dim3((cols + 255) / 256, a.strips), 256, 0, s>>>(
-      (const T*)a.dy, (const T*)a.kept, (T*)a.dz, a.part, a.m, a.n, a.ld_dy,
-      a.ld_dz, rows, a.act, a.wide);
+  const auto run = [&](auto act) {
+    dz_kernel<T, act><<<dim3((cols + 255) / 256, a.strips), 256, 0, s>>>(
+        (const T*)a.dy, (const T*)a.kept, (T*)a.dz, a.part, a.m, a.n, a.ld_dy,
+        a.ld_dz, rows, a.wide);
+  };
+  with_act(a.act, run);
   return hipGetLastError();
 }
 

@@ -27,11 +27,16 @@ struct AdamWScalars {
   const float* norm;   // null: no clipping
 };
 
+// Sums of one row of partial sums: the width, a whole number of 16 bytes.
+__host__ __device__ inline int norm_part_half(int width) {
+  return (width + 3) / 4 * 4;
+}
+
 struct NormArgs {
   const void *dy, *x, *w, *b;     // w, b: null for 1 and 0
   void *y, *dx;
   float *mean, *rstd;
-  float* part;         // `parts` rows of 2 * width sums
+  float* part;         // `parts` rows of 2 * norm_part_half(width) sums
   long rows, x_stride, dy_stride;
   int width;
   int parts;           // the backward's grid
@@ -71,7 +76,8 @@ struct LinearProduct {
 struct LinearDz {
   const void *dy, *kept;   // kept: of the epilogue, null: no activation
   void* dz;                // null: sums alone
-  float* part;             // `strips` rows of n column sums, or null
+  float* part;             // `strips` rows of norm_part_half(n) column sums,
+                           // or null
   long ld_dy;
   int m, n, ld_dz, strips, act;
   bool wide;               // 8 columns of dy and kept move as one access
@@ -88,8 +94,8 @@ hipError_t linear_pad_launch(const void* from, void* to, int rows, int width,
 
 hipError_t adamw_launch(const AdamWTensors*, const AdamWScalars*, int type,
                         hipStream_t);
-// Values that one workgroup of the step and of the norm takes.
-int adamw_chunk();
+// Values that one workgroup of square_sum_launch takes.
+int square_sum_chunk();
 // `partial` has a double for every chunk of every tensor.
 hipError_t square_sum_launch(const void* const* g, const long* n, int count,
                              int type, double* partial, hipStream_t);
@@ -108,8 +114,9 @@ hipError_t layer_norm_fwd_launch(const NormArgs*, int type, int wtype,
                                  hipStream_t);
 hipError_t layer_norm_bwd_launch(const NormArgs*, int type, int wtype,
                                  hipStream_t);
-// `count` rows of `width` fp32 sums -> out[0:split], out2[0:width - split];
-// either may be null.
-hipError_t sum_rows_launch(const float* part, int count, int width, int split,
-                           void* out, void* out2, int type, hipStream_t);
+// `count` rows of `cols` fp32 sums, cols % 4 == 0; the sums of columns
+// 0 .. n - 1 go to out, of split .. split + n - 1 to out2; either may be null.
+hipError_t sum_rows_launch(const float* part, int count, int cols, int split,
+                           int n, void* out, void* out2, int type,
+                           hipStream_t);
 }

@@ -152,7 +152,7 @@ std::vector<Tensor> layer_norm_bwd(const Tensor& dy, const Tensor& x,
     a.parts = layer_norm_parts(rows, (int)width, type, a.aligned);
     Tensor part;
     if (want_dw || want_db) {
-      part = torch::empty({a.parts, 2 * width},
+      part = torch::empty({a.parts, 2 * norm_part_half((int)width)},
                           x.options().dtype(torch::kFloat));
       a.part = part.data_ptr<float>();
     }
@@ -160,7 +160,9 @@ std::vector<Tensor> layer_norm_bwd(const Tensor& dy, const Tensor& x,
     launched(layer_norm_bwd_launch(&a, type, wt, current()),
              "layer_norm backward");
     if (a.part != nullptr)
-      launched(sum_rows_launch(a.part, a.parts, (int)(2 * width), (int)width,
+      launched(sum_rows_launch(a.part, a.parts,
+                               2 * norm_part_half((int)width),
+                               norm_part_half((int)width), (int)width,
                                want_dw ? dw.data_ptr() : nullptr,
                                want_db ? db.data_ptr() : nullptr, wt,
                                current()),
@@ -345,13 +347,15 @@ std::vector<Tensor> linear_bwd(const Tensor& dy,
     z.wide = N % 8 == 0 && ldg % 8 == 0 && aligned16(z.dy);
     Tensor part;
     if (want_db) {
-      part = torch::empty({z.strips, N}, x.options().dtype(torch::kFloat));
+      part = torch::empty({z.strips, norm_part_half(z.n)},
+                          x.options().dtype(torch::kFloat));
       z.part = part.data_ptr<float>();
     }
     launched(linear_dz_launch(&z, type, stream), "linear_act backward");
     if (want_db)
-      launched(sum_rows_launch(z.part, z.strips, (int)N, (int)N,
-                               db.data_ptr(), nullptr, type, stream),
+      launched(sum_rows_launch(z.part, z.strips, norm_part_half(z.n),
+                               norm_part_half(z.n), z.n, db.data_ptr(),
+                               nullptr, type, stream),
                "linear_act backward");
   }
   if (K == 0) return {dx, dw, db};
@@ -637,7 +641,7 @@ Tensor grad_norm(const Tensors& g) {
       at[type].push_back(dense.back().data_ptr());
     }
     n[type].push_back(t.numel());
-    parts += (t.numel() + adamw_chunk() - 1) / adamw_chunk();
+    parts += (t.numel() + square_sum_chunk() - 1) / square_sum_chunk();
   }
   const auto opts = torch::TensorOptions().device(device);
   Tensor out = torch::empty({}, opts.dtype(torch::kFloat));
@@ -648,7 +652,7 @@ Tensor grad_norm(const Tensors& g) {
     launched(square_sum_launch(at[type].data(), n[type].data(),
                                (int)at[type].size(), type, next, current()),
              "grad_norm");
-    for (const long k : n[type]) next += (k + adamw_chunk() - 1) / adamw_chunk();
+    for (const long k : n[type]) next += (k + square_sum_chunk() - 1) / square_sum_chunk();
   }
   launched(norm_launch(parts ? partial.data_ptr<double>() : nullptr,
                        (int)parts, out.data_ptr<float>(), current()),

@@ -43,8 +43,9 @@ def _pack_torch(x, signed):
     blocks = bits.view(-1, BLOCK8)
     e = (blocks.amax(1) >> 23).clamp(min=_MIN_EXP) if n else \
         torch.zeros(0, dtype=torch.int32)
-    inv = ((254 - e) << 23).view(torch.float32)
-    inv = torch.where(e == 255, torch.zeros_like(inv), inv)
+    inv = ((254 - e).clamp(min=0) << 23)
+    inv = torch.where(e == 254, torch.full_like(inv, 1 << 22),
+                      inv).view(torch.float32)        # 2^(127 - E)
     r = (flat.abs().view(-1, BLOCK8) * inv[:, None]).view(-1)
     rb = r.view(torch.int32)
     code = ((rb + 0x7FFFF + ((rb >> 20) & 1)) >> 20) - ((126 - low) << 3)
@@ -126,16 +127,13 @@ def grad_norm(tensors) -> torch.Tensor:
 
 
 def _step_torch(p, g, m, v, clip, beta1, beta2, eps, decay, rate, inv_bc2):
-    """One tensor's step; m and v are fp32 and changed in place. The root
-    goes through 64 bits, as torch's own in fp32 on the CPU is not always
-    the nearest."""
+    """One tensor's step; m and v are fp32 and changed in place."""
     gf = g.float()
     if clip is not None:
         gf = gf * clip
     m.copy_(m * beta1 + gf * (1.0 - beta1))
     v.copy_(v * beta2 + (gf * gf) * (1.0 - beta2))
-    p.copy_(p.float() * decay - m /
-            (torch.sqrt(v.double()).float() * inv_bc2 + eps) * rate)
+    p.copy_(p.float() * decay - m / (torch.sqrt(v) * inv_bc2 + eps) * rate)
 
 
 @torch.no_grad()
