@@ -17,11 +17,11 @@
 //   dW: X = dz, Y = x (both with their own index consecutive).
 //
 // A workgroup computes a kBM x kBN tile, waves in a grid over it. Each step
-// takes 128 bytes of k from both operands through LDS (three buffers of X and
-// two of Y, all of a CU's LDS with the largest tile): memory to LDS directly,
-// 16 bytes a lane, loads in flight for one to two steps; the next half step's
-// fragments are read from LDS during this half's products. The bounds are the
-// buffer descriptor's: rows and columns past the end read as 0. Lanes of one load go to consecutive LDS
+// takes 128 bytes of k from both operands through LDS (with the largest tile three
+// buffers of X and two of Y, all of a CU's LDS): memory to LDS directly, 16
+// bytes a lane, loads in flight for one to two steps or more; the next half
+// step's fragments are read from LDS during this half's products. The bounds
+// are the buffer descriptor's: rows and columns past the end read as 0. Lanes of one load go to consecutive LDS
 // addresses, so what would be a column of equal banks is spread by choosing
 // which 16 bytes a lane fetches (an exclusive or with the row's bits).
 // Operands with k consecutive are read from LDS 16 bytes a lane; with 16-bit
@@ -349,14 +349,16 @@ __host__ __device__ inline void with_act(int act, F f) {
 // Two waves a SIMD have 256 registers each, which holds the sums in ordinary
 // ones: with more, the compiler moves hundreds of sums between the two kinds
 // in each step.
-template <typename T, bool kXT, bool kYT, int kBM, int kBN, int kWM, int kWN>
+template <typename T, bool kXT, bool kYT, int kBM, int kBN, int kWM, int kWN,
+          int kAhead>
 __global__ __launch_bounds__(kWM * kWN * 64, 2) void product_kernel(
     LinearProduct a) {
   constexpr int kWaves = kWM * kWN;
   using X = Operand<T, kXT, kBM, kWaves>;
   using Y = Operand<T, kYT, kBN, kWaves>;
   constexpr int kMI = kBM / kWM / 16, kNI = kBN / kWN / 16;
-  constexpr int kYAt = 3 * X::kBytes, kLds = kYAt + 2 * Y::kBytes;
+  constexpr int kYAt = (kAhead + 1) * X::kBytes;
+  constexpr int kLds = kYAt + kAhead * Y::kBytes;
   __shared__ __attribute__((aligned(1024))) char lds[kLds];
 
   // Workgroups go round the 8 chiplets; each gets a consecutive run of tiles,
@@ -408,15 +410,17 @@ __global__ __launch_bounds__(kWM * kWN * 64, 2) void product_kernel(
           X::read(lds + xat, xr + (r ? r - kNI : 0) * 16, h, lane);
   };
 
-  // X's buffers: of this step, the next and the one after; Y's: of this step
-  // and the next.
-  int x0 = 0, x1 = X::kBytes, x2 = 2 * X::kBytes;
-  int y0 = kYAt, y1 = kYAt + Y::kBytes;
-  load_x(first, x0);
-  load_y(first, y0);
-  load_x(first + 1, x1);
-  load_y(first + 1, y1);
-  arrived<X::kLoads + Y::kLoads>();
+  // Loads are kAhead steps ahead, of X in a step's first half into the buffer
+  // of the step before, of Y in its second into this step's own, which all
+  // waves have left by then.
+#pragma unroll
+  for (int d = 0; d < kAhead; ++d) {
+    load_x(first + d, d * X::kBytes);
+    load_y(first + d, kYAt + d * Y::kBytes);
+  }
+  int x0 = 0, x1 = X::kBytes, xw = kAhead * X::kBytes;
+  int y0 = kYAt, y1 = kYAt + (kAhead > 1 ? Y::kBytes : 0);
+  arrived<(kAhead - 1) * (X::kLoads + Y::kLoads)>();
 #pragma unroll
   for (int r = 0; r < kMI + kNI; ++r) read(r, 0, x0, y0);
   // A half step: its products, row of fragments by row; the reads of the next
@@ -427,20 +431,20 @@ __global__ __launch_bounds__(kWM * kWN * 64, 2) void product_kernel(
   constexpr int kReads = (kMI + kNI + kMI - 1) / kMI < 2
                              ? 2 : (kMI + kNI + kMI - 1) / kMI;
   for (int s = first; s < last; ++s) {
-    const auto xs = x.at_step(s + 2, last);
+    const auto xs = x.at_step(s + kAhead, last);
 #pragma unroll
     for (int i = 0; i < kMI; ++i) {
 #pragma unroll
       for (int l = i * X::kLoads / kMI; l < (i + 1) * X::kLoads / kMI; ++l)
-        x.load(xs, l, at_lds + x2, wave);
+        x.load(xs, l, at_lds + xw, wave);
 #pragma unroll
       for (int r = i * kReads; r < (i + 1) * kReads; ++r) read(r, 1, x0, y0);
 #pragma unroll
       for (int j = 0; j < kNI; ++j) mma(acc[i][j], yf[0][j], xf[0][i], T{});
       __builtin_amdgcn_sched_barrier(0);
     }
-    arrived<X::kLoads>();
-    const auto ys = y.at_step(s + 2, last);
+    arrived<(kAhead - 1) * X::kLoads + (kAhead - 2) * Y::kLoads>();
+    const auto ys = y.at_step(s + kAhead, last);
 #pragma unroll
     for (int i = 0; i < kMI; ++i) {
 #pragma unroll
@@ -452,9 +456,9 @@ __global__ __launch_bounds__(kWM * kWN * 64, 2) void product_kernel(
       for (int j = 0; j < kNI; ++j) mma(acc[i][j], yf[1][j], xf[1][i], T{});
       __builtin_amdgcn_sched_barrier(0);
     }
-    const int t = x0, u = y0;
-    x0 = x1, x1 = x2, x2 = t;
-    y0 = y1, y1 = u;
+    xw = x0, x0 = x1, y0 = y1;
+    x1 = x1 + X::kBytes == kYAt ? 0 : x1 + X::kBytes;
+    y1 = y1 + Y::kBytes == kLds ? kYAt : y1 + Y::kBytes;
   }
 
   // A lane holds row lane % 16 and columns 4 (lane / 16) .. + 3 of each
@@ -472,7 +476,7 @@ __global__ __launch_bounds__(kWM * kWN * 64, 2) void product_kernel(
   char* mine = lds + wave * (kParts * 16 * kCols * 4);
   const int c = lane % kLanes, n = n0 + yr + c * kOut;
   constexpr int kTurns = kParts * 16 * kLanes / 64;        // of 64 lanes
-  constexpr int kAhead = kTurns < 4 ? kTurns : 4;
+  constexpr int kFetch = kTurns < 4 ? kTurns : 4;
   const int r_of_lane = lane / kLanes;
   const auto rows = [&](auto fetch, auto store) {
 #pragma unroll
@@ -489,18 +493,18 @@ __global__ __launch_bounds__(kWM * kWN * 64, 2) void product_kernel(
       }
       __builtin_amdgcn_wave_barrier();
 #pragma unroll 1
-      for (int t0 = 0; t0 < kTurns; t0 += kAhead) {
+      for (int t0 = 0; t0 < kTurns; t0 += kFetch) {
         // What four rows need from memory is in flight before its first use.
         const int r0 = r_of_lane + t0 * (64 / kLanes);
         const int first_m = m0 + xr + round * kParts * 16 + r0;
-        decltype(fetch(0)) fetched[kAhead];
+        decltype(fetch(0)) fetched[kFetch];
 #pragma unroll
-        for (int t = 0; t < kAhead; ++t) {
+        for (int t = 0; t < kFetch; ++t) {
           const int m = first_m + t * (64 / kLanes);
           if (m < a.m && n < a.n) fetched[t] = fetch(m);
         }
 #pragma unroll
-        for (int t = 0; t < kAhead; ++t) {
+        for (int t = 0; t < kFetch; ++t) {
           const int r = r0 + t * (64 / kLanes);
           const int m = first_m + t * (64 / kLanes);
           if (m >= a.m || n >= a.n) continue;
@@ -651,14 +655,20 @@ void run_tiles(const LinearProduct& a, hipStream_t s) {
                                    ((a.n + a.tile - 1) / a.tile) * a.splits);
   if constexpr (sizeof(T) == 2) {
     if (a.tile == 256) {
-      product_kernel<T, kXT, kYT, 256, 256, 2, 4><<<grid, 512, 0, s>>>(a);
+      product_kernel<T, kXT, kYT, 256, 256, 2, 4, 2><<<grid, 512, 0, s>>>(a);
       return;
     }
   }
-  if (a.tile == 128)
-    product_kernel<T, kXT, kYT, 128, 128, 2, 2><<<grid, 256, 0, s>>>(a);
+  // A workgroup that has its CU to itself takes more LDS and looks further
+  // ahead; otherwise the others' work covers its waits.
+  if (a.tile == 128 && grid <= 256)
+    product_kernel<T, kXT, kYT, 128, 128, 2, 4, 4><<<grid, 512, 0, s>>>(a);
+  else if (a.tile == 128)
+    product_kernel<T, kXT, kYT, 128, 128, 2, 4, 2><<<grid, 512, 0, s>>>(a);
+  else if (grid <= 256)
+    product_kernel<T, kXT, kYT, 64, 64, 2, 2, 6><<<grid, 256, 0, s>>>(a);
   else
-    product_kernel<T, kXT, kYT, 64, 64, 2, 2><<<grid, 256, 0, s>>>(a);
+    product_kernel<T, kXT, kYT, 64, 64, 2, 2, 2><<<grid, 256, 0, s>>>(a);
 }
 
 template <typename T>
