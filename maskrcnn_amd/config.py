@@ -149,6 +149,16 @@ class Config:
     CHANNELS_LAST = True
     # Use hand-written HIP kernels when on GPU (roi_align / nms / fused ops).
     USE_HIP_KERNELS = True
+    # Optimizer: "sgd" (the reference's), "adamw", or "adamw8" with its
+    # states in 8 bits. AdamW takes LEARNING_RATE, WEIGHT_DECAY (decoupled)
+    # and GRADIENT_CLIP_NORM, and the two below.
+    OPTIMIZER = "sgd"
+    ADAMW_BETAS = (0.9, 0.999)
+    ADAMW_EPS = 1e-8
+    # Norm of the box head's two dense layers: "batch" (the reference's), or
+    # "layer": each layer is linear + ReLU with a layer norm behind it, the
+    # second one residual; it needs no statistics of a pretrained model.
+    CLASSIF_HEAD_NORM = "batch"
 
     def __init__(self):
         """Compute derived attributes (reference config.py:~200)."""

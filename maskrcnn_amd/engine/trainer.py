@@ -1,7 +1,8 @@
 """Training engine.
 
 Replicates the reference training behavior (MaskRCNN.train/compile,
-mrcnn/model.py:~2120-2370): SGD(momentum=0.9, clipnorm=5.0), the five
+mrcnn/model.py:~2120-2370): SGD(momentum=0.9, clipnorm=5.0; AdamW by
+configuration), the five
 weighted losses + L2 weight decay over non-BN weights, layer-freeze
 schedules ('heads'/'3+'/'4+'/'5+'/'all'), per-epoch checkpoints
 (mask_rcnn_{name}_{epoch:04d}.pth) and resume via find_last().
@@ -24,8 +25,10 @@ log = logging.getLogger(__name__)
 
 
 def build_optimizer(model, config, learning_rate):
-    """SGD + momentum; weight decay applied only to conv/linear weights
-    (reference compile() adds L2 over non-BN weight matrices, not biases)."""
+    """config.OPTIMIZER: SGD + momentum, or AdamW with states in 32 or 8
+    bits, which clips the gradients' norm itself. Weight decay is applied
+    only to conv/linear weights (reference compile() adds L2 over non-BN
+    weight matrices, not biases)."""
     # Classify no-decay params by module TYPE (norm layers), not by name
     # substring: BN inside nn.Sequential heads is named convs.1 etc. and
     # a name check would wrongly decay its gamma/beta.
@@ -33,7 +36,8 @@ def build_optimizer(model, config, learning_rate):
                   torch.nn.GroupNorm, torch.nn.LayerNorm)
     try:
         from ..model.resnet import FrozenBatchNorm2d
-        norm_types = norm_types + (FrozenBatchNorm2d,)
+        from ..ops import LayerNorm
+        norm_types = norm_types + (FrozenBatchNorm2d, LayerNorm)
     except ImportError:
         pass
     norm_param_ids = set()
@@ -48,10 +52,19 @@ def build_optimizer(model, config, learning_rate):
             no_decay.append(p)
         else:
             decay.append(p)
-    return torch.optim.SGD(
-        [{"params": decay, "weight_decay": config.WEIGHT_DECAY},
-         {"params": no_decay, "weight_decay": 0.0}],
-        lr=learning_rate, momentum=config.LEARNING_MOMENTUM)
+    groups = [{"params": decay, "weight_decay": config.WEIGHT_DECAY},
+              {"params": no_decay, "weight_decay": 0.0}]
+    if config.OPTIMIZER == "sgd":
+        return torch.optim.SGD(groups, lr=learning_rate,
+                               momentum=config.LEARNING_MOMENTUM)
+    if config.OPTIMIZER not in ("adamw", "adamw8"):
+        raise ValueError(f"OPTIMIZER {config.OPTIMIZER!r}: sgd, adamw or "
+                         "adamw8")
+    from .optim import AdamW
+    return AdamW(groups, lr=learning_rate, betas=config.ADAMW_BETAS,
+                 eps=config.ADAMW_EPS,
+                 state_bits=8 if config.OPTIMIZER == "adamw8" else 32,
+                 max_grad_norm=config.GRADIENT_CLIP_NORM)
 
 
 class Trainer:
@@ -120,9 +133,10 @@ class Trainer:
         losses["total_loss"].backward()
         if self.ddp is not None:
             self.ddp.finalize_backward()
-        torch.nn.utils.clip_grad_norm_(
-            (p for p in self.model.parameters() if p.requires_grad),
-            self.config.GRADIENT_CLIP_NORM)
+        if getattr(optimizer, "max_grad_norm", None) is None:
+            torch.nn.utils.clip_grad_norm_(
+                (p for p in self.model.parameters() if p.requires_grad),
+                self.config.GRADIENT_CLIP_NORM)
         optimizer.step()
         return {k: float(v.detach()) for k, v in losses.items()}
 
@@ -253,17 +267,17 @@ class Trainer:
                 # saved weights only; SGD momentum + epoch make resume
                 # exact). Latest-only: overwritten each epoch.
                 torch.save({"optimizer": optimizer.state_dict(),
-                            "epoch": epoch},
+                            "kind": cfg.OPTIMIZER, "epoch": epoch},
                            os.path.join(self.wrapper.log_dir,
                                         "train_state.pth"))
             self.wrapper.epoch += 1
         return self.history
 
     def _maybe_resume_optimizer(self, optimizer) -> bool:
-        """Restore SGD momentum when resuming (find_last/set_log_dir set
-        wrapper.epoch > 0 and the matching train_state.pth is present).
+        """Restore the optimizer's state when resuming (find_last/set_log_dir
+        set wrapper.epoch > 0 and the matching train_state.pth is present).
         Param-group mismatch (different frozen set) is non-fatal: log
-        and train with fresh momentum."""
+        and train with a fresh state."""
         if self.wrapper.epoch == 0:
             return False
         path = os.path.join(self.wrapper.log_dir, "train_state.pth")
@@ -276,6 +290,11 @@ class Trainer:
                 log.warning("train_state.pth is for epoch %s, resuming "
                             "at %d: skipping optimizer restore",
                             state.get("epoch"), self.wrapper.epoch)
+                return False
+            if state.get("kind", "sgd") != self.config.OPTIMIZER:
+                log.warning("train_state.pth is of optimizer %s, not %s: "
+                            "skipping optimizer restore",
+                            state.get("kind", "sgd"), self.config.OPTIMIZER)
                 return False
             optimizer.load_state_dict(state["optimizer"])
             log.info("restored optimizer state from %s", path)

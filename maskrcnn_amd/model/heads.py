@@ -8,6 +8,10 @@ conv 1x1 -> 1024 + BN -> class logits / softmax + per-class bbox deltas.
 
 Mask: PyramidROIAlign(14x14) -> 4x (3x3 conv 256 + BN + ReLU) ->
 deconv 2x2/2 -> 1x1 conv num_classes + sigmoid -> [B, R, C, 28, 28].
+
+With config.CLASSIF_HEAD_NORM = "layer" the classifier's two dense layers are
+LN(ReLU(x W1 + b1)) and LN(ReLU(h W2 + b2) + h), on the fused dense layer and
+layer norm of maskrcnn_amd.ops; this has no counterpart in the reference.
 """
 
 from __future__ import annotations
@@ -16,6 +20,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from ..ops import LayerNorm, linear_act
 from .resnet import make_norm
 from .roialign import PyramidROIAlign
 
@@ -30,10 +35,20 @@ class FPNClassifierHead(nn.Module):
         self.roi_align = PyramidROIAlign(pool, config.IMAGE_SHAPE,
                                          mode="crop_and_resize")
         # 7x7 conv with VALID padding == fully-connected over the pooled tile.
+        norm = config.CLASSIF_HEAD_NORM
+        if norm not in ("batch", "layer"):
+            raise ValueError(f"CLASSIF_HEAD_NORM {norm!r}: batch or layer")
+        self.layer_norm = norm == "layer"
         self.mrcnn_class_conv1 = nn.Conv2d(in_channels, fc, pool)
-        self.mrcnn_class_bn1 = make_norm(fc, train_bn)
+        if self.layer_norm:
+            self.mrcnn_class_ln1 = LayerNorm(fc)
+        else:
+            self.mrcnn_class_bn1 = make_norm(fc, train_bn)
         self.mrcnn_class_conv2 = nn.Conv2d(fc, fc, 1)
-        self.mrcnn_class_bn2 = make_norm(fc, train_bn)
+        if self.layer_norm:
+            self.mrcnn_class_ln2 = LayerNorm(fc)
+        else:
+            self.mrcnn_class_bn2 = make_norm(fc, train_bn)
         self.mrcnn_class_logits = nn.Linear(fc, nc)
         self.mrcnn_bbox_fc = nn.Linear(fc, nc * 4)
         self.num_classes = nc
@@ -48,6 +63,11 @@ class FPNClassifierHead(nn.Module):
         """
         B, N, _ = rois.shape
         x = self.roi_align(rois, feature_maps)           # [B*N,256,7,7]
+        if self.layer_norm:
+            logits, bbox = self._dense_layers(x)
+            probs = F.softmax(logits, dim=-1)
+            return (logits.reshape(B, N, -1), probs.reshape(B, N, -1),
+                    bbox.reshape(B, N, self.num_classes, 4))
         w1 = self.mrcnn_class_conv1.weight
         x = F.linear(
             x.reshape(x.shape[0], -1),
@@ -63,6 +83,18 @@ class FPNClassifierHead(nn.Module):
         bbox = self.mrcnn_bbox_fc(x).reshape(B * N, self.num_classes, 4)
         return (logits.reshape(B, N, -1), probs.reshape(B, N, -1),
                 bbox.reshape(B, N, self.num_classes, 4))
+
+    def _dense_layers(self, x):
+        """The layer-normed form: pooled tiles -> (logits, box deltas)."""
+        def dense(layer, x, activation="none", residual=None):
+            w = layer.weight
+            return linear_act(x, w.reshape(w.shape[0], -1).to(x.dtype),
+                              layer.bias.to(x.dtype), activation, residual)
+
+        x = x.reshape(x.shape[0], -1)
+        h = self.mrcnn_class_ln1(dense(self.mrcnn_class_conv1, x, "relu"))
+        h = self.mrcnn_class_ln2(dense(self.mrcnn_class_conv2, h, "relu", h))
+        return dense(self.mrcnn_class_logits, h), dense(self.mrcnn_bbox_fc, h)
 
     @staticmethod
     def _bn_vec(bn, x):

@@ -44,9 +44,11 @@ def _copy(arr):
     return arr
 
 
-def keras_weight_map(backbone: str = "resnet101"
+def keras_weight_map(backbone: str = "resnet101",
+                     classif_head_norm: str = "batch"
                      ) -> Dict[str, Tuple[str, object]]:
-    """{'keras_layer/weight': (our_state_key, transform_fn)}.
+    """{'keras_layer/weight': (our_state_key, transform_fn)}; without the
+    box head's batch norms where the head has layer norms.
 
     Layer names follow mrcnn/model.py's graph builders (resnet_graph
     res{stage}{block}_branch*, fpn_*, rpn_*, mrcnn_*)."""
@@ -87,9 +89,11 @@ def keras_weight_map(backbone: str = "resnet101"
         conv(name, f"rpn.{name}")
 
     conv("mrcnn_class_conv1", "classifier_head.mrcnn_class_conv1")
-    bn("mrcnn_class_bn1", "classifier_head.mrcnn_class_bn1")
+    if classif_head_norm == "batch":
+        bn("mrcnn_class_bn1", "classifier_head.mrcnn_class_bn1")
     conv("mrcnn_class_conv2", "classifier_head.mrcnn_class_conv2")
-    bn("mrcnn_class_bn2", "classifier_head.mrcnn_class_bn2")
+    if classif_head_norm == "batch":
+        bn("mrcnn_class_bn2", "classifier_head.mrcnn_class_bn2")
     dense("mrcnn_class_logits", "classifier_head.mrcnn_class_logits")
     dense("mrcnn_bbox_fc", "classifier_head.mrcnn_bbox_fc")
 
@@ -114,7 +118,8 @@ def assign_keras_arrays(model, arrays: Dict[str, np.ndarray],
     Returns (loaded_keys, missing_keras_names, unexpected_names)."""
     import torch
 
-    wmap = keras_weight_map(model.config.BACKBONE)
+    wmap = keras_weight_map(model.config.BACKBONE,
+                            model.config.CLASSIF_HEAD_NORM)
     state = model.state_dict()
     exclude = set(exclude or [])
     loaded, unexpected = [], []

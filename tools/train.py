@@ -40,6 +40,11 @@ def main():
     ap.add_argument("--layers", default="all")
     ap.add_argument("--lr", type=float, default=None)
     ap.add_argument("--num-workers", type=int, default=4)
+    ap.add_argument("--optimizer", default=None,
+                    choices=["sgd", "adamw", "adamw8"],
+                    help="overrides the configuration's OPTIMIZER")
+    ap.add_argument("--head-norm", default=None, choices=["batch", "layer"],
+                    help="overrides the configuration's CLASSIF_HEAD_NORM")
     args = ap.parse_args()
 
     import torch
@@ -75,6 +80,10 @@ def main():
 
     if args.steps:
         config.STEPS_PER_EPOCH = args.steps
+    if args.optimizer:
+        config.OPTIMIZER = args.optimizer
+    if args.head_norm:
+        config.CLASSIF_HEAD_NORM = args.head_norm
 
     from maskrcnn_amd.engine.trainer import Trainer
     from maskrcnn_amd.model import MaskRCNN
