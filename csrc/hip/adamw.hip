@@ -117,36 +117,6 @@ __device__ inline void update(const Hyper& h, float c, float g, float& p,
   p = p * h.decay - step * h.rate;
 }
 
-template <typename T>
-__device__ inline void load4(const T* p, long left, bool wide,
-                             float (&out)[kValues]) {
-  if (wide && left >= kValues) {
-    load_f32<T, kValues>(p, out);
-  } else {
-#pragma unroll
-    for (int i = 0; i < kValues; ++i)
-      out[i] = i < left ? static_cast<float>(p[i]) : 0.0f;
-  }
-}
-
-template <typename T>
-__device__ inline void store4(T* p, long left, bool wide,
-                              const float (&in)[kValues]) {
-  if (wide && left >= kValues) {
-    store_f32<T, kValues>(p, in);
-  } else {
-#pragma unroll
-    for (int i = 0; i < kValues; ++i)
-      if (i < left) p[i] = static_cast<T>(in[i]);
-  }
-}
-
-__device__ inline bool aligned16(const void* a, const void* b, const void* c,
-                                 const void* d) {
-  return (((unsigned long)a | (unsigned long)b | (unsigned long)c |
-           (unsigned long)d) & 15) == 0;
-}
-
 // Workgroups go through the tensors from the end: the norm, if there is one,
 // has just read the gradients from the beginning, and the last of them are
 // still in the memory-side cache.
@@ -166,21 +136,20 @@ __global__ __launch_bounds__(kThreads) void adamw32_kernel(
   const T* g = static_cast<const T*>(t.g[k]);
   float* m = static_cast<float*>(t.m[k]);
   float* v = static_cast<float*>(t.v[k]);
-  const bool wide = aligned16(p, g, m, v);
   const float c = clip_factor(h);
   for (int pass = 0; pass < t.passes; ++pass) {
     const long i = at + (long)pass * kPass, left = n - i;
     if (left <= 0) return;
     float pf[kValues], gf[kValues], mf[kValues], vf[kValues];
-    load4(p + i, left, wide, pf);
-    load4(g + i, left, wide, gf);
-    load4(m + i, left, wide, mf);
-    load4(v + i, left, wide, vf);
+    load_some(p + i, left, pf);
+    load_some(g + i, left, gf);
+    load_some(m + i, left, mf);
+    load_some(v + i, left, vf);
 #pragma unroll
     for (int j = 0; j < kValues; ++j) update(h, c, gf[j], pf[j], mf[j], vf[j]);
-    store4(p + i, left, wide, pf);
-    store4(m + i, left, wide, mf);
-    store4(v + i, left, wide, vf);
+    store_some(p + i, left, pf);
+    store_some(m + i, left, mf);
+    store_some(v + i, left, vf);
   }
 }
 
@@ -252,8 +221,7 @@ __device__ inline int block_exponent(const float (&x)[kValues]) {
 
 template <bool kSigned>
 __device__ inline void store_block8(unsigned char* codes, unsigned char* scale,
-                                    long left, bool wide,
-                                    const float (&x)[kValues]) {
+                                    long left, const float (&x)[kValues]) {
   const int e = block_exponent(x);
   unsigned c[kValues] = {};
   if (e < 255) {                       // of the whole wave
@@ -261,9 +229,9 @@ __device__ inline void store_block8(unsigned char* codes, unsigned char* scale,
 #pragma unroll
     for (int j = 0; j < kValues; ++j) c[j] = encode8<kSigned>(x[j], inv);
   }
-  if (wide && left >= kValues) {
-    *reinterpret_cast<unsigned*>(codes) =
-        c[0] | (c[1] << 8) | (c[2] << 16) | (c[3] << 24);
+  if (left >= kValues) {
+    const unsigned w = c[0] | (c[1] << 8) | (c[2] << 16) | (c[3] << 24);
+    __builtin_memcpy(codes, &w, 4);
   } else {
 #pragma unroll
     for (int j = 0; j < kValues; ++j)
@@ -273,10 +241,12 @@ __device__ inline void store_block8(unsigned char* codes, unsigned char* scale,
 }
 
 // Four codes as they lie in memory, zeros past the end.
-__device__ inline unsigned load_codes(const unsigned char* codes, long left,
-                                      bool wide) {
-  if (wide && left >= kValues) return *reinterpret_cast<const unsigned*>(codes);
+__device__ inline unsigned load_codes(const unsigned char* codes, long left) {
   unsigned w = 0;
+  if (left >= kValues) {
+    __builtin_memcpy(&w, codes, 4);
+    return w;
+  }
 #pragma unroll
   for (int j = 0; j < kValues; ++j)
     if (j < left) w |= (unsigned)codes[j] << (8 * j);
@@ -306,7 +276,6 @@ __global__ __launch_bounds__(kThreads) void adamw8_kernel(
   unsigned char* v = static_cast<unsigned char*>(t.v[k]);
   unsigned char* ms = t.ms[k];
   unsigned char* vs = t.vs[k];
-  const bool wide = aligned16(p, g, m, v);
   const float c = clip_factor(h);
   for (int pass = 0; pass < t.passes; pass += kDeep) {
     float pf[kDeep][kValues], gf[kDeep][kValues];
@@ -316,10 +285,10 @@ __global__ __launch_bounds__(kThreads) void adamw8_kernel(
       const long i = at + (long)(pass + d) * kPass, left = n - i;
       const long b = i / kBlock8;
       if (pass + d >= t.passes || b * kBlock8 >= n) continue;
-      load4(p + i, left, wide, pf[d]);
-      load4(g + i, left, wide, gf[d]);
-      mc[d] = load_codes(m + i, left, wide);
-      vc[d] = load_codes(v + i, left, wide);
+      load_some(p + i, left, pf[d]);
+      load_some(g + i, left, gf[d]);
+      mc[d] = load_codes(m + i, left);
+      vc[d] = load_codes(v + i, left);
       me[d] = ms[b];
       ve[d] = vs[b];
     }
@@ -337,9 +306,9 @@ __global__ __launch_bounds__(kThreads) void adamw8_kernel(
         update(h, c, gf[d][j], pf[d][j], mf[j], vf[j]);
         if (j >= left) mf[j] = vf[j] = 0.0f;   // no part in the maximum
       }
-      store4(p + i, left, wide, pf[d]);
-      store_block8<true>(m + i, ms + b, left, wide, mf);
-      store_block8<false>(v + i, vs + b, left, wide, vf);
+      store_some(p + i, left, pf[d]);
+      store_block8<true>(m + i, ms + b, left, mf);
+      store_block8<false>(v + i, vs + b, left, vf);
     }
   }
 }
@@ -352,10 +321,9 @@ __global__ __launch_bounds__(kThreads) void pack8_kernel(
   const long i = ((long)blockIdx.x * kThreads + threadIdx.x) * kValues;
   const long b = i / kBlock8, left = n - i;
   if (b * kBlock8 >= n) return;
-  const bool wide = aligned16(x, codes, nullptr, nullptr);
   float f[kValues];
-  load4(x + i, left, wide, f);
-  store_block8<kSigned>(codes + i, scales + b, left, wide, f);
+  load_some(x + i, left, f);
+  store_block8<kSigned>(codes + i, scales + b, left, f);
 }
 
 // 16 values a thread.
@@ -366,14 +334,14 @@ __global__ __launch_bounds__(kThreads) void unpack8_kernel(
   const long i = ((long)blockIdx.x * kThreads + threadIdx.x) * kUnpack;
   if (i >= n) return;
   const float e = scale8(scales[i / kBlock8]);
-  if (i + kUnpack <= n && aligned16(codes, out, nullptr, nullptr)) {
-    const Pack<unsigned, 4> w =
-        *reinterpret_cast<const Pack<unsigned, 4>*>(codes + i);
+  if (i + kUnpack <= n) {
+    unsigned w[kUnpack / 4];
+    __builtin_memcpy(w, codes + i, kUnpack);
     constexpr int kStore = 16 / sizeof(T);       // values of 16 bytes
     float f[kUnpack];
 #pragma unroll
     for (int j = 0; j < kUnpack; ++j)
-      f[j] = decode8<kSigned>((w.v[j / 4] >> (8 * (j % 4))) & 255u, e);
+      f[j] = decode8<kSigned>((w[j / 4] >> (8 * (j % 4))) & 255u, e);
 #pragma unroll
     for (int j = 0; j < kUnpack; j += kStore) {
       float o[kStore];
@@ -402,7 +370,6 @@ __global__ __launch_bounds__(kThreads) void square_sum_kernel(
                   threadIdx.x * kValues;
   const long n = t.n[k];
   const T* g = static_cast<const T*>(t.g[k]);
-  const bool wide = ((unsigned long)g & 15) == 0;
   double s = 0.0;
   for (int pass = 0; pass < kNormPasses; pass += kDeep) {
     const long i = at + (long)pass * kPass;
@@ -410,7 +377,7 @@ __global__ __launch_bounds__(kThreads) void square_sum_kernel(
     float f[kDeep][kValues];
 #pragma unroll
     for (int d = 0; d < kDeep; ++d)
-      load4(g + i + d * kPass, n - i - d * kPass, wide, f[d]);
+      load_some(g + i + d * kPass, n - i - d * kPass, f[d]);
 #pragma unroll
     for (int d = 0; d < kDeep; ++d)
 #pragma unroll

@@ -9,8 +9,8 @@
 // Memory bound: x (and dy) are read once and stay in registers between the
 // statistics and the result; the variance is taken from the differences to
 // the mean, in fp32. A row belongs to a team of kTeam lanes (a part of a
-// wave up to 64, a workgroup above), each holding kVecs packets of kWidth
-// consecutive values (16 bytes where rows are aligned for it, else 1 value).
+// wave up to 64, a workgroup above), each holding kVecs packets of 16 bytes;
+// a row may begin anywhere and its last packet may be a part of one.
 // In the backward each lane also keeps its columns' sums of dy xh and dy
 // over all rows it sees; they leave once per workgroup as one row of
 // partial sums and a second launch adds the rows up in a fixed order, so
@@ -64,15 +64,33 @@ __device__ inline void team_sum2(float& a, float& b, float* lds) {
   }
 }
 
+// Values of 16 bytes, what a lane moves at a time.
+template <typename T>
+constexpr int width_of() { return 16 / sizeof(T); }
+
 template <int kTeam>
 constexpr int threads_of() { return kTeam < 256 ? 256 : kTeam; }
 
+// A packet of a row, of which `left` values are there if rows are ragged.
+template <bool kRagged, typename T, int N>
+__device__ inline void load_part(const T* p, int left, float (&out)[N]) {
+  if constexpr (kRagged) load_some<T, N>(p, left, out);
+  else load_f32<T, N>(p, out);
+}
+
+template <bool kRagged, typename T, int N>
+__device__ inline void store_part(T* p, int left, const float (&in)[N]) {
+  if constexpr (kRagged) store_some<T, N>(p, left, in);
+  else store_f32<T, N>(p, in);
+}
+
 // T: x and y; W: weight and bias (null: 1 and 0).
-template <typename T, typename W, int kTeam, int kVecs, int kWidth>
+template <typename T, typename W, int kTeam, int kVecs, bool kRagged>
 __global__ __launch_bounds__(threads_of<kTeam>()) void norm_fwd_kernel(
     const T* x, const W* w, const W* b, T* y, float* mean, float* rstd,
     long rows, int width, long x_stride, float eps) {
   constexpr int kRows = threads_of<kTeam>() / kTeam;   // of one workgroup
+  constexpr int kWidth = width_of<T>();
   __shared__ float lds[32];
   const long row = (long)blockIdx.x * kRows + threadIdx.x / kTeam;
   const int lane = threadIdx.x % kTeam;
@@ -85,7 +103,7 @@ __global__ __launch_bounds__(threads_of<kTeam>()) void norm_fwd_kernel(
   for (int k = 0; k < kVecs; ++k) {
     const int c = (k * kTeam + lane) * kWidth;
     if (c < width) {
-      load_f32<T, kWidth>(x + c, v[k]);
+      load_part<kRagged>(x + c, width - c, v[k]);
 #pragma unroll
       for (int i = 0; i < kWidth; ++i) s += v[k][i];
     }
@@ -99,7 +117,7 @@ __global__ __launch_bounds__(threads_of<kTeam>()) void norm_fwd_kernel(
     if (c < width) {
 #pragma unroll
       for (int i = 0; i < kWidth; ++i) {
-        v[k][i] -= mu;
+        v[k][i] = !kRagged || c + i < width ? v[k][i] - mu : 0.0f;
         s += v[k][i] * v[k][i];
       }
     }
@@ -112,11 +130,11 @@ __global__ __launch_bounds__(threads_of<kTeam>()) void norm_fwd_kernel(
       float wf[kWidth], bf[kWidth];
 #pragma unroll
       for (int i = 0; i < kWidth; ++i) { wf[i] = 1.0f; bf[i] = 0.0f; }
-      if (w != nullptr) load_f32<W, kWidth>(w + c, wf);
-      if (b != nullptr) load_f32<W, kWidth>(b + c, bf);
+      if (w != nullptr) load_part<kRagged>(w + c, width - c, wf);
+      if (b != nullptr) load_part<kRagged>(b + c, width - c, bf);
 #pragma unroll
       for (int i = 0; i < kWidth; ++i) v[k][i] = v[k][i] * r * wf[i] + bf[i];
-      store_f32<T, kWidth>(y + c, v[k]);
+      store_part<kRagged>(y + c, width - c, v[k]);
     }
   }
   if (mean != nullptr && lane == 0) {
@@ -127,12 +145,13 @@ __global__ __launch_bounds__(threads_of<kTeam>()) void norm_fwd_kernel(
 
 // `part`: gridDim.x rows of two halves of sums (dy xh, then dy); null: no
 // weight gradients wanted. `dx` may be null too.
-template <typename T, typename W, int kTeam, int kVecs, int kWidth>
+template <typename T, typename W, int kTeam, int kVecs, bool kRagged>
 __global__ __launch_bounds__(threads_of<kTeam>()) void norm_bwd_kernel(
     const T* dy, const T* x, const W* w, const float* mean, const float* rstd,
     T* dx, float* part, long rows, int width, long dy_stride, long x_stride) {
   constexpr int kThreads = threads_of<kTeam>();
   constexpr int kRows = kThreads / kTeam;
+  constexpr int kWidth = width_of<T>();
   constexpr int kCols = kTeam * kVecs * kWidth;
   __shared__ float lds[32];
   __shared__ float sums[kRows > 1 ? 2 * kRows * kCols : 1];
@@ -146,7 +165,8 @@ __global__ __launch_bounds__(threads_of<kTeam>()) void norm_bwd_kernel(
       wf[k][i] = 1.0f;
       dw[k][i] = db[k][i] = 0.0f;
     }
-    if (w != nullptr && c < width) load_f32<W, kWidth>(w + c, wf[k]);
+    if (w != nullptr && c < width)
+      load_part<kRagged>(w + c, width - c, wf[k]);
   }
   const float inv = 1.0f / (float)width;
   for (long row = (long)blockIdx.x * kRows + team; row < rows;
@@ -160,8 +180,8 @@ __global__ __launch_bounds__(threads_of<kTeam>()) void norm_bwd_kernel(
     for (int k = 0; k < kVecs; ++k) {
       const int c = (k * kTeam + lane) * kWidth;
       if (c < width) {
-        load_f32<T, kWidth>(xr + c, xh[k]);
-        load_f32<T, kWidth>(dyr + c, d[k]);
+        load_part<kRagged>(xr + c, width - c, xh[k]);
+        load_part<kRagged>(dyr + c, width - c, d[k]);
       }
     }
 #pragma unroll
@@ -191,7 +211,7 @@ __global__ __launch_bounds__(threads_of<kTeam>()) void norm_bwd_kernel(
 #pragma unroll
         for (int i = 0; i < kWidth; ++i)
           d[k][i] = r * (d[k][i] - s1 - xh[k][i] * s2);
-        store_f32<T, kWidth>(dxr + c, d[k]);
+        store_part<kRagged>(dxr + c, width - c, d[k]);
       }
     }
   }
@@ -203,8 +223,8 @@ __global__ __launch_bounds__(threads_of<kTeam>()) void norm_bwd_kernel(
     for (int k = 0; k < kVecs; ++k) {
       const int c = (k * kTeam + lane) * kWidth;
       if (c < width) {
-        store_f32<float, kWidth>(part + c, dw[k]);
-        store_f32<float, kWidth>(part + pad + c, db[k]);
+        store_part<kRagged>(part + c, width - c, dw[k]);
+        store_part<kRagged>(part + pad + c, width - c, db[k]);
       }
     }
   } else {
@@ -355,16 +375,16 @@ __global__ __launch_bounds__(1024) void sum_rows_kernel(
 
 namespace {
 
-template <typename T, typename W, int kTeam, int kVecs, int kWidth>
+template <typename T, typename W, int kTeam, int kVecs, bool kRagged>
 void run_team(const NormArgs& a, bool backward, hipStream_t s) {
   constexpr int threads = threads_of<kTeam>(), per = threads / kTeam;
   if (!backward) {
     const unsigned grid = (unsigned)((a.rows + per - 1) / per);
-    norm_fwd_kernel<T, W, kTeam, kVecs, kWidth><<<grid, threads, 0, s>>>(
+    norm_fwd_kernel<T, W, kTeam, kVecs, kRagged><<<grid, threads, 0, s>>>(
         (const T*)a.x, (const W*)a.w, (const W*)a.b, (T*)a.y, a.mean, a.rstd,
         a.rows, a.width, a.x_stride, a.eps);
   } else {
-    norm_bwd_kernel<T, W, kTeam, kVecs, kWidth><<<a.parts, threads, 0, s>>>(
+    norm_bwd_kernel<T, W, kTeam, kVecs, kRagged><<<a.parts, threads, 0, s>>>(
         (const T*)a.dy, (const T*)a.x, (const W*)a.w, a.mean, a.rstd,
         (T*)a.dx, a.part, a.rows, a.width, a.dy_stride, a.x_stride);
   }
@@ -378,23 +398,23 @@ int rows_at_once(int packets) {
 
 // A team is as small as its row allows, with few packets a lane: the
 // exchange takes fewer steps and more rows are in flight.
-template <typename T, typename W, int kWidth>
+template <typename T, typename W, bool kRagged>
 bool run_width(const NormArgs& a, bool backward, hipStream_t s) {
-  const int packets = (a.width + kWidth - 1) / kWidth;
-  if (packets <= 8) run_team<T, W, 8, 1, kWidth>(a, backward, s);
-  else if (packets <= 16) run_team<T, W, 16, 1, kWidth>(a, backward, s);
-  else if (packets <= 32) run_team<T, W, 32, 1, kWidth>(a, backward, s);
-  else if (packets <= 64) run_team<T, W, 64, 1, kWidth>(a, backward, s);
-  else if (packets <= 128) run_team<T, W, 64, 2, kWidth>(a, backward, s);
-  else if (packets <= 256) run_team<T, W, 256, 1, kWidth>(a, backward, s);
-  else if (packets <= 512) run_team<T, W, 256, 2, kWidth>(a, backward, s);
-  else if (packets <= 1024) run_team<T, W, 256, 4, kWidth>(a, backward, s);
-  else if (packets <= 2048) run_team<T, W, 512, 4, kWidth>(a, backward, s);
+  const int packets = (a.width + width_of<T>() - 1) / width_of<T>();
+  if (packets <= 8) run_team<T, W, 8, 1, kRagged>(a, backward, s);
+  else if (packets <= 16) run_team<T, W, 16, 1, kRagged>(a, backward, s);
+  else if (packets <= 32) run_team<T, W, 32, 1, kRagged>(a, backward, s);
+  else if (packets <= 64) run_team<T, W, 64, 1, kRagged>(a, backward, s);
+  else if (packets <= 128) run_team<T, W, 64, 2, kRagged>(a, backward, s);
+  else if (packets <= 256) run_team<T, W, 256, 1, kRagged>(a, backward, s);
+  else if (packets <= 512) run_team<T, W, 256, 2, kRagged>(a, backward, s);
+  else if (packets <= 1024) run_team<T, W, 256, 4, kRagged>(a, backward, s);
+  else if (packets <= 2048) run_team<T, W, 512, 4, kRagged>(a, backward, s);
   else if (packets <= 4096) {
     // 1024 lanes have 128 registers each: the backward's four arrays of 32
     // values do not fit, so such rows go to the wide kernels.
-    if constexpr (kWidth < 8) {
-      run_team<T, W, 1024, 4, kWidth>(a, backward, s);
+    if constexpr (sizeof(T) == 4) {
+      run_team<T, W, 1024, 4, kRagged>(a, backward, s);
     } else {
       return false;
     }
@@ -406,9 +426,8 @@ bool run_width(const NormArgs& a, bool backward, hipStream_t s) {
 
 template <typename T, typename W>
 void run_types(const NormArgs& a, bool backward, hipStream_t s) {
-  constexpr int full = 16 / sizeof(T);
-  if (a.aligned ? run_width<T, W, full>(a, backward, s)
-                : run_width<T, W, 1>(a, backward, s))
+  if (a.width % width_of<T>() ? run_width<T, W, true>(a, backward, s)
+                              : run_width<T, W, false>(a, backward, s))
     return;
   if (!backward) {
     norm_fwd_wide_kernel<T, W><<<(unsigned)a.rows, kWide, 0, s>>>(
@@ -441,8 +460,8 @@ hipError_t run_norm(const NormArgs& a, int type, int wtype, bool backward,
 
 // Rows of partial sums that the backward writes: a workgroup for each set of
 // rows up to four a CU, so that many rows share one row of sums.
-extern "C" int layer_norm_parts(long rows, int width, int type, bool aligned) {
-  const int per = aligned ? (type == kElemF32 ? 4 : 8) : 1;
+extern "C" int layer_norm_parts(long rows, int width, int type) {
+  const int per = type == kElemF32 ? 4 : 8;
   const int at_once = rows_at_once((width + per - 1) / per);
   const long sets = (rows + at_once - 1) / at_once;
   return (int)(sets < 1024 ? sets : 1024);

@@ -289,16 +289,14 @@ struct Raw {
   i32x4 q[sizeof(T) * kOut / 16];
 };
 
-// The residual's columns n .. n + 7 of row m, where 8 move as one access.
+// The residual's columns n .. n + 7 of row m, if all are there.
 template <typename T>
-__device__ inline Raw<T> load_residual(const LinearEpilogue& e, long m,
-                                       int n) {
+__device__ inline Raw<T> load_residual(const LinearEpilogue& e, long m, int n,
+                                       int N) {
   Raw<T> r = {};
-  if (e.residual == nullptr || !e.wide) return r;
-  const i32x4* p =
-      (const i32x4*)((const T*)e.residual + m * e.ld_residual + n);
-#pragma unroll
-  for (int i = 0; i < (int)(sizeof(T) * kOut / 16); ++i) r.q[i] = p[i];
+  if (e.residual != nullptr && n + kOut <= N)
+    __builtin_memcpy(&r, (const T*)e.residual + m * e.ld_residual + n,
+                     sizeof(r));
   return r;
 }
 
@@ -309,7 +307,7 @@ __device__ inline void finish(const LinearEpilogue& e, long m, int n, int N,
                               float (&z)[kOut]) {
   T* out = (T*)e.y + m * (long)N + n;
   T* keep = e.kept ? (T*)e.kept + m * (long)N + n : nullptr;
-  if (e.wide) {      // then N % 8 == 0
+  if (n + kOut <= N) {
     typedef T Res __attribute__((ext_vector_type(kOut)));
     const Res r = __builtin_bit_cast(Res, raw);
     float kept[kOut];
@@ -532,7 +530,7 @@ __global__ __launch_bounds__(kWM * kWN * 64, 2) void product_kernel(
   float b[kOut];
   load_bias<T>(a.e, n, a.n, b);
   with_act(a.e.act, [&](auto act) {
-    rows([&](int m) { return load_residual<T>(a.e, m, n); },
+    rows([&](int m) { return load_residual<T>(a.e, m, n, a.n); },
          [&](int m, Raw<T> r, float (&z)[kOut]) {
            finish<T, act>(a.e, m, n, a.n, b, r, z);
          });
@@ -550,7 +548,7 @@ __global__ __launch_bounds__(256) void join_kernel(LinearProduct a) {
   const float* p = a.part + m * a.ld_part + n;
   float z[kOut], b[kOut];
   load_bias<T>(a.e, n, a.n, b);
-  const Raw<T> r = load_residual<T>(a.e, m, n);
+  const Raw<T> r = load_residual<T>(a.e, m, n, a.n);
   load_f32<float, kOut>(p, z);
 #pragma unroll 4
   for (int s = 1; s < a.splits; ++s) {
@@ -572,7 +570,7 @@ __global__ __launch_bounds__(256) void join_kernel(LinearProduct a) {
 template <typename T, int kAct>
 __global__ __launch_bounds__(256) void dz_kernel(
     const T* dy, const T* kept, T* dz, float* part, int m, int n, long ld_dy,
-    int ld_dz, int rows, bool wide) {
+    int ld_dz, int rows) {
   constexpr int kDeep = 4;
   __shared__ float lds[8][256 + 8];
   const int c = blockIdx.x * 256 + (threadIdx.x & 31) * 8;
@@ -585,20 +583,9 @@ __global__ __launch_bounds__(256) void dz_kernel(
       const int row = r + 8 * d;
       const T* p = dy + row * ld_dy + c;
       const T* q = kept + (long)row * n + c;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) g[d][i] = s[d][i] = 0.0f;
       if (row >= r1) continue;
-      if (wide && c < n) {
-        load_f32<T, 8>(p, g[d]);
-        if (kAct != kActNone) load_f32<T, 8>(q, s[d]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (c + i >= n) continue;
-          g[d][i] = (float)p[i];
-          if (kAct != kActNone) s[d][i] = (float)q[i];
-        }
-      }
+      load_some<T, 8>(p, n - c, g[d]);
+      if (kAct != kActNone) load_some<T, 8>(q, n - c, s[d]);
     }
 #pragma unroll
     for (int d = 0; d < kDeep; ++d) {
@@ -610,14 +597,7 @@ __global__ __launch_bounds__(256) void dz_kernel(
         sum[i] += g[d][i];
       }
       if (dz) {
-        T* o = dz + (long)row * ld_dz + c;
-        if (c + 8 <= ld_dz) {
-          store_f32<T, 8>(o, g[d]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (c + i < ld_dz) o[i] = (T)g[d][i];
-        }
+        store_some<T, 8>(dz + (long)row * ld_dz + c, ld_dz - c, g[d]);
       }
     }
   }
@@ -635,17 +615,28 @@ __global__ __launch_bounds__(256) void dz_kernel(
   }
 }
 
-// Rows of `width` values at any stride -> rows of `ld` values, zeros behind.
+// Rows of `width` values at any stride -> rows of `ld` values, a whole number
+// of 16 bytes, zeros behind. A thread has 16 bytes of the result.
 template <typename T>
 __global__ __launch_bounds__(256) void pad_kernel(const T* from, T* to,
                                                   int rows, int width,
                                                   long stride, int ld) {
-  const long total = (long)rows * ld;
+  constexpr int kPer = 16 / sizeof(T);
+  const int across = ld / kPer;
+  const long total = (long)rows * across;
   for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total;
        i += (long)gridDim.x * 256) {
-    const long r = i / ld;
-    const int c = (int)(i % ld);
-    to[i] = c < width ? from[r * stride + c] : (T)0.0f;
+    const long r = i / across;
+    const int c = (int)(i % across) * kPer;
+    const T* p = from + r * stride + c;
+    T v[kPer];
+    if (c + kPer <= width) {
+      __builtin_memcpy(v, p, 16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) v[j] = c + j < width ? p[j] : (T)0.0f;
+    }
+    __builtin_memcpy(to + r * ld + c, v, 16);
   }
 }
 
@@ -686,7 +677,7 @@ hipError_t run_product(const LinearProduct& a, hipStream_t s) {
 template <typename T>
 hipError_t run_pad(const void* from, void* to, int rows, int width,
                    long stride, int ld, hipStream_t s) {
-  const long blocks = ((long)rows * ld + 1023) / 1024;
+  const long blocks = ((long)rows * ld * sizeof(T) + 4095) / 4096;
   pad_kernel<T><<<(unsigned)(blocks < 65536 ? blocks : 65536), 256, 0, s>>>(
       (const T*)from, (T*)to, rows, width, stride, ld);
   return hipGetLastError();
@@ -705,7 +696,7 @@ extern "C" void linear_plan(LinearProduct* a, int type) {
   struct Shape { int tile; double step, alone, rest; };
   static const Shape kHalf[] = {{256, 1.55, 1.55, 6.0},
                                 {128, 0.55, 0.55, 2.5},
-                                {64, 0.25, 0.40, 1.0}};
+                                {64, 0.25, 0.30, 1.0}};
   static const Shape kFull[] = {{128, 1.8, 1.8, 2.5}, {64, 0.5, 0.5, 1.0}};
   const Shape* shapes = type == kElemF32 ? kFull : kHalf;
   const int count = type == kElemF32 ? 2 : 3;
@@ -722,7 +713,7 @@ extern "C" void linear_plan(LinearProduct* a, int type) {
       const double us =
           rounds * (each * (rounds == 1 ? shapes[i].alone : shapes[i].step) +
                     shapes[i].rest) +
-          (s > 1 ? 3.5 + (double)s * a->m * a->n * 8.0 / 4.5e6 : 0.0);
+          (s > 1 ? 4.8 + (double)s * a->m * a->n * 8.0 / 4.5e6 : 0.0);
       if (best == 0.0 || us < best) {
         best = us;
         a->tile = t;
@@ -760,7 +751,7 @@ static hipError_t run_dz(const LinearDz& a, hipStream_t s) {
   const auto run = [&](auto act) {
     dz_kernel<T, act><<<dim3((cols + 255) / 256, a.strips), 256, 0, s>>>(
         (const T*)a.dy, (const T*)a.kept, (T*)a.dz, a.part, a.m, a.n, a.ld_dy,
-        a.ld_dz, rows, a.wide);
+        a.ld_dz, rows);
   };
   with_act(a.act, run);
   return hipGetLastError();

@@ -40,7 +40,6 @@ struct NormArgs {
   long rows, x_stride, dy_stride;
   int width;
   int parts;           // the backward's grid
-  bool aligned;        // rows of all operands begin at multiples of 16 bytes
   float eps;
 };
 
@@ -54,7 +53,6 @@ struct LinearEpilogue {
                            // ReLU's derivative, else z
   long ld_residual;
   int act;
-  bool wide;               // 8 columns move as one access, and n % 8 == 0
 };
 
 // D[m][n] = sum over k of X(m, k) Y(n, k). Rows of both operands begin at
@@ -80,7 +78,6 @@ struct LinearDz {
                            // or null
   long ld_dy;
   int m, n, ld_dz, strips, act;
-  bool wide;               // 8 columns of dy and kept move as one access
 };
 
 extern "C" {
@@ -88,7 +85,8 @@ void linear_plan(LinearProduct*, int type);
 hipError_t linear_product_launch(const LinearProduct*, int type, hipStream_t);
 int linear_dz_strips(int m, int n);
 hipError_t linear_dz_launch(const LinearDz*, int type, hipStream_t);
-// Rows of `width` values -> rows of `ld` values, zeros behind.
+// Rows of `width` values -> rows of `ld` values, a whole number of 16 bytes,
+// zeros behind.
 hipError_t linear_pad_launch(const void* from, void* to, int rows, int width,
                              long stride, int ld, int type, hipStream_t);
 
@@ -109,7 +107,7 @@ hipError_t unpack8_launch(const unsigned char* codes,
                           bool is_signed, int type, hipStream_t);
 
 // Rows of partial sums that the norm's backward writes.
-int layer_norm_parts(long rows, int width, int type, bool aligned);
+int layer_norm_parts(long rows, int width, int type);
 hipError_t layer_norm_fwd_launch(const NormArgs*, int type, int wtype,
                                  hipStream_t);
 hipError_t layer_norm_bwd_launch(const NormArgs*, int type, int wtype,

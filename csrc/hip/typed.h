@@ -7,26 +7,49 @@
 using bf16_t = __bf16;
 using fp16_t = _Float16;
 
-// N values of T that move as one access of N * sizeof(T) bytes.
-template <typename T, int N>
-struct alignas(sizeof(T) * N) Pack {
-  T v[N];
-};
-
+// N consecutive values of T that move as one access (two of 16 bytes above
+// that), at any address that is T's own: global memory takes wide accesses
+// unaligned, for a little more time where one crosses a line.
 template <typename T, int N>
 __device__ inline void load_f32(const T* p, float (&out)[N]) {
-  const Pack<T, N> a = *reinterpret_cast<const Pack<T, N>*>(p);
+  typedef T Vec __attribute__((ext_vector_type(N)));
+  Vec a;
+  __builtin_memcpy(&a, p, sizeof(T) * N);
 #pragma unroll
-  for (int i = 0; i < N; ++i) out[i] = static_cast<float>(a.v[i]);
+  for (int i = 0; i < N; ++i) out[i] = static_cast<float>(a[i]);
 }
 
 // One rounding, to nearest even, from the fp32 result to the tensor's type.
 template <typename T, int N>
 __device__ inline void store_f32(T* p, const float (&in)[N]) {
-  Pack<T, N> a;
+  typedef T Vec __attribute__((ext_vector_type(N)));
+  Vec a;
 #pragma unroll
-  for (int i = 0; i < N; ++i) a.v[i] = static_cast<T>(in[i]);
-  *reinterpret_cast<Pack<T, N>*>(p) = a;
+  for (int i = 0; i < N; ++i) a[i] = static_cast<T>(in[i]);
+  __builtin_memcpy(p, &a, sizeof(T) * N);
+}
+
+// The same where only the first `left` values are there; the others are 0.
+template <typename T, int N>
+__device__ inline void load_some(const T* p, long left, float (&out)[N]) {
+  if (left >= N) {
+    load_f32<T, N>(p, out);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    out[i] = i < left ? static_cast<float>(p[i]) : 0.0f;
+}
+
+template <typename T, int N>
+__device__ inline void store_some(T* p, long left, const float (&in)[N]) {
+  if (left >= N) {
+    store_f32<T, N>(p, in);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (i < left) p[i] = static_cast<T>(in[i]);
 }
 
 // Types as the launchers take them.

@@ -47,12 +47,6 @@ Tensor as_rows(const Tensor& x, int64_t width) {
   return x.contiguous().view({-1, width});
 }
 
-bool norm_aligned(const Tensor& rows) {
-  const int64_t e = rows.element_size(), full = 16 / e;
-  return rows.size(1) % full == 0 && rows.stride(0) % full == 0 &&
-         aligned16(rows.data_ptr());
-}
-
 void check_norm(const Tensor& x, const std::optional<Tensor>& w,
                 const char* name) {
   if (!w) return;
@@ -103,7 +97,6 @@ std::vector<Tensor> layer_norm_fwd(const Tensor& x, std::optional<Tensor> w,
     a.rows = rows;
     a.width = (int)width;
     a.x_stride = rows > 1 ? xr.stride(0) : width;
-    a.aligned = norm_aligned(xr) && aligned16(a.w) && aligned16(a.b);
     a.eps = (float)eps;
     launched(layer_norm_fwd_launch(
                  &a, type, w ? elem_type(*w, "layer_norm")
@@ -148,8 +141,7 @@ std::vector<Tensor> layer_norm_bwd(const Tensor& dy, const Tensor& x,
     a.width = (int)width;
     a.x_stride = rows > 1 ? xr.stride(0) : width;
     a.dy_stride = rows > 1 ? dyr.stride(0) : width;
-    a.aligned = norm_aligned(xr) && norm_aligned(dyr) && aligned16(a.w);
-    a.parts = layer_norm_parts(rows, (int)width, type, a.aligned);
+    a.parts = layer_norm_parts(rows, (int)width, type);
     Tensor part;
     if (want_dw || want_db) {
       part = torch::empty({a.parts, 2 * norm_part_half((int)width)},
@@ -281,17 +273,14 @@ std::vector<Tensor> linear_fwd(const Tensor& x, const Tensor& w,
   a.e.act = (int)act;
   a.e.y = y.data_ptr();
   a.e.kept = kept.defined() ? kept.data_ptr() : nullptr;
-  a.e.wide = N % 8 == 0;
   if (bias) {
     b = bias->contiguous();
     a.e.bias = b.data_ptr();
-    a.e.wide = a.e.wide && aligned16(a.e.bias);
   }
   if (residual) {
     r = as_matrix(*residual, M, N);
     a.e.residual = r.data_ptr();
     a.e.ld_residual = M > 1 ? r.stride(0) : N;
-    a.e.wide = a.e.wide && aligned16(a.e.residual) && a.e.ld_residual % 8 == 0;
   }
   product(a, type, x, stream);
   return {y, kept};
@@ -344,7 +333,6 @@ std::vector<Tensor> linear_bwd(const Tensor& dy,
     z.m = (int)M;
     z.n = (int)N;
     z.strips = linear_dz_strips(z.m, z.n);
-    z.wide = N % 8 == 0 && ldg % 8 == 0 && aligned16(z.dy);
     Tensor part;
     if (want_db) {
       part = torch::empty({z.strips, norm_part_half(z.n)},
@@ -373,7 +361,6 @@ std::vector<Tensor> linear_bwd(const Tensor& dy,
     a.n = (int)K;
     a.ext_y = wo.width;
     a.e.y = dx.data_ptr();
-    a.e.wide = K % 8 == 0;
     product(a, type, x, stream);
   }
   if (want_dw) {
@@ -390,7 +377,6 @@ std::vector<Tensor> linear_bwd(const Tensor& dy,
     a.n = (int)K;
     a.ext_y = xo.width;
     a.e.y = dw.data_ptr();
-    a.e.wide = K % 8 == 0;
     product(a, type, x, stream);
   }
   return {dx, dw, db};
