@@ -141,15 +141,15 @@ __global__ __launch_bounds__(kThreads) void adamw32_kernel(
     const long i = at + (long)pass * kPass, left = n - i;
     if (left <= 0) return;
     float pf[kValues], gf[kValues], mf[kValues], vf[kValues];
-    load_some(p + i, left, pf);
+    stream_in(p + i, left, pf);
     load_some(g + i, left, gf);
-    load_some(m + i, left, mf);
-    load_some(v + i, left, vf);
+    stream_in(m + i, left, mf);
+    stream_in(v + i, left, vf);
 #pragma unroll
     for (int j = 0; j < kValues; ++j) update(h, c, gf[j], pf[j], mf[j], vf[j]);
-    store_some(p + i, left, pf);
-    store_some(m + i, left, mf);
-    store_some(v + i, left, vf);
+    stream_out(p + i, left, pf);
+    stream_out(m + i, left, mf);
+    stream_out(v + i, left, vf);
   }
 }
 
@@ -285,7 +285,7 @@ __global__ __launch_bounds__(kThreads) void adamw8_kernel(
       const long i = at + (long)(pass + d) * kPass, left = n - i;
       const long b = i / kBlock8;
       if (pass + d >= t.passes || b * kBlock8 >= n) continue;
-      load_some(p + i, left, pf[d]);
+      stream_in(p + i, left, pf[d]);
       load_some(g + i, left, gf[d]);
       mc[d] = load_codes(m + i, left);
       vc[d] = load_codes(v + i, left);
@@ -306,7 +306,7 @@ __global__ __launch_bounds__(kThreads) void adamw8_kernel(
         update(h, c, gf[d][j], pf[d][j], mf[j], vf[j]);
         if (j >= left) mf[j] = vf[j] = 0.0f;   // no part in the maximum
       }
-      store_some(p + i, left, pf[d]);
+      stream_out(p + i, left, pf[d]);
       store_block8<true>(m + i, ms + b, left, mf);
       store_block8<false>(v + i, vs + b, left, vf);
     }

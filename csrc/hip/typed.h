@@ -29,6 +29,37 @@ __device__ inline void store_f32(T* p, const float (&in)[N]) {
   __builtin_memcpy(p, &a, sizeof(T) * N);
 }
 
+// The same past the caches: data that nobody reads again soon leaves them to
+// what is.
+template <typename T, int N>
+__device__ inline void stream_in(const T* p, long left, float (&out)[N]) {
+  if (left >= N && ((unsigned long)p & (sizeof(T) * N - 1)) == 0) {
+    typedef T Vec __attribute__((ext_vector_type(N)));
+    const Vec a = __builtin_nontemporal_load((const Vec*)p);
+#pragma unroll
+    for (int i = 0; i < N; ++i) out[i] = static_cast<float>(a[i]);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    out[i] = i < left ? static_cast<float>(p[i]) : 0.0f;
+}
+
+template <typename T, int N>
+__device__ inline void stream_out(T* p, long left, const float (&in)[N]) {
+  if (left >= N && ((unsigned long)p & (sizeof(T) * N - 1)) == 0) {
+    typedef T Vec __attribute__((ext_vector_type(N)));
+    Vec a;
+#pragma unroll
+    for (int i = 0; i < N; ++i) a[i] = static_cast<T>(in[i]);
+    __builtin_nontemporal_store(a, (Vec*)p);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (i < left) p[i] = static_cast<T>(in[i]);
+}
+
 // The same where only the first `left` values are there; the others are 0.
 template <typename T, int N>
 __device__ inline void load_some(const T* p, long left, float (&out)[N]) {
