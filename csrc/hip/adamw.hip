@@ -142,7 +142,7 @@ __global__ __launch_bounds__(kThreads) void adamw32_kernel(
     if (left <= 0) return;
     float pf[kValues], gf[kValues], mf[kValues], vf[kValues];
     stream_in(p + i, left, pf);
-    load_some(g + i, left, gf);
+    stream_in(g + i, left, gf);
     stream_in(m + i, left, mf);
     stream_in(v + i, left, vf);
 #pragma unroll
@@ -286,7 +286,7 @@ __global__ __launch_bounds__(kThreads) void adamw8_kernel(
       const long b = i / kBlock8;
       if (pass + d >= t.passes || b * kBlock8 >= n) continue;
       stream_in(p + i, left, pf[d]);
-      load_some(g + i, left, gf[d]);
+      stream_in(g + i, left, gf[d]);
       mc[d] = load_codes(m + i, left);
       vc[d] = load_codes(v + i, left);
       me[d] = ms[b];
