@@ -255,26 +255,51 @@ __global__ __launch_bounds__(threads_of<kTeam>()) void norm_bwd_kernel(
 
 constexpr int kWide = 1024;   // threads of one row
 
+// f(column, values there) for the thread's packets of a row.
+template <typename T, typename F>
+__device__ inline void each_packet(int width, F f) {
+  constexpr int kWidth = width_of<T>();
+  for (int c = threadIdx.x * kWidth; c < width; c += kWide * kWidth)
+    f(c, width - c);
+}
+
 template <typename T, typename W>
 __global__ __launch_bounds__(kWide) void norm_fwd_wide_kernel(
     const T* x, const W* w, const W* b, T* y, float* mean, float* rstd,
     int width, long x_stride, float eps) {
+  constexpr int kWidth = width_of<T>();
   __shared__ float lds[32];
   const long row = blockIdx.x;
   x += row * x_stride;
   y += row * (long)width;
   float s = 0.0f;
-  for (int c = threadIdx.x; c < width; c += kWide) s += (float)x[c];
+  each_packet<T>(width, [&](int c, int left) {
+    float v[kWidth];
+    load_some<T, kWidth>(x + c, left, v);
+#pragma unroll
+    for (int i = 0; i < kWidth; ++i) s += v[i];
+  });
   const float mu = team_sum<kWide>(s, lds) / (float)width;
   s = 0.0f;
-  for (int c = threadIdx.x; c < width; c += kWide) {
-    const float v = (float)x[c] - mu;
-    s += v * v;
-  }
+  each_packet<T>(width, [&](int c, int left) {
+    float v[kWidth];
+    load_some<T, kWidth>(x + c, left, v);
+#pragma unroll
+    for (int i = 0; i < kWidth; ++i)
+      s += i < left ? (v[i] - mu) * (v[i] - mu) : 0.0f;
+  });
   const float r = 1.0f / sqrtf(team_sum<kWide>(s, lds) / (float)width + eps);
-  for (int c = threadIdx.x; c < width; c += kWide)
-    y[c] = (T)(((float)x[c] - mu) * r * (w ? (float)w[c] : 1.0f) +
-               (b ? (float)b[c] : 0.0f));
+  each_packet<T>(width, [&](int c, int left) {
+    float v[kWidth], wf[kWidth], bf[kWidth];
+    load_some<T, kWidth>(x + c, left, v);
+#pragma unroll
+    for (int i = 0; i < kWidth; ++i) { wf[i] = 1.0f; bf[i] = 0.0f; }
+    if (w != nullptr) load_some<W, kWidth>(w + c, left, wf);
+    if (b != nullptr) load_some<W, kWidth>(b + c, left, bf);
+#pragma unroll
+    for (int i = 0; i < kWidth; ++i) v[i] = (v[i] - mu) * r * wf[i] + bf[i];
+    store_some<T, kWidth>(y + c, left, v);
+  });
   if (mean != nullptr && threadIdx.x == 0) {
     mean[row] = mu;
     rstd[row] = r;
@@ -285,44 +310,74 @@ template <typename T, typename W>
 __global__ __launch_bounds__(kWide) void norm_dx_wide_kernel(
     const T* dy, const T* x, const W* w, const float* mean, const float* rstd,
     T* dx, int width, long dy_stride, long x_stride) {
+  constexpr int kWidth = width_of<T>();
   __shared__ float lds[32];
   const long row = blockIdx.x;
   const float mu = mean[row], r = rstd[row];
   x += row * x_stride;
   dy += row * dy_stride;
   dx += row * (long)width;
+  // d = dy w and xh of a packet; d is 0 past the row's end.
+  const auto load = [&](int c, int left, float (&d)[kWidth],
+                        float (&xh)[kWidth]) {
+    load_some<T, kWidth>(dy + c, left, d);
+    load_some<T, kWidth>(x + c, left, xh);
+    float wf[kWidth];
+#pragma unroll
+    for (int i = 0; i < kWidth; ++i) wf[i] = 1.0f;
+    if (w != nullptr) load_some<W, kWidth>(w + c, left, wf);
+#pragma unroll
+    for (int i = 0; i < kWidth; ++i) {
+      d[i] *= wf[i];
+      xh[i] = (xh[i] - mu) * r;
+    }
+  };
   float s1 = 0.0f, s2 = 0.0f;
-  for (int c = threadIdx.x; c < width; c += kWide) {
-    const float d = (float)dy[c] * (w ? (float)w[c] : 1.0f);
-    s1 += d;
-    s2 += d * (((float)x[c] - mu) * r);
-  }
+  each_packet<T>(width, [&](int c, int left) {
+    float d[kWidth], xh[kWidth];
+    load(c, left, d, xh);
+#pragma unroll
+    for (int i = 0; i < kWidth; ++i) {
+      s1 += d[i];
+      s2 += d[i] * xh[i];
+    }
+  });
   team_sum2<kWide>(s1, s2, lds);
   s1 /= (float)width;
   s2 /= (float)width;
-  for (int c = threadIdx.x; c < width; c += kWide) {
-    const float d = (float)dy[c] * (w ? (float)w[c] : 1.0f);
-    dx[c] = (T)(r * (d - s1 - ((float)x[c] - mu) * r * s2));
-  }
+  each_packet<T>(width, [&](int c, int left) {
+    float d[kWidth], xh[kWidth];
+    load(c, left, d, xh);
+#pragma unroll
+    for (int i = 0; i < kWidth; ++i) d[i] = r * (d[i] - s1 - xh[i] * s2);
+    store_some<T, kWidth>(dx + c, left, d);
+  });
 }
 
-// One column a thread, gridDim.y strips of rows.
+// A packet of columns a thread, gridDim.y strips of rows.
 template <typename T>
 __global__ __launch_bounds__(256) void norm_dw_wide_kernel(
     const T* dy, const T* x, const float* mean, const float* rstd,
     float* part, long rows, int width, long dy_stride, long x_stride) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
+  constexpr int kWidth = width_of<T>();
+  const int c = (blockIdx.x * 256 + threadIdx.x) * kWidth;
   if (c >= width) return;
-  float a = 0.0f, b = 0.0f;
+  float a[kWidth] = {}, b[kWidth] = {};
   for (long row = blockIdx.y; row < rows; row += gridDim.y) {
-    const float d = (float)dy[row * dy_stride + c];
-    a += d * (((float)x[row * x_stride + c] - mean[row]) * rstd[row]);
-    b += d;
+    const float mu = mean[row], r = rstd[row];
+    float d[kWidth], v[kWidth];
+    load_some<T, kWidth>(dy + row * dy_stride + c, width - c, d);
+    load_some<T, kWidth>(x + row * x_stride + c, width - c, v);
+#pragma unroll
+    for (int i = 0; i < kWidth; ++i) {
+      a[i] += d[i] * ((v[i] - mu) * r);
+      b[i] += d[i];
+    }
   }
   const int pad = norm_part_half(width);
-  part += (long)blockIdx.y * 2 * pad;
-  part[c] = a;
-  part[pad + c] = b;
+  part += (long)blockIdx.y * 2 * pad + c;
+  store_some<float, kWidth>(part, width - c, a);
+  store_some<float, kWidth>(part + pad, width - c, b);
 }
 
 // --------------------------------------------------- partial sums' sum
@@ -441,7 +496,9 @@ void run_types(const NormArgs& a, bool backward, hipStream_t s) {
         (T*)a.dx, a.width, a.dy_stride, a.x_stride);
   if (a.part != nullptr)
     norm_dw_wide_kernel<T>
-        <<<dim3((a.width + 255) / 256, a.parts), 256, 0, s>>>(
+        <<<dim3((a.width + 256 * width_of<T>() - 1) / (256 * width_of<T>()),
+                a.parts),
+           256, 0, s>>>(
             (const T*)a.dy, (const T*)a.x, a.mean, a.rstd, a.part, a.rows,
             a.width, a.dy_stride, a.x_stride);
 }
@@ -458,13 +515,21 @@ hipError_t run_norm(const NormArgs& a, int type, int wtype, bool backward,
 
 }  // namespace
 
-// Rows of partial sums that the backward writes: a workgroup for each set of
-// rows up to four a CU, so that many rows share one row of sums.
+// Rows of partial sums that the backward writes, its workgroups: enough to
+// fill the chip, few enough that their sums stay small beside x. Measured on
+// one MI355X with 64 .. 2048 of them (us with the sums' sum): bf16
+// 131072x256 71, 45, 38 and 44 at 256, 512, 1024 and 2048; 4000x4096 39, 28,
+// 30 and 41; 1000x12544 37, 30, 38 and 54 at 128, 256, 512 and 1024; 500x30000
+// 51, 55, 63 and 85 at 64, 128, 256 and 512.
 extern "C" int layer_norm_parts(long rows, int width, int type) {
   const int per = type == kElemF32 ? 4 : 8;
-  const int at_once = rows_at_once((width + per - 1) / per);
+  const int packets = (width + per - 1) / per;
+  const int at_once = rows_at_once(packets);
   const long sets = (rows + at_once - 1) / at_once;
-  return (int)(sets < 1024 ? sets : 1024);
+  const bool in_registers = packets <= (type == kElemF32 ? 4096 : 2048);
+  const long most = !in_registers ? 64 : packets > 1024 ? 256
+                    : packets > 512 ? 512 : 1024;
+  return (int)(sets < most ? sets : most);
 }
 
 extern "C" hipError_t layer_norm_fwd_launch(const NormArgs* a, int type,

@@ -5,6 +5,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include <algorithm>
 #include <cmath>
@@ -471,20 +472,33 @@ Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& w,
 
 // ----------------------------------------------------------------- AdamW
 
-// Written ranges of memory: sorted, they must not meet.
-struct Written {
-  std::vector<std::pair<uintptr_t, uintptr_t>> ranges;
-  void add(const Tensor& t) {
+// Ranges of memory that a call writes or reads: no written one may meet
+// another.
+struct Ranges {
+  struct Range { uintptr_t from, to; bool written; };
+  std::vector<Range> all;
+  void add(const Tensor& t, bool written) {
     const auto a = (uintptr_t)t.data_ptr();
-    ranges.emplace_back(a, a + (uintptr_t)t.numel() * t.element_size());
+    if (t.numel())
+      all.push_back({a, a + (uintptr_t)t.numel() * t.element_size(), written});
   }
   void check(const char* what) {
-    std::sort(ranges.begin(), ranges.end());
-    for (size_t i = 1; i < ranges.size(); ++i)
-      TORCH_CHECK(ranges[i].first >= ranges[i - 1].second, what,
-                  ": two of the tensors to write share memory");
+    std::sort(all.begin(), all.end(),
+              [](const Range& a, const Range& b) { return a.from < b.from; });
+    uintptr_t written = 0, any = 0;      // where the ranges so far end
+    for (const Range& r : all) {
+      TORCH_CHECK(r.from >= (r.written ? any : written), what,
+                  ": a tensor to write shares memory with another");
+      any = std::max(any, r.to);
+      if (r.written) written = std::max(written, r.to);
+    }
   }
 };
+
+// Autograd sees that a tensor's values have changed.
+void changed(const Tensor& t) {
+  if (!t.is_inference()) torch::autograd::impl::bump_version(t);
+}
 
 constexpr int64_t kBlock8 = 256;
 
@@ -516,8 +530,8 @@ void adamw_step(const Tensors& p, const Tensors& g, const Tensors& m,
               "adamw_step: the step's number and rate are the host's and "
               "would stay the same in every replay of a captured graph");
 
-  Written written;
-  written.ranges.reserve(count * (ms ? 5 : 3));
+  Ranges ranges;
+  ranges.all.reserve(count * (ms ? 6 : 4));
   Tensors copies;               // gradients laid out like their parameter
   std::vector<const void*> grads(count);
   for (size_t i = 0; i < count; ++i) {
@@ -545,14 +559,15 @@ void adamw_step(const Tensors& p, const Tensors& g, const Tensors& m,
                 "tensor ", i, " must have the parameter's strides");
     if (laid_out(g[i])) {
       grads[i] = g[i].data_ptr();
+      ranges.add(g[i], false);
     } else {
       copies.push_back(torch::empty_strided(p[i].sizes(), p[i].strides(),
                                             p[i].options()).copy_(g[i]));
       grads[i] = copies.back().data_ptr();
     }
-    written.add(p[i]);
-    written.add(m[i]);
-    written.add(v[i]);
+    ranges.add(p[i], true);
+    ranges.add(m[i], true);
+    ranges.add(v[i], true);
     if (ms) {
       const int64_t blocks = (p[i].numel() + kBlock8 - 1) / kBlock8;
       for (const Tensor* s : {&(*ms)[i], &(*vs)[i]}) {
@@ -561,11 +576,11 @@ void adamw_step(const Tensors& p, const Tensors& g, const Tensors& m,
                         s->is_contiguous() && s->numel() == blocks,
                     "adamw_step: the scales of tensor ", i, " must be ",
                     blocks, " contiguous bytes");
-        written.add(*s);
+        ranges.add(*s, true);
       }
     }
   }
-  written.check("adamw_step");
+  ranges.check("adamw_step");
 
   AdamWScalars s{};
   s.beta1 = (float)beta1;
@@ -602,6 +617,15 @@ void adamw_step(const Tensors& p, const Tensors& g, const Tensors& m,
                          tv.data(), ms ? tms.data() : nullptr,
                          ms ? tvs.data() : nullptr, tn.data()};
     launched(adamw_launch(&a, &s, type, stream), "adamw_step");
+  }
+  for (size_t i = 0; i < count; ++i) {
+    changed(p[i]);
+    changed(m[i]);
+    changed(v[i]);
+    if (ms) {
+      changed((*ms)[i]);
+      changed((*vs)[i]);
+    }
   }
 }
 

@@ -153,7 +153,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *,
     count as scaled to max_grad_norm where it is above that.
 
     step and lr are the host's, so the call is refused while a stream is
-    captured into a graph. No two tensors to write may share memory.
+    captured into a graph. A tensor to write may share memory with no other.
     """
     beta1, beta2 = betas
     if not 0.0 <= beta1 < 1.0 or not 0.0 <= beta2 < 1.0:

@@ -417,6 +417,9 @@ def test_refusals_on_the_gpu():
                   [t[::2] for t in m], [t[::2] for t in v])):
         with pytest.raises(RuntimeError):
             adamw_step(*args, **HYPER)
+    both = torch.zeros(12, device="cuda")
+    with pytest.raises(RuntimeError, match="shares memory"):
+        adamw_step([both[:8]], [both[4:]], m[:1], v[:1], **HYPER)
     with pytest.raises(RuntimeError):
         adamw_step(p, g, m, v, grad_norm=torch.ones(()), max_grad_norm=1.0,
                    **HYPER)
@@ -455,3 +458,29 @@ def test_other_stream():
     s.synchronize()
     assert all(torch.equal(x, y) for k, j in zip((p, m, v), (a[0], a[2], a[3]))
                for x, y in zip(k, j))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_autograd_sees_the_change(device):
+    """A graph that saved a parameter does not take its new values."""
+    p, g, m, v = tensors([8], torch.float32, device)
+    w = p[0].requires_grad_()
+    x = torch.ones(8, device=device, requires_grad=True)
+    y = (w * x).sum()
+    adamw_step([w], g, m, v, **HYPER)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.backward()
+    with torch.inference_mode():
+        q = [t.detach().clone() for t in (w, g[0], m[0], v[0])]
+        adamw_step(*[[t] for t in q], **HYPER)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_shared_gradient(device):
+    """One tensor may be the gradient of two parameters."""
+    p, g, m, v = tensors([300, 300], torch.float32, device)
+    one = [[t.clone() for t in k] for k in (p, m, v)]
+    adamw_step(p, [g[0], g[0]], m, v, **HYPER)
+    for i in range(2):
+        adamw_step([one[0][i]], [g[0]], [one[1][i]], [one[2][i]], **HYPER)
+        assert torch.equal(p[i], one[0][i])

@@ -268,3 +268,43 @@ def test_other_stream_and_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, layer_norm(new, w, b))
+
+
+@pytest.mark.gpu
+def test_captured_backward():
+    """Forward and backward in one graph, on leaves of its own."""
+    x, w, b, dy = inputs(200, 264, torch.bfloat16, torch.float32, "cuda")
+    leaves = [t.detach().clone().requires_grad_() for t in (x, w, b)]
+
+    def step():
+        y = layer_norm(*leaves)
+        return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in range(3):
+        new = inputs(200, 264, torch.bfloat16, torch.float32, "cuda", seed)
+        with torch.no_grad():
+            leaves[0].copy_(new[0])
+        dy.copy_(new[3])
+        graph.replay()
+        torch.cuda.synchronize()
+        want = run(new[0], w, b, new[3])
+        for t, name in zip(out, ("y", "dx", "dw", "db")):
+            assert torch.equal(t, want[name])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_no_second_gradient(device):
+    x, w, b, dy = inputs(4, 16, torch.float32, torch.float32, device)
+    x.requires_grad_()
+    y = layer_norm(x, w, b)
+    with pytest.raises(RuntimeError):
+        d, = torch.autograd.grad(y, x, dy, create_graph=True)
+        d.sum().backward()

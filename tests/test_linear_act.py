@@ -328,3 +328,45 @@ def test_other_stream_and_graphs():
         torch.cuda.synchronize()
         for act, out in zip(("gelu", "relu"), outs):
             assert torch.equal(out, linear_act(x, w, b, act, r))
+
+
+@pytest.mark.gpu
+def test_captured_backward():
+    """Forward and backward in one graph, on leaves of its own."""
+    args = inputs(300, 500, 250, torch.bfloat16, "cuda")
+    dy = args[4]
+    leaves = [t.detach().clone().requires_grad_() for t in args[:4]]
+
+    def step(x, w, b, r, dy):
+        y = linear_act(x, w, b, "silu", r)
+        return (y.detach(), *torch.autograd.grad(y, (x, w, b, r), dy))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*leaves, dy)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(*leaves, dy)
+    for seed in range(3):
+        new = inputs(300, 500, 250, torch.bfloat16, "cuda", seed + 5)
+        with torch.no_grad():
+            for leaf, t in zip(leaves, new):
+                leaf.copy_(t)
+        dy.copy_(new[4])
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step(*[t.requires_grad_() for t in new[:4]], new[4])
+        for a, b in zip(out, want):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_no_second_gradient(device):
+    x, w, b, r, dy = inputs(4, 16, 8, torch.float32, device)
+    x.requires_grad_()
+    y = linear_act(x, w, b, "gelu", r)
+    with pytest.raises(RuntimeError):
+        d, = torch.autograd.grad(y, x, dy, create_graph=True)
+        d.sum().backward()
