@@ -99,6 +99,21 @@ __device__ inline i32x4 descriptor(const char* base, int bytes) {
   return d;
 }
 
+// Bytes that a step may read of an operand with k consecutive: to the end of
+// the last row's part in it, `left` packets from the row's end. A row of
+// fewer than 128 bytes ends the range earlier, or the rows behind the last
+// one would begin inside it. (A row is never longer than `ld`, so they are
+// outside.)
+constexpr __host__ __device__ int step_range(int rows, int ld, int left) {
+  return (rows - 1) * ld + (left < 0 ? 0 : left * 16 < kRow ? left * 16 : kRow);
+}
+static_assert(step_range(3, 16, 1) == 48 && step_range(1, 16, 1) == 16,
+              "rows of 16 bytes end with their own");
+static_assert(step_range(2, 4096, 8) == 4096 + 128 &&
+                  step_range(2, 4096, 200) == 4096 + 128,
+              "a whole step of long rows");
+static_assert(step_range(2, 176, 3) == 176 + 48, "the last step of rows");
+
 // One operand's tile of kR rows (its own index) and 128 bytes of k.
 template <typename T, bool kTrans, int kR, int kWaves>
 struct Operand {
@@ -162,7 +177,8 @@ struct Operand {
   __device__ Step at_step(int step, int end) const {
     const int k0 = step * kK, left = step < end ? k - k0 : 0;
     if constexpr (!kTrans)
-      return {descriptor(base + (long)step * kRow, (rows - 1) * ld + kRow),
+      return {descriptor(base + (long)step * kRow,
+                         step_range(rows, ld, left / kPer)),
               left / kPer};
     const int rows_k = left < kK ? left : kK;
     return {descriptor(base + (long)k0 * ld,
