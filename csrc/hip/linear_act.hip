@@ -4,11 +4,12 @@
 //   z = x W^T + b      y = act(z) + r
 //   dz = dy act'(z)    dx = dz W           dW = dz^T x      db = sum dz
 //
-// What is kept for the backward, in the tensors' type: ReLU's derivative,
-// taken where z is still in fp32 and so exact; z itself for GELU and SiLU,
-// because z act''(z) stays below 0.32, so that the rounding of z costs the
-// derivative a third of what its own rounding would. dz is rounded once, as
-// the matrix cores take it in that type; db sums it unrounded.
+// What is kept for the backward: act'(z), formed where z is still in fp32, so
+// that no erf or exp is computed twice. With 16-bit tensors it is a 16-bit
+// fixed point number, off by 2^-16 at most, a small part of what dz's one
+// rounding costs (the matrix cores take dz in the tensors' type; db sums it
+// unrounded); in bf16 or fp16 the derivative's own rounding would cost as
+// much again. ReLU's 0 and 1 are exact.
 //
 // All three products are one kernel, D[m][n] = sum_k X(m,k) Y(n,k), where
 // either operand may lie with k consecutive or with its own index
@@ -266,15 +267,10 @@ __device__ inline float activate(float z) {
   return z;
 }
 
-// What the backward needs of z.
-template <int kAct>
-__device__ inline float kept_of(float z) {
-  return kAct == kActRelu ? (z > 0.0f ? 1.0f : 0.0f) : z;
-}
-
-// act'(z) from that.
+// act'(z).
 template <typename T, int kAct>
 __device__ inline float slope_of(float z) {
+  if constexpr (kAct == kActRelu) return z > 0.0f ? 1.0f : 0.0f;
   if constexpr (kAct == kActSilu) {
     const float s = sigmoid(z);
     return s * (1.0f + z * (1.0f - s));
@@ -284,7 +280,22 @@ __device__ inline float slope_of(float z) {
     normal<T>(z, e, cdf);
     return cdf + z * (0.39894228f * e);
   }
-  return z;
+  return 1.0f;
+}
+
+// The derivative as it is kept: fp32 as it is; else in steps of 2^-15 from
+// -1/4 (all of them lie between -0.13 and 1.13), the last number for NaN.
+template <typename T>
+using Kept = std::conditional_t<sizeof(T) == 4, float, unsigned short>;
+
+__device__ inline float keep(float slope, float) { return slope; }
+__device__ inline float keep(float slope, unsigned short) {
+  return slope == slope ? rintf(slope * 32768.0f) + 8192.0f : 65535.0f;
+}
+__device__ inline float kept(float k, float) { return k; }
+__device__ inline float kept(float k, unsigned short) {
+  return k == 65535.0f ? __int_as_float(0x7fc00000)
+                       : (k - 8192.0f) * (1.0f / 32768.0f);
 }
 
 constexpr int kOut = 8;       // consecutive columns that a lane finishes
@@ -322,34 +333,36 @@ __device__ inline void finish(const LinearEpilogue& e, long m, int n, int N,
                               const float (&b)[kOut], Raw<T> raw,
                               float (&z)[kOut]) {
   T* out = (T*)e.y + m * (long)N + n;
-  T* keep = e.kept ? (T*)e.kept + m * (long)N + n : nullptr;
+  using K = Kept<T>;
+  K* slopes = e.kept ? (K*)e.kept + m * (long)N + n : nullptr;
+  if (kAct != kActNone && slopes) {
+    float k[kOut];
+#pragma unroll
+    for (int i = 0; i < kOut; ++i)
+      k[i] = keep(slope_of<T, kAct>(z[i] + b[i]), K{});
+    store_some<K, kOut>(slopes, N - n, k);
+  }
   if (n + kOut <= N) {
     typedef T Res __attribute__((ext_vector_type(kOut)));
     const Res r = __builtin_bit_cast(Res, raw);
-    float kept[kOut];
 #pragma unroll
-    for (int i = 0; i < kOut; ++i) {
-      kept[i] = kept_of<kAct>(z[i] + b[i]);
+    for (int i = 0; i < kOut; ++i)
       z[i] = activate<T, kAct>(z[i] + b[i]) + (float)r[i];
-    }
     store_f32<T, kOut>(out, z);
-    if (kAct != kActNone && keep) store_f32<T, kOut>(keep, kept);
     return;
   }
   const T* res = (const T*)e.residual + m * e.ld_residual + n;
 #pragma unroll
   for (int i = 0; i < kOut; ++i) {
     if (n + i >= N) continue;
-    const float v = z[i] + b[i];
-    out[i] = (T)(activate<T, kAct>(v) +
+    out[i] = (T)(activate<T, kAct>(z[i] + b[i]) +
                  (e.residual ? (float)res[i] : 0.0f));
-    if (kAct != kActNone && keep) keep[i] = (T)kept_of<kAct>(v);
   }
 }
 
 // f(the activation as a constant)
 template <typename F>
-__host__ __device__ inline void with_act(int act, F f) {
+__device__ inline void with_act(int act, F f) {
   switch (act) {
     case kActRelu: f(std::integral_constant<int, kActRelu>{}); break;
     case kActGelu: f(std::integral_constant<int, kActGelu>{}); break;
@@ -579,14 +592,14 @@ __global__ __launch_bounds__(256) void join_kernel(LinearProduct a) {
 
 // --------------------------------------------------- dz, db and alignment
 
-// dz = dy act'(z) with rows of ld_dz values, zeros past n;
+// dz = dy act'(z) (kAct) or dy with rows of ld_dz values, zeros past n;
 // part: a row of column sums of the unrounded dz for each blockIdx.y. A
 // thread has 8 columns, 32 threads a row; 8 rows at a time four deep, whose
 // loads are all in flight.
-template <typename T, int kAct>
+template <typename T, bool kAct>
 __global__ __launch_bounds__(256) void dz_kernel(
-    const T* dy, const T* kept, T* dz, float* part, int m, int n, long ld_dy,
-    int ld_dz, int rows) {
+    const T* dy, const Kept<T>* slopes, T* dz, float* part, int m, int n,
+    long ld_dy, int ld_dz, int rows) {
   constexpr int kDeep = 4;
   __shared__ float lds[8][256 + 8];
   const int c = blockIdx.x * 256 + (threadIdx.x & 31) * 8;
@@ -598,10 +611,10 @@ __global__ __launch_bounds__(256) void dz_kernel(
     for (int d = 0; d < kDeep; ++d) {
       const int row = r + 8 * d;
       const T* p = dy + row * ld_dy + c;
-      const T* q = kept + (long)row * n + c;
+      const Kept<T>* q = slopes + (long)row * n + c;
       if (row >= r1) continue;
       load_some<T, 8>(p, n - c, g[d]);
-      if (kAct != kActNone) load_some<T, 8>(q, n - c, s[d]);
+      if (kAct) load_some<Kept<T>, 8>(q, n - c, s[d]);
     }
 #pragma unroll
     for (int d = 0; d < kDeep; ++d) {
@@ -609,7 +622,7 @@ __global__ __launch_bounds__(256) void dz_kernel(
       if (row >= r1) continue;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        if (kAct != kActNone) g[d][i] *= slope_of<T, kAct>(s[d][i]);
+        if (kAct) g[d][i] *= kept(s[d][i], Kept<T>{});
         sum[i] += g[d][i];
       }
       if (dz) {
@@ -764,12 +777,16 @@ template <typename T>
 static hipError_t run_dz(const LinearDz& a, hipStream_t s) {
   const int rows = (a.m + a.strips - 1) / a.strips;
   const int cols = a.dz && a.ld_dz > a.n ? a.ld_dz : a.n;
-  const auto run = [&](auto act) {
-    dz_kernel<T, act><<<dim3((cols + 255) / 256, a.strips), 256, 0, s>>>(
-        (const T*)a.dy, (const T*)a.kept, (T*)a.dz, a.part, a.m, a.n, a.ld_dy,
-        a.ld_dz, rows);
-  };
-  with_act(a.act, run);
+  const dim3 grid((cols + 255) / 256, a.strips);
+  const auto* kept = (const Kept<T>*)a.kept;
+  if (kept != nullptr)
+    dz_kernel<T, true><<<grid, 256, 0, s>>>((const T*)a.dy, kept, (T*)a.dz,
+                                            a.part, a.m, a.n, a.ld_dy,
+                                            a.ld_dz, rows);
+  else
+    dz_kernel<T, false><<<grid, 256, 0, s>>>((const T*)a.dy, kept, (T*)a.dz,
+                                             a.part, a.m, a.n, a.ld_dy,
+                                             a.ld_dz, rows);
   return hipGetLastError();
 }
 

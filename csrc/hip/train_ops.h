@@ -49,8 +49,8 @@ struct LinearEpilogue {
   const void* bias;        // null: 0
   const void* residual;    // null: 0
   void* y;                 // rows of n values
-  void* kept;              // for the backward, rows of n values, or null:
-                           // ReLU's derivative, else z
+  void* kept;              // act'(z) for the backward, rows of n values of
+                           // fp32 or 16 bits as the tensors, or null
   long ld_residual;
   int act;
 };
@@ -77,7 +77,7 @@ struct LinearDz {
   float* part;             // `strips` rows of norm_part_half(n) column sums,
                            // or null
   long ld_dy;
-  int m, n, ld_dz, strips, act;
+  int m, n, ld_dz, strips;
 };
 
 extern "C" {

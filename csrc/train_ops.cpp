@@ -257,7 +257,9 @@ std::vector<Tensor> linear_fwd(const Tensor& x, const Tensor& w,
   Tensor y = torch::empty(shape, x.options().memory_format(
                                      at::MemoryFormat::Contiguous));
   Tensor kept;
-  if (want_kept && act != kActNone) kept = torch::empty_like(y);
+  if (want_kept && act != kActNone)
+    kept = type == 0 ? torch::empty_like(y)
+                     : torch::empty_like(y, torch::kShort);
   if (M == 0) return {y, kept};
 
   const Operand xo(as_matrix(x, M, K), type, stream);
@@ -329,7 +331,6 @@ std::vector<Tensor> linear_bwd(const Tensor& dy,
   if (z.dz != nullptr || want_db) {
     z.dy = g.data_ptr();
     z.kept = act == kActNone ? nullptr : kept.data_ptr();
-    z.act = (int)act;
     z.ld_dy = ldg;
     z.m = (int)M;
     z.n = (int)N;

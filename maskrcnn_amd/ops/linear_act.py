@@ -41,19 +41,20 @@ def _fwd_torch(x, weight, bias, act, residual):
     y, slope = _act_torch(z, act)
     if residual is not None:
         y = y + residual.to(wide)
-    # For the backward: ReLU's derivative, else z, in x's type.
-    kept = None if act == "none" else \
-        (slope if act == "relu" else z).to(x.dtype)
-    return y.to(x.dtype), kept
+    if act == "none":
+        return y.to(x.dtype), None
+    if x.dtype in (torch.bfloat16, torch.float16):
+        # Steps of 2^-15, as 16 bits hold it; ReLU's 0 and 1 are exact.
+        slope = torch.round(slope * 32768.0) / 32768.0
+    return y.to(x.dtype), slope
 
 
-def _bwd_torch(grad, kept, x, weight, act):
+def _bwd_torch(grad, slope, x, weight):
     wide = torch.float64 if x.dtype == torch.float64 else torch.float32
     n, k = weight.shape
     dz = grad.to(wide).reshape(-1, n)
-    if kept is not None:
-        kept = kept.to(wide).reshape(-1, n)
-        dz = dz * (kept if act == "relu" else _act_torch(kept, act)[1])
+    if slope is not None:
+        dz = dz * slope.reshape(-1, n)
     dx = (dz @ weight.to(wide)).reshape(x.shape)
     dw = dz.t() @ x.to(wide).reshape(dz.shape[0], k)
     return dx.to(x.dtype), dw.to(x.dtype), dz.sum(0).to(x.dtype)
@@ -62,16 +63,15 @@ def _bwd_torch(grad, kept, x, weight, act):
 class _LinearActFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act):
-        y, kept = _fwd_torch(x, weight, bias, act, residual)
-        ctx.save_for_backward(x, weight, kept)
-        ctx.act = act
+        y, slope = _fwd_torch(x, weight, bias, act, residual)
+        ctx.save_for_backward(x, weight, slope)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        x, weight, kept = ctx.saved_tensors
-        grads = (*_bwd_torch(grad, kept, x, weight, ctx.act), grad)
+        x, weight, slope = ctx.saved_tensors
+        grads = (*_bwd_torch(grad, slope, x, weight), grad)
         return (*(g if n else None
                   for g, n in zip(grads, ctx.needs_input_grad)), None)
 
@@ -85,9 +85,10 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor,
     residual: [..., N] or None. All in one type, float32, bfloat16 or
     float16, of any strides; sums are in fp32. activation: "none", "relu",
     "gelu" (by erf) or "silu". Returns a contiguous [..., N] in x's type.
-    In 16 bits z is kept for the backward in that type (ReLU's mask is
-    exact), and its gradient is rounded to it once. The gradients have no
-    gradients (create_graph). On the GPU rows may lie up to 8 MB apart.
+    In 16 bits act'(z) is kept for the backward in steps of 2^-15 (ReLU's is
+    exact), and the gradient of z is rounded to x's type once. The gradients
+    have no gradients (create_graph). On the GPU rows may lie up to 8 MB
+    apart.
     """
     act = _INDEX.get(activation)
     if act is None:

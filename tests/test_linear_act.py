@@ -43,7 +43,7 @@ def check(x, w, b, r, dy, act):
     by at most 2 U (K + 8) of the sum of magnitudes. act has a slope below
     1.13 and the slope one below 0.8 (jumps of ReLU's are allowed where z is
     within its error of 0); erf, exp and the products around them take 8 U.
-    z is kept for the backward rounded to the tensors' type.
+    In 16 bits the derivative is kept in steps of 2^-15.
     """
     dtype = x.dtype
     half = torch.finfo(dtype).eps / 2 * (1 + 2.0 ** -6)
@@ -75,7 +75,9 @@ def check(x, w, b, r, dy, act):
         elif act == "relu":
             es = (z.abs() <= ez).double()
         else:
-            es = 0.8 * (half * z.abs() + ez) + 8 * U * (1 + z.abs()) + tiny
+            es = 0.8 * ez + 8 * U * (1 + z.abs()) + tiny
+            if dtype != torch.float32:
+                es = es + 2.0 ** -16
         dz = D * slope
         edb = D.abs() * es + U * dz.abs()
         edz = edb + half * dz.abs() + tiny
