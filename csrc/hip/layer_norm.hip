@@ -434,10 +434,16 @@ template <typename T, typename W, int kTeam, int kVecs, bool kRagged>
 void run_team(const NormArgs& a, bool backward, hipStream_t s) {
   constexpr int threads = threads_of<kTeam>(), per = threads / kTeam;
   if (!backward) {
-    const unsigned grid = (unsigned)((a.rows + per - 1) / per);
-    norm_fwd_kernel<T, W, kTeam, kVecs, kRagged><<<grid, threads, 0, s>>>(
-        (const T*)a.x, (const W*)a.w, (const W*)a.b, (T*)a.y, a.mean, a.rstd,
-        a.rows, a.width, a.x_stride, a.eps);
+    // A launch has less than 2^32 threads.
+    constexpr long most = (1L << 31) / threads * per;
+    for (long at = 0; at < a.rows; at += most) {
+      const long rows = a.rows - at < most ? a.rows - at : most;
+      const unsigned grid = (unsigned)((rows + per - 1) / per);
+      norm_fwd_kernel<T, W, kTeam, kVecs, kRagged><<<grid, threads, 0, s>>>(
+          (const T*)a.x + at * a.x_stride, (const W*)a.w, (const W*)a.b,
+          (T*)a.y + at * a.width, a.mean ? a.mean + at : nullptr,
+          a.rstd ? a.rstd + at : nullptr, rows, a.width, a.x_stride, a.eps);
+    }
   } else {
     norm_bwd_kernel<T, W, kTeam, kVecs, kRagged><<<a.parts, threads, 0, s>>>(
         (const T*)a.dy, (const T*)a.x, (const W*)a.w, a.mean, a.rstd,

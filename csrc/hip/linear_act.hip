@@ -79,7 +79,7 @@ __device__ inline void load_lds(i32x4 desc, unsigned from, unsigned to) {
       "buffer_load_dwordx4 %1, %2, 0 offen lds"
       :
       : "s"(to), "v"(from), "s"(desc)
-      : "memory");
+      : "memory", "m0");
 }
 
 // All but the latest kLater loads into LDS have arrived and every read of it

@@ -40,8 +40,10 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 // ------------------------------------------------------------ layer norm
 
-// x as rows of consecutive values; a copy only where its strides need one.
-Tensor as_rows(const Tensor& x, int64_t width) {
+// x as rows of consecutive values; a copy only where its strides need one or
+// it is a negative view.
+Tensor as_rows(const Tensor& given, int64_t width) {
+  const Tensor x = given.resolve_neg();
   if (x.dim() == 2 && (x.stride(1) == 1 || width == 1) &&
       (x.stride(0) >= width || x.stride(0) == 0))
     return x;
@@ -84,8 +86,8 @@ std::vector<Tensor> layer_norm_fwd(const Tensor& x, std::optional<Tensor> w,
   if (stats) st = torch::empty({2, rows}, x.options().dtype(torch::kFloat));
   if (rows > 0) {
     const Tensor xr = as_rows(x, width);
-    if (w) w = w->contiguous();
-    if (b) b = b->contiguous();
+    if (w) w = w->resolve_neg().contiguous();
+    if (b) b = b->resolve_neg().contiguous();
     NormArgs a{};
     a.x = xr.data_ptr();
     a.w = w ? w->data_ptr() : nullptr;
@@ -130,7 +132,7 @@ std::vector<Tensor> layer_norm_bwd(const Tensor& dy, const Tensor& x,
     db = rows ? torch::empty({width}, wopts) : torch::zeros({width}, wopts);
   if (rows > 0) {
     const Tensor xr = as_rows(x, width), dyr = as_rows(dy, width);
-    if (w) w = w->contiguous();
+    if (w) w = w->resolve_neg().contiguous();
     NormArgs a{};
     a.dy = dyr.data_ptr();
     a.x = xr.data_ptr();
@@ -177,8 +179,7 @@ struct Operand {
     const int64_t per = 16 / t.element_size();
     rows = (int)t.size(0);
     width = (int)((t.size(1) + per - 1) / per * per);
-    ld = rows > 1 ? t.stride(0) : std::max<int64_t>(t.stride(0), width);
-    if (rows <= 1) ld = (ld + per - 1) / per * per;
+    ld = rows > 1 ? t.stride(0) : width;
     if (t.size(1) == width && ld % per == 0 && aligned16(t.data_ptr()))
       return;
     held = torch::empty({rows, width}, t.options());
@@ -192,7 +193,8 @@ struct Operand {
 };
 
 // Rows with a stride of their own, never overlapping.
-Tensor as_matrix(const Tensor& t, int64_t rows, int64_t width) {
+Tensor as_matrix(const Tensor& given, int64_t rows, int64_t width) {
+  const Tensor t = given.resolve_neg();
   if (t.dim() == 2 && (t.stride(1) == 1 || width <= 1) &&
       (t.stride(0) >= width || t.size(0) <= 1))
     return t;
@@ -201,12 +203,15 @@ Tensor as_matrix(const Tensor& t, int64_t rows, int64_t width) {
 
 constexpr int64_t kMostRows = 1LL << 30;
 
+// A tile's 256 rows of this many bytes are within a descriptor's range.
+bool near(int64_t row) { return row * 256 + 128 < (1LL << 31); }
+
 // `a` with x, y, the extents and the epilogue set.
 void product(LinearProduct& a, int type, const Tensor& like,
              hipStream_t stream) {
   const int64_t row = std::max(a.ldx, a.ldy) * like.element_size();
-  TORCH_CHECK(row * 256 + 128 < (1LL << 31),
-              "linear_act: rows of ", row, " bytes are too far apart");
+  TORCH_CHECK(near(row), "linear_act: rows of ", row,
+              " bytes are too far apart");
   linear_plan(&a, type);
   Tensor part;
   if (a.splits > 1) {
@@ -235,6 +240,8 @@ std::vector<Tensor> linear_fwd(const Tensor& x, const Tensor& w,
   for (size_t i = 0; i + 1 < shape.size(); ++i) M *= shape[i];
   TORCH_CHECK(M <= kMostRows && N <= kMostRows && K <= kMostRows,
               "linear_act: more than 2^30 rows or columns");
+  TORCH_CHECK(!want_kept || near((N + 7) * x.element_size()),
+              "linear_act: ", N, " columns are too many for the gradients");
   const auto like_x = [&](const Tensor& t, const char* name) {
     TORCH_CHECK(t.device() == x.device() &&
                     t.scalar_type() == x.scalar_type(),
@@ -277,7 +284,7 @@ std::vector<Tensor> linear_fwd(const Tensor& x, const Tensor& w,
   a.e.y = y.data_ptr();
   a.e.kept = kept.defined() ? kept.data_ptr() : nullptr;
   if (bias) {
-    b = bias->contiguous();
+    b = bias->resolve_neg().contiguous();
     a.e.bias = b.data_ptr();
   }
   if (residual) {
@@ -318,7 +325,7 @@ std::vector<Tensor> linear_bwd(const Tensor& dy,
   const long ldg = M > 1 ? g.stride(0) : Np;
   const bool products = want_dx || want_dw;
   const bool as_is = act == kActNone && N == Np && ldg % per == 0 &&
-                     aligned16(g.data_ptr());
+                     near(ldg * x.element_size()) && aligned16(g.data_ptr());
   Tensor dz = g;
   long ld_dz = ldg;
   LinearDz z{};
@@ -384,6 +391,29 @@ std::vector<Tensor> linear_bwd(const Tensor& dy,
   return {dx, dw, db};
 }
 
+bool is_capturing(hipStream_t stream, const char* what) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  launched(hipStreamIsCapturing(stream, &status), what);
+  return status != hipStreamCaptureStatusNone;
+}
+
+// A leaf's gradient goes through the accumulator that a live graph of it
+// holds, on the stream where that was made. In the capture of a backward this
+// would tie another stream to the captured one, which ends the process.
+void check_accumulators(const torch::autograd::variable_list& leaves,
+                        const char* what) {
+  const auto stream = c10::hip::getCurrentHIPStream();
+  if (!is_capturing(stream.stream(), what)) return;
+  for (const Tensor& t : leaves) {
+    if (!t.defined() || !t.is_leaf() || !t.requires_grad()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+    const auto at = node ? node->stream() : std::nullopt;
+    TORCH_CHECK(!at || at->id() == stream.unwrap().id(), what,
+                ": a captured backward of a leaf that an earlier graph, made "
+                "on another stream, still holds; free that graph first");
+  }
+}
+
 // The autograd nodes are in C++: small layers are bound by the host's time.
 class LinearActNode
     : public torch::autograd::Function<LinearActNode> {
@@ -393,7 +423,8 @@ class LinearActNode
                         const std::optional<Tensor>& bias,
                         const std::optional<Tensor>& residual, int64_t act) {
     auto out = linear_fwd(x, w, bias, act, residual, true);
-    ctx->save_for_backward({x, w, out[1]});
+    const bool leaf = bias && bias->is_leaf();
+    ctx->save_for_backward({x, w, out[1], leaf ? *bias : Tensor()});
     // The edges are the given tensors' alone: which there are goes with act.
     ctx->saved_data["act"] = act | (bias ? 8 : 0) | (residual ? 16 : 0);
     return out[0];
@@ -405,6 +436,7 @@ class LinearActNode
     TORCH_CHECK(!at::GradMode::is_enabled(),
                 "linear_act: its gradients have no gradient (create_graph)");
     const auto saved = ctx->get_saved_variables();
+    check_accumulators({saved[0], saved[1], saved[3]}, "linear_act");
     const int64_t act = ctx->saved_data["act"].toInt();
     const bool bias = act & 8, residual = act & 16;
     auto g = linear_bwd(grads[0], saved[2], saved[0], saved[1], act & 7,
@@ -435,7 +467,9 @@ class LayerNormNode : public torch::autograd::Function<LayerNormNode> {
                         const Tensor& x, const std::optional<Tensor>& w,
                         const std::optional<Tensor>& b, double eps) {
     auto out = layer_norm_fwd(x, w, b, eps, true);
-    ctx->save_for_backward({x, w ? *w : Tensor(), out[1]});
+    const bool leaf = b && b->is_leaf();
+    ctx->save_for_backward(
+        {x, w ? *w : Tensor(), out[1], leaf ? *b : Tensor()});
     // The edges are the given tensors' alone: which there are goes with the
     // parameters' type.
     ctx->saved_data["given"] =
@@ -451,6 +485,7 @@ class LayerNormNode : public torch::autograd::Function<LayerNormNode> {
     TORCH_CHECK(!at::GradMode::is_enabled(),
                 "layer_norm: its gradients have no gradient (create_graph)");
     const auto saved = ctx->get_saved_variables();
+    check_accumulators({saved[0], saved[1], saved[3]}, "layer_norm");
     const int64_t given = ctx->saved_data["given"].toInt();
     const bool weight = given & 256, bias = given & 512;
     auto g = layer_norm_bwd(
@@ -525,9 +560,7 @@ void adamw_step(const Tensors& p, const Tensors& g, const Tensors& m,
                 "parameters' device");
   const c10::DeviceGuard guard(device);
   const hipStream_t stream = current();
-  hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
-  launched(hipStreamIsCapturing(stream, &capturing), "adamw_step");
-  TORCH_CHECK(capturing == hipStreamCaptureStatusNone,
+  TORCH_CHECK(!is_capturing(stream, "adamw_step"),
               "adamw_step: the step's number and rate are the host's and "
               "would stay the same in every replay of a captured graph");
 
@@ -549,8 +582,10 @@ void adamw_step(const Tensors& p, const Tensors& g, const Tensors& m,
     TORCH_CHECK(g[i].sizes() == p[i].sizes() && m[i].sizes() == p[i].sizes() &&
                     v[i].sizes() == p[i].sizes(),
                 "adamw_step: tensor ", i, ": sizes differ");
-    TORCH_CHECK(p[i].is_non_overlapping_and_dense(), "adamw_step: parameter ",
-                i, " must be dense");
+    TORCH_CHECK(p[i].is_non_overlapping_and_dense() && !p[i].is_neg() &&
+                    !m[i].is_neg() && !v[i].is_neg(),
+                "adamw_step: parameter ", i, " must be dense, and it and its "
+                "states no negative views");
     elem_type(p[i], "adamw_step");
     const bool plain = p[i].is_contiguous();
     const auto laid_out = [&](const Tensor& t) {
@@ -558,7 +593,7 @@ void adamw_step(const Tensors& p, const Tensors& g, const Tensors& m,
     };
     TORCH_CHECK(laid_out(m[i]) && laid_out(v[i]), "adamw_step: the states of "
                 "tensor ", i, " must have the parameter's strides");
-    if (laid_out(g[i])) {
+    if (laid_out(g[i]) && !g[i].is_neg()) {
       grads[i] = g[i].data_ptr();
       ranges.add(g[i], false);
     } else {
@@ -645,7 +680,7 @@ Tensor grad_norm(const Tensors& g) {
     const int type = elem_type(t, "grad_norm");
     TORCH_CHECK(!t.is_sparse(), "grad_norm: a tensor is sparse");
     if (t.numel() == 0) continue;
-    if (t.is_non_overlapping_and_dense()) {
+    if (t.is_non_overlapping_and_dense()) {   // a sign changes no square
       at[type].push_back(t.data_ptr());
     } else {
       dense.push_back(t.contiguous());
@@ -673,7 +708,7 @@ Tensor grad_norm(const Tensors& g) {
 
 std::tuple<Tensor, Tensor> pack_state8(const Tensor& x, bool is_signed) {
   TORCH_CHECK(x.is_cuda() && x.scalar_type() == torch::kFloat &&
-                  x.is_non_overlapping_and_dense(),
+                  x.is_non_overlapping_and_dense() && !x.is_neg(),
               "pack_state8: a dense float32 tensor on GPU");
   const c10::DeviceGuard guard(x.device());
   Tensor codes = torch::empty_strided(x.sizes(), x.strides(),

@@ -69,6 +69,9 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor = None,
     """
     if x.is_cuda:
         return require_ext().layer_norm(x, weight, bias, eps)
+    if not x.is_floating_point():
+        raise RuntimeError(f"layer_norm: float32, bfloat16 or float16, not "
+                           f"{x.dtype}")
     if x.dim() < 1 or x.shape[-1] < 1:
         raise RuntimeError("layer_norm: the last dimension is empty")
     for name, t in (("weight", weight), ("bias", bias)):

@@ -96,6 +96,9 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor,
                          f"of {ACTIVATIONS}")
     if x.is_cuda:
         return require_ext().linear_act(x, weight, bias, act, residual)
+    if not x.is_floating_point():
+        raise RuntimeError(f"linear_act: float32, bfloat16 or float16, not "
+                           f"{x.dtype}")
     if x.dim() < 1 or weight.dim() != 2 or not weight.shape[0] or \
             weight.shape[1] != x.shape[-1]:
         raise RuntimeError(

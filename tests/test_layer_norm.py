@@ -308,3 +308,57 @@ def test_no_second_gradient(device):
     with pytest.raises(RuntimeError):
         d, = torch.autograd.grad(y, x, dy, create_graph=True)
         d.sum().backward()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_whole_numbers_are_refused(device):
+    with pytest.raises(RuntimeError):
+        layer_norm(torch.ones(2, 8, dtype=torch.int32, device=device))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_negative_views(device):
+    x, w, b, dy = inputs(6, 16, torch.float32, torch.float32, device)
+
+    def neg(t):
+        held = torch.complex(torch.zeros_like(t), -t).conj().imag
+        assert held.is_neg()
+        return held
+    want, got = run(x, w, b, dy), run(neg(x), neg(w), neg(b), neg(dy))
+    assert all(torch.equal(want[k], got[k]) for k in want)
+
+
+@pytest.mark.gpu
+def test_more_rows_than_one_launch_has():
+    rows = (1 << 28) + 37
+    x = torch.zeros(rows, 2, dtype=torch.bfloat16, device="cuda")
+    x[::5, 0] = 4.0
+    y = layer_norm(x)
+    for part in (slice(0, 100), slice((1 << 28) - 50, rows)):
+        assert torch.equal(y[part], layer_norm(x[part].clone()))
+    assert int((y[:, 0] > 0.5).sum()) == -(-rows // 5)
+
+
+@pytest.mark.gpu
+def test_captured_backward_of_a_held_leaf():
+    """An earlier graph of a leaf, on another stream, is refused."""
+    x, w, b, dy = inputs(40, 64, torch.bfloat16, torch.float32, "cuda")
+    for i in range(3):
+        leaves = [t.detach().clone().requires_grad_(i == j)
+                  for j, t in enumerate((x, w, b))]
+        held = layer_norm(*leaves)
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="free that graph"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                y = layer_norm(*leaves)
+                torch.autograd.grad(y, leaves[i], dy)
+        want, = torch.autograd.grad(held, leaves[i], dy)
+        del held, y
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = layer_norm(*leaves)
+            got, = torch.autograd.grad(y, leaves[i], dy)
+        for _ in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)

@@ -372,3 +372,64 @@ def test_no_second_gradient(device):
     with pytest.raises(RuntimeError):
         d, = torch.autograd.grad(y, x, dy, create_graph=True)
         d.sum().backward()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_negative_views(device):
+    """An imaginary part of a conjugate is a view that negates lazily."""
+    x, w, b, r, dy = inputs(6, 16, 8, torch.float32, device)
+    held = []
+    for t in (x, w, b, r, dy):
+        c = torch.complex(torch.zeros_like(t), -t).conj()
+        assert c.imag.is_neg()
+        held.append(c.imag)
+    check(*held, "gelu")
+
+
+@pytest.mark.gpu
+def test_far_rows_where_they_do_not_matter():
+    """One row has no distance, and a gradient's strides are not the
+    caller's."""
+    x, w, b, r, dy = inputs(2, 16, 8, torch.bfloat16, "cuda")
+    far = torch.empty_strided((2, 16), (1 << 23, 1), dtype=x.dtype,
+                              device="cuda")
+    far.copy_(x)
+    assert torch.equal(linear_act(far[:1], w, b), linear_act(x[:1], w, b))
+    assert torch.equal(linear_act(x, far[1:], b[:1]),
+                       linear_act(x, x[1:], b[:1]))
+    wide = far.as_strided((2, 8), far.stride())
+    wide.copy_(dy)
+    check(x, w, b, r, wide, "none")
+    check(x, w, b, r, wide, "silu")
+
+
+@pytest.mark.gpu
+def test_captured_backward_of_a_held_leaf():
+    """An earlier graph of a leaf, on another stream, is refused."""
+    x, w, b, r, dy = inputs(40, 64, 32, torch.bfloat16, "cuda")
+    for i in range(3):
+        leaves = [t.detach().clone().requires_grad_(i == j)
+                  for j, t in enumerate((x, w, b))]
+        held = linear_act(*leaves, "gelu")
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="free that graph"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                y = linear_act(*leaves, "gelu")
+                torch.autograd.grad(y, leaves[i], dy)
+        want, = torch.autograd.grad(held, leaves[i], dy)
+        del held, y
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = linear_act(*leaves, "gelu")
+            got, = torch.autograd.grad(y, leaves[i], dy)
+        for _ in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_whole_numbers_are_refused(device):
+    x = torch.ones(2, 8, dtype=torch.int32, device=device)
+    with pytest.raises(RuntimeError):
+        linear_act(x, x)
