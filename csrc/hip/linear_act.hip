@@ -373,12 +373,13 @@ __device__ inline void with_act(int act, F f) {
 
 // ------------------------------------------------------------------ kernel
 
-// Two waves a SIMD have 256 registers each, which holds the sums in ordinary
-// ones: with more, the compiler moves hundreds of sums between the two kinds
-// in each step.
+// kWM x kWN waves over the tile, in kGroups that each take a part of the
+// steps, with buffers of their own. Two waves a SIMD have 256 registers each,
+// which holds the sums in ordinary ones: with more, the compiler moves
+// hundreds of sums between the two kinds in each step.
 template <typename T, bool kXT, bool kYT, int kBM, int kBN, int kWM, int kWN,
-          int kAhead>
-__global__ __launch_bounds__(kWM * kWN * 64, 2) void product_kernel(
+          int kGroups, int kAhead>
+__global__ __launch_bounds__(kWM * kWN * kGroups * 64, 2) void product_kernel(
     LinearProduct a) {
   constexpr int kWaves = kWM * kWN;
   using X = Operand<T, kXT, kBM, kWaves>;
@@ -386,7 +387,7 @@ __global__ __launch_bounds__(kWM * kWN * 64, 2) void product_kernel(
   constexpr int kMI = kBM / kWM / 16, kNI = kBN / kWN / 16;
   constexpr int kYAt = (kAhead + 1) * X::kBytes;
   constexpr int kLds = kYAt + kAhead * Y::kBytes;
-  __shared__ __attribute__((aligned(1024))) char lds[kLds];
+  __shared__ __attribute__((aligned(1024))) char lds_all[kGroups * kLds];
 
   // Workgroups go round the 8 chiplets; each gets a consecutive run of tiles,
   // blocks of `group` rows of tiles by all columns, down the rows first, so
@@ -402,7 +403,9 @@ __global__ __launch_bounds__(kWM * kWN * 64, 2) void product_kernel(
   const int m0 = (block * a.group + in % deep) * kBM, n0 = in / deep * kBN;
 
   const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int id_wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int group = id_wave / kWaves, wave = id_wave % kWaves;
+  char* lds = lds_all + group * kLds;
   const int xr = wave / kWN * (kBM / kWM), yr = wave % kWN * (kBN / kWN);
   X x;
   Y y;
@@ -410,10 +413,16 @@ __global__ __launch_bounds__(kWM * kWN * 64, 2) void product_kernel(
   y.init(a.y, a.ldy, n0, a.ext_y, a.ky, wave, lane);
 
   const int steps = (a.kx + X::kK - 1) / X::kK;
-  const int first = split * a.steps_per_split;
-  const int last = first + a.steps_per_split < steps
-                       ? first + a.steps_per_split : steps;
-  const unsigned at_lds = (unsigned)(unsigned long)(lds_char*)&lds[0];
+  const int first_all = split * a.steps_per_split;
+  const int last_all = first_all + a.steps_per_split < steps
+                           ? first_all + a.steps_per_split : steps;
+  // All groups take as many turns, the last ones perhaps past their steps,
+  // where they get zeros.
+  const int turns = (last_all - first_all + kGroups - 1) / kGroups;
+  const int first = first_all + group * turns;
+  const int last = first + turns < last_all ? first + turns : last_all;
+  const unsigned at_lds =
+      (unsigned)(unsigned long)(lds_char*)&lds_all[0] + group * kLds;
 
   f32x4 acc[kMI][kNI] = {};
   i32x4 xf[2][kMI], yf[2][kNI];
@@ -457,7 +466,7 @@ __global__ __launch_bounds__(kWM * kWN * 64, 2) void product_kernel(
   // the next step has arrived and no wave still reads this one.
   constexpr int kReads = (kMI + kNI + kMI - 1) / kMI < 2
                              ? 2 : (kMI + kNI + kMI - 1) / kMI;
-  for (int s = first; s < last; ++s) {
+  for (int s = first; s < first + turns; ++s) {
     const auto xs = x.at_step(s + kAhead, last);
 #pragma unroll
     for (int i = 0; i < kMI; ++i) {
@@ -500,6 +509,25 @@ __global__ __launch_bounds__(kWM * kWN * 64, 2) void product_kernel(
   static_assert(kParts > 0 && kParts <= kFit, "a wave's share of LDS");
   constexpr int kLanes = kCols / kOut;                     // of one row
   arrived<0>();
+  if constexpr (kGroups > 1) {
+    // The first group gets the others' sums, a lane the ones of its own place.
+    constexpr int kSums = kMI * kNI * 64 * 16;             // bytes of a wave
+    static_assert(kWaves * kSums <= kLds, "a group's sums in its buffers");
+    if (group > 0) {
+#pragma unroll
+      for (int i = 0; i < kMI * kNI; ++i)
+        *(f32x4*)(lds + wave * kSums + (i * 64 + lane) * 16) =
+            acc[i / kNI][i % kNI];
+    }
+    arrived<0>();
+    if (group > 0) return;
+#pragma unroll
+    for (int g = 1; g < kGroups; ++g)
+#pragma unroll
+      for (int i = 0; i < kMI * kNI; ++i)
+        acc[i / kNI][i % kNI] += *(const f32x4*)(
+            lds + g * kLds + wave * kSums + (i * 64 + lane) * 16);
+  }
   char* mine = lds + wave * (kParts * 16 * kCols * 4);
   const int c = lane % kLanes, n = n0 + yr + c * kOut;
   constexpr int kTurns = kParts * 16 * kLanes / 64;        // of 64 lanes
@@ -675,20 +703,22 @@ void run_tiles(const LinearProduct& a, hipStream_t s) {
                                    ((a.n + a.tile - 1) / a.tile) * a.splits);
   if constexpr (sizeof(T) == 2) {
     if (a.tile == 256) {
-      product_kernel<T, kXT, kYT, 256, 256, 2, 4, 2><<<grid, 512, 0, s>>>(a);
+      product_kernel<T, kXT, kYT, 256, 256, 2, 4, 1, 2><<<grid, 512, 0, s>>>(a);
       return;
     }
   }
   // A workgroup that has its CU to itself takes more LDS and looks further
-  // ahead; otherwise the others' work covers its waits.
+  // ahead, with the small tile also in two groups of waves that halve its
+  // steps (bf16 1024x1024x3999 22.3 -> 17.6 us, 100x1024x81 8.3 -> 7.2; with
+  // the 128-wide tile no gain); otherwise the others' work covers its waits.
   if (a.tile == 128 && grid <= 256)
-    product_kernel<T, kXT, kYT, 128, 128, 2, 4, 4><<<grid, 512, 0, s>>>(a);
+    product_kernel<T, kXT, kYT, 128, 128, 2, 4, 1, 4><<<grid, 512, 0, s>>>(a);
   else if (a.tile == 128)
-    product_kernel<T, kXT, kYT, 128, 128, 2, 4, 2><<<grid, 512, 0, s>>>(a);
+    product_kernel<T, kXT, kYT, 128, 128, 2, 4, 1, 2><<<grid, 512, 0, s>>>(a);
   else if (grid <= 256)
-    product_kernel<T, kXT, kYT, 64, 64, 2, 2, 6><<<grid, 256, 0, s>>>(a);
+    product_kernel<T, kXT, kYT, 64, 64, 2, 2, 2, 4><<<grid, 512, 0, s>>>(a);
   else
-    product_kernel<T, kXT, kYT, 64, 64, 2, 2, 2><<<grid, 256, 0, s>>>(a);
+    product_kernel<T, kXT, kYT, 64, 64, 2, 2, 1, 2><<<grid, 256, 0, s>>>(a);
 }
 
 template <typename T>
@@ -725,7 +755,7 @@ extern "C" void linear_plan(LinearProduct* a, int type) {
   struct Shape { int tile; double step, alone, rest; };
   static const Shape kHalf[] = {{256, 1.55, 1.55, 6.0},
                                 {128, 0.55, 0.55, 2.5},
-                                {64, 0.25, 0.30, 1.0}};
+                                {64, 0.25, 0.22, 1.0}};
   static const Shape kFull[] = {{128, 1.8, 1.8, 2.5}, {64, 0.5, 0.5, 1.0}};
   const Shape* shapes = type == kElemF32 ? kFull : kHalf;
   const int count = type == kElemF32 ? 2 : 3;
