@@ -255,32 +255,26 @@ __device__ inline float sigmoid(float z) {
   return __builtin_amdgcn_rcpf(1.0f + __expf(-z));
 }
 
+// act(z); slope: act'(z), of the same exponential.
 template <typename T, int kAct>
-__device__ inline float activate(float z) {
-  if constexpr (kAct == kActRelu) return z < 0.0f ? 0.0f : z;   // NaN stays
-  if constexpr (kAct == kActSilu) return z * sigmoid(z);
-  if constexpr (kAct == kActGelu) {
-    float e, cdf;
-    normal<T>(z, e, cdf);
-    return z * cdf;
+__device__ inline float activate(float z, float& slope) {
+  if constexpr (kAct == kActRelu) {
+    slope = z > 0.0f ? 1.0f : 0.0f;
+    return z < 0.0f ? 0.0f : z;                             // NaN stays
   }
-  return z;
-}
-
-// act'(z).
-template <typename T, int kAct>
-__device__ inline float slope_of(float z) {
-  if constexpr (kAct == kActRelu) return z > 0.0f ? 1.0f : 0.0f;
   if constexpr (kAct == kActSilu) {
     const float s = sigmoid(z);
-    return s * (1.0f + z * (1.0f - s));
+    slope = s * (1.0f + z * (1.0f - s));
+    return z * s;
   }
   if constexpr (kAct == kActGelu) {
     float e, cdf;
     normal<T>(z, e, cdf);
-    return cdf + z * (0.39894228f * e);
+    slope = cdf + z * (0.39894228f * e);
+    return z * cdf;
   }
-  return 1.0f;
+  slope = 1.0f;
+  return z;
 }
 
 // The derivative as it is kept: fp32 as it is; else in steps of 2^-15 from
@@ -335,29 +329,33 @@ __device__ inline void finish(const LinearEpilogue& e, long m, int n, int N,
   T* out = (T*)e.y + m * (long)N + n;
   using K = Kept<T>;
   K* slopes = e.kept ? (K*)e.kept + m * (long)N + n : nullptr;
+  float slope;
   if (kAct != kActNone && slopes) {
     float k[kOut];
 #pragma unroll
-    for (int i = 0; i < kOut; ++i)
-      k[i] = keep(slope_of<T, kAct>(z[i] + b[i]), K{});
+    for (int i = 0; i < kOut; ++i) {
+      z[i] = activate<T, kAct>(z[i] + b[i], slope);
+      k[i] = keep(slope, K{});
+    }
     store_some<K, kOut>(slopes, N - n, k);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kOut; ++i)
+      z[i] = activate<T, kAct>(z[i] + b[i], slope);
   }
   if (n + kOut <= N) {
     typedef T Res __attribute__((ext_vector_type(kOut)));
     const Res r = __builtin_bit_cast(Res, raw);
 #pragma unroll
-    for (int i = 0; i < kOut; ++i)
-      z[i] = activate<T, kAct>(z[i] + b[i]) + (float)r[i];
+    for (int i = 0; i < kOut; ++i) z[i] += (float)r[i];
     store_f32<T, kOut>(out, z);
     return;
   }
   const T* res = (const T*)e.residual + m * e.ld_residual + n;
 #pragma unroll
-  for (int i = 0; i < kOut; ++i) {
-    if (n + i >= N) continue;
-    out[i] = (T)(activate<T, kAct>(z[i] + b[i]) +
-                 (e.residual ? (float)res[i] : 0.0f));
-  }
+  for (int i = 0; i < kOut; ++i)
+    if (n + i < N)
+      out[i] = (T)(z[i] + (e.residual ? (float)res[i] : 0.0f));
 }
 
 // f(the activation as a constant)
