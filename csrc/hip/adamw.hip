@@ -30,6 +30,12 @@
 // 8-bit states, some 60 and 120 vector instructions. One thread holds 4
 // consecutive values (16-byte accesses; with 8-bit states a wave is exactly
 // one block of 256, whose maximum is a wave reduction).
+//
+// Measured on one MI355X with the 63.8 million parameters of the 101-layer
+// detector in fp32: the norm 55 us and the step 285 us (1.79 GB, 6.2 TB/s; a
+// part of the gradients comes from the memory-side cache), 412 together
+// before p, m and v went past the caches. With 8-bit states the step takes
+// 200 us (1.02 GB, 5.1 TB/s).
 #include <hip/hip_runtime.h>
 
 #include "train_ops.h"
@@ -437,14 +443,14 @@ extern "C" hipError_t adamw_launch(const AdamWTensors* a,
                                    hipStream_t stream) {
   const Hyper h{s->beta1, s->one_minus_beta1, s->beta2, s->one_minus_beta2,
                 s->eps, s->decay, s->rate, s->inv_bc2, s->max_norm, s->norm};
-  // Four passes a workgroup amortise its search for the tensor; few values
-  // are spread over more workgroups instead.
-  long values = 0;
-  for (int i = 0; i < a->count; ++i) values += a->n[i];
-  const int passes = values >= 1024L * kPasses * kPass ? kPasses : 1;
   const int most = a->ms == nullptr ? kTensors32 : kTensors8;
   for (int to = a->count; to > 0;) {
     const int from = to > most ? to - most : 0;
+    // Four passes a workgroup amortise its search for the tensor; few values
+    // are spread over more workgroups instead.
+    long values = 0;
+    for (int i = from; i < to; ++i) values += a->n[i];
+    const int passes = values >= 1024L * kPasses * kPass ? kPasses : 1;
     if (a->ms == nullptr) {
       Table32<kTensors32> t;
       const int wg = fill(t, *a, from, to, passes);

@@ -18,11 +18,12 @@
 //   dW: X = dz, Y = x (both with their own index consecutive).
 //
 // A workgroup computes a kBM x kBN tile, waves in a grid over it. Each step
-// takes 128 bytes of k from both operands through LDS (with the largest tile three
-// buffers of X and two of Y, all of a CU's LDS): memory to LDS directly, 16
-// bytes a lane, loads in flight for one to two steps or more; the next half
-// step's fragments are read from LDS during this half's products. The bounds
-// are the buffer descriptor's: rows and columns past the end read as 0. Lanes of one load go to consecutive LDS
+// takes 128 bytes of k from both operands through LDS, from memory directly,
+// 16 bytes a lane, kAhead steps ahead: kAhead + 1 buffers of X and kAhead of
+// Y, since X's next loads go where the last step's were and Y's where this
+// step's first half was. The next half step's fragments are read from LDS
+// during this half's products. The bounds are the buffer descriptor's: rows
+// and columns past the end read as 0. Lanes of one load go to consecutive LDS
 // addresses, so what would be a column of equal banks is spread by choosing
 // which 16 bytes a lane fetches (an exclusive or with the row's bits).
 // Operands with k consecutive are read from LDS 16 bytes a lane; with 16-bit
@@ -32,6 +33,20 @@
 //
 // Few tiles: the k axis is split, partial sums go to memory in fp32 and a
 // second kernel adds them in order and applies the epilogue.
+//
+// What bounds it, measured on one MI355X in bf16 (times of a kernel):
+//   256-wide tiles: the matrix cores and the card's power. 32000x12544x1024
+//     with bias and ReLU 620 us, 1330 TFLOP/s; products without any load
+//     reach 1450 to 1530 on such data, the library's product alone 1250. The
+//     matrix cores are busy 73% of the cycles, LDS has no bank conflicts.
+//     Four waves of 512 registers were slower than eight of 256.
+//   128-wide tiles: LDS. In a step 8 waves read 96 KB of it and the loads
+//     write 32 KB, 1024 cycles at 128 bytes each, for 515 cycles of products:
+//     0.55 us, 975 TFLOP/s. 1000x12544x1024 in 4 splits 32 us and 5 to add
+//     them up; the library 45.
+//   64-wide tiles and few steps: the latency of loads and of the launch;
+//     100x1024x81 7.2 us, of which a launch of one step takes 5.
+//   fp32: the matrix cores, 126 to 136 TFLOP/s, as the library's.
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
