@@ -81,15 +81,19 @@ struct TableNorm {
   int count;
 };
 
-// The last tensor whose first workgroup is not above `wg`.
+// The last tensor whose first workgroup is not above `wg`: a lane compares
+// one tensor's, all at a time, as the table is far away.
 template <typename Table>
 __device__ inline int find_tensor(const Table& t, int wg) {
-  int lo = 0, hi = t.count - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (t.first[mid] <= wg) lo = mid; else hi = mid - 1;
+  constexpr int most = sizeof(t.first) / sizeof(t.first[0]);
+  int k = -1;
+#pragma unroll
+  for (int i = 0; i < most; i += 64) {
+    const int at = i + (threadIdx.x & 63);
+    const int first = t.first[at < most ? at : most - 1];
+    k += __popcll(__ballot(at < t.count && first <= wg));
   }
-  return lo;
+  return __builtin_amdgcn_readfirstlane(k);
 }
 
 struct Hyper {
