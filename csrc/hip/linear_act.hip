@@ -44,7 +44,8 @@
 //     write 32 KB, 1024 cycles at 128 bytes each, for 515 cycles of products:
 //     0.55 us, 975 TFLOP/s. 1000x12544x1024 in 4 splits 32 us and 5 to add
 //     them up; the library 45.
-//   64-wide tiles and few steps: the latency of loads and of the launch;
+//   64-wide tiles: with many steps the L2s, which give 20 TB/s (dW of
+//     3999x1024x1024 17 us); with few the latency of loads and of the launch:
 //     100x1024x81 7.2 us, of which a launch of one step takes 5.
 //   fp32: the matrix cores, 126 to 136 TFLOP/s, as the library's.
 #include <hip/hip_runtime.h>
@@ -156,10 +157,14 @@ struct Operand {
   static __device__ int twist(int r) {
     if constexpr (!kTrans) return (r >> 1) & 7;
     // The rows of k that one read takes fall on different banks: 8 g + 0..3
-    // for 16-bit types, 4 g for fp32.
-    const int f = sizeof(T) == 2 ? (r & 3) | ((r >> 3) & 1) << 2
-                                 : (r >> 2) & 3;
-    return f & (kUnits - 1);
+    // for 16-bit types, two g at a time, 4 g for fp32. Rows of 128 bytes lie
+    // on the two halves of the banks in turn, which is the lowest bit.
+    const int g = (r >> 3) & 1;
+    const int f = sizeof(T) == 4 ? (r >> 2) & 3
+                  : kUnits == 4  ? ((r >> 1) & 1) | g << 1
+                                 : (r & 3) | g << 2;
+    static_assert(kUnits == 4 || kUnits >= 8, "f is below the units");
+    return f;
   }
 
   __device__ void init(const void* p, long ld_values, int first, int total,
