@@ -336,33 +336,29 @@ __global__ __launch_bounds__(kThreads) void pack8_kernel(
   store_block8<kSigned>(codes + i, scales + b, left, f);
 }
 
-// 16 values a thread.
-constexpr int kUnpack = 16;
+// 16 bytes of the result a thread, four times: a wave's accesses lie together,
+// and past the caches no line is written in parts. (The result is larger than
+// what the caches should give up for it.)
+constexpr int kUnpackTimes = 4;
+template <typename T>
+constexpr int unpack_of() { return kUnpackTimes * kThreads * (16 / (int)sizeof(T)); }
+
 template <bool kSigned, typename T>
 __global__ __launch_bounds__(kThreads) void unpack8_kernel(
     const unsigned char* codes, const unsigned char* scales, T* out, long n) {
-  const long i = ((long)blockIdx.x * kThreads + threadIdx.x) * kUnpack;
-  if (i >= n) return;
-  const float e = scale8(scales[i / kBlock8]);
-  if (i + kUnpack <= n) {
-    unsigned w[kUnpack / 4];
-    __builtin_memcpy(w, codes + i, kUnpack);
-    constexpr int kStore = 16 / sizeof(T);       // values of 16 bytes
-    float f[kUnpack];
+  constexpr int kStore = 16 / sizeof(T);
+  const long first = (long)blockIdx.x * unpack_of<T>() + threadIdx.x * kStore;
 #pragma unroll
-    for (int j = 0; j < kUnpack; ++j)
-      f[j] = decode8<kSigned>((w[j / 4] >> (8 * (j % 4))) & 255u, e);
+  for (int d = 0; d < kUnpackTimes; ++d) {
+    const long i = first + d * kThreads * kStore;
+    if (i >= n) return;
+    const float e = scale8(scales[i / kBlock8]);
+    float f[kStore];
+    load_some<unsigned char, kStore>(codes + i, n - i, f);
 #pragma unroll
-    for (int j = 0; j < kUnpack; j += kStore) {
-      float o[kStore];
-#pragma unroll
-      for (int q = 0; q < kStore; ++q) o[q] = f[j + q];
-      store_f32<T, kStore>(out + i + j, o);
-    }
-    return;
+    for (int j = 0; j < kStore; ++j) f[j] = decode8<kSigned>((unsigned)f[j], e);
+    stream_out<T, kStore>(out + i, n - i, f);
   }
-  for (int j = 0; j < kUnpack && i + j < n; ++j)
-    out[i + j] = (T)decode8<kSigned>(codes[i + j], e);
 }
 
 // ------------------------------------------------------------------ norm
@@ -530,7 +526,8 @@ extern "C" hipError_t pack8_launch(const float* x, unsigned char* codes,
 template <bool kSigned>
 static void unpack8(const unsigned char* codes, const unsigned char* scales,
                     void* out, long n, int type, hipStream_t stream) {
-  const unsigned wg = (unsigned)chunks(n, kUnpack * kThreads);
+  const unsigned wg = (unsigned)chunks(
+      n, type == kElemF32 ? unpack_of<float>() : unpack_of<bf16_t>());
   switch (type) {
     case kElemF32: unpack8_kernel<kSigned, float><<<wg, kThreads, 0, stream>>>(codes, scales, (float*)out, n); break;
     case kElemBF16: unpack8_kernel<kSigned, bf16_t><<<wg, kThreads, 0, stream>>>(codes, scales, (bf16_t*)out, n); break;
