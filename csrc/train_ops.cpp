@@ -399,19 +399,28 @@ bool is_capturing(hipStream_t stream, const char* what) {
 
 // A leaf's gradient goes through the accumulator that a live graph of it
 // holds, on the stream where that was made. In the capture of a backward this
-// would tie another stream to the captured one, which ends the process.
-void check_accumulators(const torch::autograd::variable_list& leaves,
-                        const char* what) {
-  const auto stream = c10::hip::getCurrentHIPStream();
-  if (!is_capturing(stream.stream(), what)) return;
-  for (const Tensor& t : leaves) {
-    if (!t.defined() || !t.is_leaf() || !t.requires_grad()) continue;
-    const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+// would tie that stream to the captured one, which ends the process. Whether
+// it is another one than the forward's shows in the forward.
+bool held_elsewhere(const Tensor& x,
+                    std::initializer_list<const Tensor*> inputs) {
+  const auto stream = c10::hip::getCurrentHIPStream(x.device().index());
+  for (const Tensor* t : inputs) {
+    if (t == nullptr || !t->is_leaf() || !t->requires_grad()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
     const auto at = node ? node->stream() : std::nullopt;
-    TORCH_CHECK(!at || at->id() == stream.unwrap().id(), what,
-                ": a captured backward of a leaf that an earlier graph, made "
-                "on another stream, still holds; free that graph first");
+    if (at && at->id() != stream.unwrap().id()) return true;
   }
+  return false;
+}
+
+void check_capture(bool held, const char* what) {
+  TORCH_CHECK(!held || !is_capturing(current(), what), what,
+              ": a captured backward of a leaf that an earlier graph, made on "
+              "another stream, still holds; free that graph first");
+}
+
+const Tensor* given(const std::optional<Tensor>& t) {
+  return t ? &*t : nullptr;
 }
 
 // The autograd nodes are in C++: small layers are bound by the host's time.
@@ -423,10 +432,11 @@ class LinearActNode
                         const std::optional<Tensor>& bias,
                         const std::optional<Tensor>& residual, int64_t act) {
     auto out = linear_fwd(x, w, bias, act, residual, true);
-    const bool leaf = bias && bias->is_leaf();
-    ctx->save_for_backward({x, w, out[1], leaf ? *bias : Tensor()});
+    ctx->save_for_backward({x, w, out[1]});
+    const bool held = held_elsewhere(x, {&x, &w, given(bias), given(residual)});
     // The edges are the given tensors' alone: which there are goes with act.
-    ctx->saved_data["act"] = act | (bias ? 8 : 0) | (residual ? 16 : 0);
+    ctx->saved_data["act"] =
+        act | (bias ? 8 : 0) | (residual ? 16 : 0) | (held ? 32 : 0);
     return out[0];
   }
 
@@ -436,8 +446,8 @@ class LinearActNode
     TORCH_CHECK(!at::GradMode::is_enabled(),
                 "linear_act: its gradients have no gradient (create_graph)");
     const auto saved = ctx->get_saved_variables();
-    check_accumulators({saved[0], saved[1], saved[3]}, "linear_act");
     const int64_t act = ctx->saved_data["act"].toInt();
+    check_capture(act & 32, "linear_act");
     const bool bias = act & 8, residual = act & 16;
     auto g = linear_bwd(grads[0], saved[2], saved[0], saved[1], act & 7,
                         ctx->needs_input_grad(0), ctx->needs_input_grad(1),
@@ -467,15 +477,14 @@ class LayerNormNode : public torch::autograd::Function<LayerNormNode> {
                         const Tensor& x, const std::optional<Tensor>& w,
                         const std::optional<Tensor>& b, double eps) {
     auto out = layer_norm_fwd(x, w, b, eps, true);
-    const bool leaf = b && b->is_leaf();
-    ctx->save_for_backward(
-        {x, w ? *w : Tensor(), out[1], leaf ? *b : Tensor()});
+    ctx->save_for_backward({x, w ? *w : Tensor(), out[1]});
+    const bool held = held_elsewhere(x, {&x, given(w), given(b)});
     // The edges are the given tensors' alone: which there are goes with the
     // parameters' type.
     ctx->saved_data["given"] =
         (int64_t)(w ? w->scalar_type()
                     : b ? b->scalar_type() : x.scalar_type()) |
-        (w ? 256 : 0) | (b ? 512 : 0);
+        (w ? 256 : 0) | (b ? 512 : 0) | (held ? 1024 : 0);
     return out[0];
   }
 
@@ -485,8 +494,8 @@ class LayerNormNode : public torch::autograd::Function<LayerNormNode> {
     TORCH_CHECK(!at::GradMode::is_enabled(),
                 "layer_norm: its gradients have no gradient (create_graph)");
     const auto saved = ctx->get_saved_variables();
-    check_accumulators({saved[0], saved[1], saved[3]}, "layer_norm");
     const int64_t given = ctx->saved_data["given"].toInt();
+    check_capture(given & 1024, "layer_norm");
     const bool weight = given & 256, bias = given & 512;
     auto g = layer_norm_bwd(
         grads[0], saved[0],

@@ -362,3 +362,15 @@ def test_captured_backward_of_a_held_leaf():
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_bias_may_change_before_the_backward(device):
+    """It has no part in any gradient, so no version of it is kept."""
+    x, w, b, dy = inputs(4, 16, torch.float32, torch.float32, device)
+    b.requires_grad_()
+    y = layer_norm(x, w, b)
+    with torch.no_grad():
+        b.add_(1.0)
+    db, = torch.autograd.grad(y, b, dy)
+    assert torch.allclose(db, dy.sum(0), rtol=1e-5, atol=1e-5)

@@ -407,20 +407,22 @@ def test_far_rows_where_they_do_not_matter():
 def test_captured_backward_of_a_held_leaf():
     """An earlier graph of a leaf, on another stream, is refused."""
     x, w, b, r, dy = inputs(40, 64, 32, torch.bfloat16, "cuda")
-    for i in range(3):
+    for i in range(4):
         leaves = [t.detach().clone().requires_grad_(i == j)
-                  for j, t in enumerate((x, w, b))]
-        held = linear_act(*leaves, "gelu")
+                  for j, t in enumerate((x, w, b, r))]
+        leaves.insert(3, "gelu")
+        i += i == 3
+        held = linear_act(*leaves)
         torch.cuda.synchronize()
         with pytest.raises(RuntimeError, match="free that graph"):
             with torch.cuda.graph(torch.cuda.CUDAGraph()):
-                y = linear_act(*leaves, "gelu")
+                y = linear_act(*leaves)
                 torch.autograd.grad(y, leaves[i], dy)
         want, = torch.autograd.grad(held, leaves[i], dy)
         del held, y
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
-            y = linear_act(*leaves, "gelu")
+            y = linear_act(*leaves)
             got, = torch.autograd.grad(y, leaves[i], dy)
         for _ in range(3):
             graph.replay()
@@ -433,3 +435,15 @@ def test_whole_numbers_are_refused(device):
     x = torch.ones(2, 8, dtype=torch.int32, device=device)
     with pytest.raises(RuntimeError):
         linear_act(x, x)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_bias_may_change_before_the_backward(device):
+    """It has no part in any gradient, so no version of it is kept."""
+    x, w, b, r, dy = inputs(4, 16, 8, torch.float32, device)
+    b.requires_grad_()
+    y = linear_act(x, w, b)
+    with torch.no_grad():
+        b.add_(1.0)
+    db, = torch.autograd.grad(y, b, dy)
+    assert torch.allclose(db, dy.sum(0), rtol=1e-5, atol=1e-5)
