@@ -92,11 +92,12 @@ hipError_t linear_pad_launch(const void* from, void* to, int rows, int width,
 
 hipError_t adamw_launch(const AdamWTensors*, const AdamWScalars*, int type,
                         hipStream_t);
-// Values that one workgroup of square_sum_launch takes.
-int square_sum_chunk();
+// Values that one workgroup of square_sum_launch takes, of so many altogether.
+int square_sum_chunk(long values);
 // `partial` has a double for every chunk of every tensor.
 hipError_t square_sum_launch(const void* const* g, const long* n, int count,
-                             int type, double* partial, hipStream_t);
+                             int chunk, int type, double* partial,
+                             hipStream_t);
 hipError_t norm_launch(const double* partial, int count, float* out,
                        hipStream_t);
 hipError_t pack8_launch(const float* x, unsigned char* codes,

@@ -682,7 +682,9 @@ Tensor grad_norm(const Tensors& g) {
   Tensors dense;
   std::vector<const void*> at[3];
   std::vector<long> n[3];
-  long parts = 0;
+  long parts = 0, values = 0;
+  for (const Tensor& t : g) values += t.numel();
+  const int chunk = square_sum_chunk(values);
   for (const Tensor& t : g) {
     TORCH_CHECK(t.device() == device,
                 "grad_norm: the tensors are on several devices");
@@ -696,7 +698,7 @@ Tensor grad_norm(const Tensors& g) {
       at[type].push_back(dense.back().data_ptr());
     }
     n[type].push_back(t.numel());
-    parts += (t.numel() + square_sum_chunk() - 1) / square_sum_chunk();
+    parts += (t.numel() + chunk - 1) / chunk;
   }
   const auto opts = torch::TensorOptions().device(device);
   Tensor out = torch::empty({}, opts.dtype(torch::kFloat));
@@ -705,9 +707,10 @@ Tensor grad_norm(const Tensors& g) {
   for (int type = 0; type < 3; ++type) {
     if (at[type].empty()) continue;
     launched(square_sum_launch(at[type].data(), n[type].data(),
-                               (int)at[type].size(), type, next, current()),
+                               (int)at[type].size(), chunk, type, next,
+                               current()),
              "grad_norm");
-    for (const long k : n[type]) next += (k + square_sum_chunk() - 1) / square_sum_chunk();
+    for (const long k : n[type]) next += (k + chunk - 1) / chunk;
   }
   launched(norm_launch(parts ? partial.data_ptr<double>() : nullptr,
                        (int)parts, out.data_ptr<float>(), current()),
