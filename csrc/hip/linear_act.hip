@@ -40,10 +40,10 @@
 //     reach 1450 to 1530 on such data, the library's product alone 1250. The
 //     matrix cores are busy 73% of the cycles, LDS has no bank conflicts.
 //     Four waves of 512 registers were slower than eight of 256.
-//   128-wide tiles: LDS. In a step 8 waves read 96 KB of it and the loads
-//     write 32 KB, 1024 cycles at 128 bytes each, for 515 cycles of products:
-//     0.55 us, 975 TFLOP/s. 1000x12544x1024 in 4 splits 32 us and 5 to add
-//     them up; the library 45.
+//   128-wide tiles: LDS. In a step waves with 64x64 of it read 64 KB (those
+//     with 64x32 96 KB) and the loads write 32 KB, 768 cycles (1024) at 128
+//     bytes each, for 515 cycles of products: 0.48 us (0.55), 1120 TFLOP/s.
+//     1000x12544x1024 in 4 splits 31 us and 5 to add them up; the library 45.
 //   64-wide tiles: with many steps the L2s, which give 20 TB/s (dW of
 //     3999x1024x1024 17 us); with few the latency of loads and of the launch:
 //     100x1024x81 7.2 us, of which a launch of one step takes 5.
@@ -725,12 +725,14 @@ void run_tiles(const LinearProduct& a, hipStream_t s) {
       return;
     }
   }
-  // A workgroup that has its CU to itself takes more LDS and looks further
-  // ahead, with the small tile also in two groups of waves that halve its
-  // steps (bf16 1024x1024x3999 22.3 -> 17.6 us, 100x1024x81 8.3 -> 7.2; with
-  // the 128-wide tile no gain); otherwise the others' work covers its waits.
+  // A workgroup that has its CU to itself has two groups of waves, which halve
+  // its steps, in place of one with more or more loads ahead: 64-wide bf16
+  // 1024x1024x3999 22.3 -> 17.6 us and 100x1024x81 8.3 -> 7.2; 128-wide,
+  // whose waves then read a quarter less LDS, 1024x1024x20000 in 4 splits
+  // 53 -> 46, 1000x12544x1024 33 -> 31, few steps as before. Otherwise the
+  // other workgroups' work covers its waits.
   if (a.tile == 128 && grid <= 256)
-    product_kernel<T, kXT, kYT, 128, 128, 2, 4, 1, 4><<<grid, 512, 0, s>>>(a);
+    product_kernel<T, kXT, kYT, 128, 128, 2, 2, 2, 2><<<grid, 512, 0, s>>>(a);
   else if (a.tile == 128)
     product_kernel<T, kXT, kYT, 128, 128, 2, 4, 1, 2><<<grid, 512, 0, s>>>(a);
   else if (grid <= 256)
@@ -772,7 +774,7 @@ hipError_t run_pad(const void* from, void* to, int rows, int width,
 extern "C" void linear_plan(LinearProduct* a, int type) {
   struct Shape { int tile; double step, alone, rest; };
   static const Shape kHalf[] = {{256, 1.55, 1.55, 6.0},
-                                {128, 0.55, 0.55, 2.5},
+                                {128, 0.55, 0.48, 2.5},
                                 {64, 0.25, 0.22, 1.0}};
   static const Shape kFull[] = {{128, 1.8, 1.8, 2.5}, {64, 0.5, 0.5, 1.0}};
   const Shape* shapes = type == kElemF32 ? kFull : kHalf;
