@@ -521,39 +521,41 @@ __global__ __launch_bounds__(kWM * kWN * kGroups * 64, 2) void product_kernel(
   // consecutive columns: full-width accesses, and one copy of the epilogue's
   // code.
   constexpr int kCols = kBN / kWN, kQuads = kCols / 4;
-  constexpr int kFit = kLds / kWaves / (16 * kCols * 4);   // parts down
-  constexpr int kParts = kFit >= kMI ? kMI : kFit >= kMI / 2 ? kMI / 2
-                                                             : kMI / 4;
+  constexpr int kOwn = kMI / kGroups;        // parts down that a group finishes
+  constexpr int kSums = kGroups > 1 ? kWaves * kOwn * kNI * 64 * 16 : 0;
+  constexpr int kFit = (kLds - kSums) / kWaves / (16 * kCols * 4);
+  constexpr int kParts = kFit >= kOwn ? kOwn : kFit >= kOwn / 2 ? kOwn / 2
+                                                                : kOwn / 4;
   static_assert(kParts > 0 && kParts <= kFit, "a wave's share of LDS");
   constexpr int kLanes = kCols / kOut;                     // of one row
   arrived<0>();
   if constexpr (kGroups > 1) {
-    // The first group gets the others' sums, a lane the ones of its own place.
-    constexpr int kSums = kMI * kNI * 64 * 16;             // bytes of a wave
-    static_assert(kWaves * kSums <= kLds, "a group's sums in its buffers");
-    if (group > 0) {
+    // Each group finishes a half of the parts: it leaves its sums of the other
+    // half to the other group, a lane the ones of its own place.
+    static_assert(kGroups == 2 && kMI % 2 == 0, "halves");
+    const int at = wave * (kOwn * kNI * 64 * 16) + lane * 16;
 #pragma unroll
-      for (int i = 0; i < kMI * kNI; ++i)
-        *(f32x4*)(lds + wave * kSums + (i * 64 + lane) * 16) =
-            acc[i / kNI][i % kNI];
-    }
+    for (int i = 0; i < kOwn * kNI; ++i)
+      *(f32x4*)(lds + at + i * 1024) = group ? acc[i / kNI][i % kNI]
+                                             : acc[kOwn + i / kNI][i % kNI];
     arrived<0>();
-    if (group > 0) return;
+    const char* theirs = lds_all + (1 - group) * kLds;
 #pragma unroll
-    for (int g = 1; g < kGroups; ++g)
-#pragma unroll
-      for (int i = 0; i < kMI * kNI; ++i)
-        acc[i / kNI][i % kNI] += *(const f32x4*)(
-            lds + g * kLds + wave * kSums + (i * 64 + lane) * 16);
+    for (int i = 0; i < kOwn * kNI; ++i) {
+      f32x4& sum = acc[i / kNI][i % kNI];
+      if (group) sum = acc[kOwn + i / kNI][i % kNI];
+      sum += *(const f32x4*)(theirs + at + i * 1024);
+    }
   }
-  char* mine = lds + wave * (kParts * 16 * kCols * 4);
+  char* mine = lds + kSums + wave * (kParts * 16 * kCols * 4);
+  const int own_m = m0 + xr + group * kOwn * 16;
   const int c = lane % kLanes, n = n0 + yr + c * kOut;
   constexpr int kTurns = kParts * 16 * kLanes / 64;        // of 64 lanes
   constexpr int kFetch = kTurns < 4 ? kTurns : 4;
   const int r_of_lane = lane / kLanes;
   const auto rows = [&](auto fetch, auto store) {
 #pragma unroll
-    for (int round = 0; round < kMI / kParts; ++round) {
+    for (int round = 0; round < kOwn / kParts; ++round) {
 #pragma unroll
       for (int i = 0; i < kParts; ++i) {
         const int r = i * 16 + (lane & 15);
@@ -569,7 +571,7 @@ __global__ __launch_bounds__(kWM * kWN * kGroups * 64, 2) void product_kernel(
       for (int t0 = 0; t0 < kTurns; t0 += kFetch) {
         // What four rows need from memory is in flight before its first use.
         const int r0 = r_of_lane + t0 * (64 / kLanes);
-        const int first_m = m0 + xr + round * kParts * 16 + r0;
+        const int first_m = own_m + round * kParts * 16 + r0;
         decltype(fetch(0)) fetched[kFetch];
 #pragma unroll
         for (int t = 0; t < kFetch; ++t) {
