@@ -5,12 +5,16 @@
 //   v = b2 v + (1 - b2) (c g)^2
 //   p = p (1 - lr wd) - lr / bc1 * m / (sqrt(v) / sqrt(bc2) + eps)
 //
-// All of it in fp32; the scalars are formed in double on the host. Every
-// product and sum of the states is rounded by itself (no contraction), so
-// that a plain elementwise program gets the same states to the bit, and with
-// them the same 8-bit codes. The update's root and quotient are the
-// instructions' (1 unit in the last place each): 3 units of an update that is
-// itself a small part of p, for a fifth of the 8-bit kernel's instructions.
+// All of it in fp32; the scalars are formed in double on the host. With betas
+// from 0.5 on the states are formed as m + (1 - b1) (c g - m), a difference
+// and a fused product and sum: one rounding of the result, and that of a
+// beta such as 0.999 to fp32, a fifth of a unit in the last place, leaves no
+// trace. (With smaller betas the difference would cancel: there it is the
+// products' sum, each rounded by itself.) The same in plain elementwise
+// operations gives the states to the bit, and with them the same 8-bit codes.
+// The update's root and quotient are the instructions' (1 unit in the last
+// place each): 3 units of an update that is itself a small part of p, for a
+// fifth of the 8-bit kernel's instructions.
 //
 // 8-bit states: 256 consecutive values of a tensor share a power of two
 // 2^(E-127), the exponent of the largest magnitude among them, kept as one
@@ -35,7 +39,7 @@
 // detector in fp32: the norm 55 us and the step 285 us (1.79 GB, 6.2 TB/s; a
 // part of the gradients comes from the memory-side cache), 412 together
 // before p, m and v went past the caches. With 8-bit states the step takes
-// 200 us (1.02 GB, 5.1 TB/s).
+// 195 us (1.02 GB, 5.3 TB/s).
 #include <hip/hip_runtime.h>
 
 #include "train_ops.h"
@@ -115,12 +119,24 @@ __device__ inline float root(float v) {
   return tiny ? s * 0x1p-32f : s;
 }
 
+// The state after `in`; where it may be one (k32), an overflown state stays.
+template <bool kLerp, bool k32>
+__device__ inline float moved(float state, float in, float beta,
+                              float one_minus) {
+#pragma clang fp contract(off)
+  if constexpr (!kLerp) return state * beta + in * one_minus;
+  const float d = in - state;
+  const float x = __builtin_fmaf(d, one_minus, state);
+  return k32 && __builtin_isinf(state) ? state + in : x;
+}
+
+template <bool kLerp, bool k32>
 __device__ inline void update(const Hyper& h, float c, float g, float& p,
                               float& m, float& v) {
 #pragma clang fp contract(off)
   g = g * c;
-  m = m * h.beta1 + g * h.one_minus_beta1;
-  v = v * h.beta2 + (g * g) * h.one_minus_beta2;
+  m = moved<kLerp, k32>(m, g, h.beta1, h.one_minus_beta1);
+  v = moved<kLerp, k32>(v, g * g, h.beta2, h.one_minus_beta2);
   const float step =
       m * __builtin_amdgcn_rcpf(root(v) * h.inv_bc2 + h.eps);
   p = p * h.decay - step * h.rate;
@@ -134,7 +150,7 @@ __device__ inline int turned(const Table&) {
   return gridDim.x - 1 - blockIdx.x;
 }
 
-template <typename T>
+template <typename T, bool kLerp>
 __global__ __launch_bounds__(kThreads) void adamw32_kernel(
     Table32<kTensors32> t, Hyper h) {
   const int wg = turned(t), k = find_tensor(t, wg);
@@ -155,7 +171,8 @@ __global__ __launch_bounds__(kThreads) void adamw32_kernel(
     stream_in(m + i, left, mf);
     stream_in(v + i, left, vf);
 #pragma unroll
-    for (int j = 0; j < kValues; ++j) update(h, c, gf[j], pf[j], mf[j], vf[j]);
+    for (int j = 0; j < kValues; ++j)
+      update<kLerp, true>(h, c, gf[j], pf[j], mf[j], vf[j]);
     stream_out(p + i, left, pf);
     stream_out(m + i, left, mf);
     stream_out(v + i, left, vf);
@@ -270,11 +287,30 @@ __device__ inline void decode_block8(unsigned w, int e, float (&x)[kValues]) {
     x[j] = decode8<kSigned>((w >> (8 * j)) & 255u, scale);
 }
 
-// Two passes at a time, so that the loads of both are in flight.
-template <typename T>
+// 0 for a number in the middle between two codes.
+__device__ inline unsigned middle(float x) {
+  return (__float_as_uint(x) << 12) + 0x80000000u;
+}
+
+// x = moved(state, in) in such a middle goes by its last bit to where it was
+// before its rounding, so that its code is that of the unrounded state. (The
+// difference to the old state loses a last bit at most, far below what was
+// rounded off.)
+__device__ inline void leave_middle(float& x, float state, float in,
+                                    float one_minus) {
+#pragma clang fp contract(off)
+  if (middle(x) != 0) return;
+  const float lost = __builtin_fmaf(in - state, one_minus, state - x);
+  const int up = lost == 0.0f ? 0 : (lost > 0.0f) == (x > 0.0f) ? 1 : -1;
+  x = __int_as_float(__float_as_int(x) + up);
+}
+
+// One pass at a time: 60 registers, so that eight waves of a SIMD cover each
+// other's loads. Two at a time took 92 and 143 us in place of 125 for 48
+// million values.
+template <typename T, bool kLerp>
 __global__ __launch_bounds__(kThreads) void adamw8_kernel(
     Table8<kTensors8> t, Hyper h) {
-  constexpr int kDeep = 2;
   const int wg = turned(t), k = find_tensor(t, wg);
   const long at = (long)(wg - t.first[k]) * t.passes * kPass +
                   threadIdx.x * kValues;
@@ -286,39 +322,41 @@ __global__ __launch_bounds__(kThreads) void adamw8_kernel(
   unsigned char* ms = t.ms[k];
   unsigned char* vs = t.vs[k];
   const float c = clip_factor(h);
-  for (int pass = 0; pass < t.passes; pass += kDeep) {
-    float pf[kDeep][kValues], gf[kDeep][kValues];
-    unsigned mc[kDeep], vc[kDeep], me[kDeep], ve[kDeep];
+  for (int pass = 0; pass < t.passes; ++pass) {
+    const long i = at + (long)pass * kPass, left = n - i;
+    const long b = i / kBlock8;
+    // A wave is past its end as a whole: it has one block.
+    if (b * kBlock8 >= n) return;
+    float pf[kValues], gf[kValues], mf[kValues], vf[kValues];
+    stream_in(p + i, left, pf);
+    stream_in(g + i, left, gf);
+    const unsigned mc = load_codes(m + i, left), vc = load_codes(v + i, left);
+    const unsigned me = ms[b], ve = vs[b];
+    decode_block8<true>(mc, me, mf);
+    decode_block8<false>(vc, ve, vf);
+    unsigned between = 1;
 #pragma unroll
-    for (int d = 0; d < kDeep; ++d) {
-      const long i = at + (long)(pass + d) * kPass, left = n - i;
-      const long b = i / kBlock8;
-      if (pass + d >= t.passes || b * kBlock8 >= n) continue;
-      stream_in(p + i, left, pf[d]);
-      stream_in(g + i, left, gf[d]);
-      mc[d] = load_codes(m + i, left);
-      vc[d] = load_codes(v + i, left);
-      me[d] = ms[b];
-      ve[d] = vs[b];
+    for (int j = 0; j < kValues; ++j) {
+      update<kLerp, false>(h, c, gf[j], pf[j], mf[j], vf[j]);
+      between = min(between, min(middle(mf[j]), middle(vf[j])));
     }
-#pragma unroll
-    for (int d = 0; d < kDeep; ++d) {
-      const long i = at + (long)(pass + d) * kPass, left = n - i;
-      const long b = i / kBlock8;
-      // A wave is past its end as a whole: it has one block.
-      if (pass + d >= t.passes || b * kBlock8 >= n) return;
-      float mf[kValues], vf[kValues];
-      decode_block8<true>(mc[d], me[d], mf);
-      decode_block8<false>(vc[d], ve[d], vf);
+    if (kLerp && between == 0) {             // one wave in a few thousand
+      float m0[kValues], v0[kValues];
+      decode_block8<true>(mc, me, m0);
+      decode_block8<false>(vc, ve, v0);
 #pragma unroll
       for (int j = 0; j < kValues; ++j) {
-        update(h, c, gf[d][j], pf[d][j], mf[j], vf[j]);
-        if (j >= left) mf[j] = vf[j] = 0.0f;   // no part in the maximum
+        const float in = gf[j] * c;
+        leave_middle(mf[j], m0[j], in, h.one_minus_beta1);
+        leave_middle(vf[j], v0[j], in * in, h.one_minus_beta2);
       }
-      stream_out(p + i, left, pf[d]);
-      store_block8<true>(m + i, ms + b, left, mf);
-      store_block8<false>(v + i, vs + b, left, vf);
     }
+#pragma unroll
+    for (int j = 0; j < kValues; ++j)
+      if (j >= left) mf[j] = vf[j] = 0.0f;   // no part in the maximum
+    stream_out(p + i, left, pf);
+    store_block8<true>(m + i, ms + b, left, mf);
+    store_block8<false>(v + i, vs + b, left, vf);
   }
 }
 
@@ -438,45 +476,55 @@ static int fill(Table& t, const AdamWTensors& a, int from, int to,
   return wg;
 }
 
-extern "C" hipError_t adamw_launch(const AdamWTensors* a,
-                                   const AdamWScalars* s, int type,
-                                   hipStream_t stream) {
-  const Hyper h{s->beta1, s->one_minus_beta1, s->beta2, s->one_minus_beta2,
-                s->eps, s->decay, s->rate, s->inv_bc2, s->max_norm, s->norm};
-  const int most = a->ms == nullptr ? kTensors32 : kTensors8;
-  for (int to = a->count; to > 0;) {
+template <typename T, bool kLerp>
+static hipError_t run_adamw(const AdamWTensors& a, const Hyper& h,
+                            hipStream_t stream) {
+  const int most = a.ms == nullptr ? kTensors32 : kTensors8;
+  for (int to = a.count; to > 0;) {
     const int from = to > most ? to - most : 0;
     // Four passes a workgroup amortise its search for the tensor; few values
     // are spread over more workgroups instead.
     long values = 0;
-    for (int i = from; i < to; ++i) values += a->n[i];
+    for (int i = from; i < to; ++i) values += a.n[i];
     const int passes = values >= 1024L * kPasses * kPass ? kPasses : 1;
-    if (a->ms == nullptr) {
+    if (a.ms == nullptr) {
       Table32<kTensors32> t;
-      const int wg = fill(t, *a, from, to, passes);
-      switch (type) {
-        case kElemF32: adamw32_kernel<float><<<wg, kThreads, 0, stream>>>(t, h); break;
-        case kElemBF16: adamw32_kernel<bf16_t><<<wg, kThreads, 0, stream>>>(t, h); break;
-        default: adamw32_kernel<fp16_t><<<wg, kThreads, 0, stream>>>(t, h);
-      }
+      const int wg = fill(t, a, from, to, passes);
+      adamw32_kernel<T, kLerp><<<wg, kThreads, 0, stream>>>(t, h);
     } else {
       Table8<kTensors8> t;
-      const int wg = fill(t, *a, from, to, passes);
+      const int wg = fill(t, a, from, to, passes);
       for (int i = from; i < to; ++i) {
-        t.ms[i - from] = a->ms[i];
-        t.vs[i - from] = a->vs[i];
+        t.ms[i - from] = a.ms[i];
+        t.vs[i - from] = a.vs[i];
       }
-      switch (type) {
-        case kElemF32: adamw8_kernel<float><<<wg, kThreads, 0, stream>>>(t, h); break;
-        case kElemBF16: adamw8_kernel<bf16_t><<<wg, kThreads, 0, stream>>>(t, h); break;
-        default: adamw8_kernel<fp16_t><<<wg, kThreads, 0, stream>>>(t, h);
-      }
+      adamw8_kernel<T, kLerp><<<wg, kThreads, 0, stream>>>(t, h);
     }
     to = from;
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
   return hipSuccess;
+}
+
+template <bool kLerp>
+static hipError_t run_adamw(const AdamWTensors& a, const Hyper& h, int type,
+                            hipStream_t stream) {
+  switch (type) {
+    case kElemF32: return run_adamw<float, kLerp>(a, h, stream);
+    case kElemBF16: return run_adamw<bf16_t, kLerp>(a, h, stream);
+    default: return run_adamw<fp16_t, kLerp>(a, h, stream);
+  }
+}
+
+extern "C" hipError_t adamw_launch(const AdamWTensors* a,
+                                   const AdamWScalars* s, int type,
+                                   hipStream_t stream) {
+  const Hyper h{s->beta1, s->one_minus_beta1, s->beta2, s->one_minus_beta2,
+                s->eps, s->decay, s->rate, s->inv_bc2, s->max_norm, s->norm};
+  return s->beta1 >= 0.5f && s->beta2 >= 0.5f
+             ? run_adamw<true>(*a, h, type, stream)
+             : run_adamw<false>(*a, h, type, stream);
 }
 
 // Values of one partial sum. Few values altogether are spread over more

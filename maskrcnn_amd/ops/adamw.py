@@ -9,8 +9,12 @@ are read, never rewritten, so the clipped norm costs no pass of its own over
 them. CPU: the same operations in plain torch (the numerics oracle; the two
 give the same bits).
 
+With betas from 0.5 on a state is formed as m + (1 - beta1) (c g - m) with one
+rounding of the result.
+
 8-bit states: 256 values in memory order share a power of two, and a value
-is its ratio to it with 3 bits of mantissa (pack_state8, unpack_state8).
+is its ratio to it with 3 bits of mantissa (pack_state8, unpack_state8); a
+step's new codes are those of the unrounded states.
 """
 
 from __future__ import annotations
@@ -126,13 +130,31 @@ def grad_norm(tensors) -> torch.Tensor:
                         for t in tensors]).sum().sqrt().float()
 
 
-def _step_torch(p, g, m, v, clip, beta1, beta2, eps, decay, rate, inv_bc2):
+def _moved(state, value, beta, codes, lerp):
+    """The state after `value`, rounded once to fp32 (csrc/hip/adamw.hip)."""
+    if not lerp:
+        return state * beta + value * (1.0 - beta)
+    weight = float(torch.tensor(1.0 - beta, dtype=torch.float32))
+    wide = state.double() + (value - state).double() * weight
+    x = wide.float()
+    if not codes:
+        return torch.where(state.isinf(), state + value, x)
+    bits = x.view(torch.int32)
+    lost = (value - state).double() * weight + (state - x).double()
+    up = (torch.sign(lost) * torch.sign(x)).to(torch.int32)
+    middle = ((bits & 0xFFFFF) == 0x80000) & ~x.isnan()
+    return torch.where(middle, bits + up, bits).view(torch.float32)
+
+
+def _step_torch(p, g, m, v, clip, beta1, beta2, eps, decay, rate, inv_bc2,
+                codes):
     """One tensor's step; m and v are fp32 and changed in place."""
     gf = g.float()
     if clip is not None:
         gf = gf * clip
-    m.copy_(m * beta1 + gf * (1.0 - beta1))
-    v.copy_(v * beta2 + (gf * gf) * (1.0 - beta2))
+    lerp = beta1 >= 0.5 and beta2 >= 0.5
+    m.copy_(_moved(m, gf, beta1, codes, lerp))
+    v.copy_(_moved(v, gf * gf, beta2, codes, lerp))
     p.copy_(p.float() * decay - m / (torch.sqrt(v) * inv_bc2 + eps) * rate)
 
 
@@ -181,7 +203,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *,
                 (grad_norm + 1e-6)).clamp(max=1.0)
     scalars = (clip, beta1, beta2, eps, 1.0 - lr * weight_decay,
                lr / (1.0 - beta1 ** step),
-               1.0 / math.sqrt(1.0 - beta2 ** step))
+               1.0 / math.sqrt(1.0 - beta2 ** step), eight)
     for i, (p, g, m, v) in enumerate(zip(params, grads, exp_avgs,
                                          exp_avg_sqs)):
         want = torch.uint8 if eight else torch.float32

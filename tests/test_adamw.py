@@ -484,3 +484,62 @@ def test_shared_gradient(device):
     for i in range(2):
         adamw_step([one[0][i]], [g[0]], [one[1][i]], [one[2][i]], **HYPER)
         assert torch.equal(p[i], one[0][i])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("betas", [(0.9, 0.999), (0.3, 0.2), (0.0, 0.0),
+                                   (0.5, 0.5), (0.2, 0.99)])
+def test_betas(device, betas):
+    """Small ones as well, and states that tower over what comes."""
+    p, g, m, v = tensors([5000], torch.float32, device)
+    m[0][:2000] *= 1e6
+    v[0][:2000] *= 1e9
+    for _ in range(2):
+        old = [t[0].clone() for t in (m, v)]
+        adamw_step(p, g, m, v, **dict(HYPER, betas=betas))
+        assert p[0].isfinite().all()
+        # As in test_step_32, with these betas: two roundings of terms, a
+        # sum's and the constants'.
+        for got, was, new, beta in ((m[0], old[0], g[0].double(), betas[0]),
+                                    (v[0], old[1], g[0].double().square(),
+                                     betas[1])):
+            a, b = beta * was.double(), (1 - beta) * new
+            off = (got.double() - (a + b)).abs()
+            assert (off <= 5 * U * (a.abs() + b.abs()) + 1e-40).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("betas", [(0.9, 0.999), (0.3, 0.2)])
+def test_overflown_state(device, betas):
+    """It stays one and leaves its parameter to the decay alone."""
+    p, g, m, v = tensors([300], torch.float32, device)
+    v[0][7] = float("inf")
+    for _ in range(2):
+        was = float(p[0][7])
+        adamw_step(p, g, m, v, **dict(HYPER, betas=betas))
+        assert v[0][7].isinf() and v[0].isinf().sum() == 1
+        assert abs(float(p[0][7]) - was * (1 - 1e-4)) <= 2 * U * abs(was)
+        assert p[0].isfinite().all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_codes_are_the_unrounded_states(device):
+    """Sums that fp32 rounds to the middle between two codes: (1 + g) / 2 with
+    g = 1.125 + k 2^-23 lies k/2 units above or below it."""
+    n, u = 512, 2.0 ** -23
+    m = torch.ones(n, device=device)
+    g = torch.full((n,), 1.125, device=device)
+    g[0::4] += u
+    g[1::4] -= u
+    g[2::4] += 3 * u
+    mc, ms = pack_state8(m, True)
+    vc, vs = pack_state8(m, False)
+    adamw_step([m.clone()], [g], [mc], [vc], exp_avg_scales=[ms],
+               exp_avg_sq_scales=[vs], step=1, lr=0.1, betas=(0.5, 0.5))
+    got = unpack_state8(mc, ms, True)
+    # The middle itself goes to the even code.
+    for at, want in enumerate((1.125, 1.0, 1.125, 1.0)):
+        assert (got[at::4] == want).all(), at
+    square = g * g
+    want = (1.0 + square.double()) / 2
+    assert torch.equal(unpack_state8(vc, vs, False), grid(want, False))
