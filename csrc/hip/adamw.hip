@@ -25,10 +25,23 @@
 //                  a value above zero never gets the code of zero, because a
 //                  zero in the denominator would blow the update up, while a
 //                  value held too large only makes it smaller
-// Rounding is to nearest even; a ratio above 1.875 (up to 2) takes the top
-// code, no further off than half a step. With a power of two as the scale
-// the ratio is exact, and so is the held value in bf16. E = 255 (an infinity
-// or NaN among the values) stands for NaN in the whole block.
+// With a power of two as the scale the ratio is exact, and so is the held value
+// in bf16. E = 255 (an infinity or NaN among the values) stands for NaN in the
+// whole block.
+//   Rounding to nearest (even) has the least error in one step; a ratio above
+// 1.875 (up to 2) takes the top code, no further off than half a step. Over
+// many steps it loses what moves a state by less than half a step of its code:
+// codes lie 6 to 12% apart and a beta of 0.999 moves v down by 0.1% at most, so
+// that v never falls and rises only on squares 34 to 63 times as large. With a
+// seed the state is therefore rounded up or down at random, up with the
+// probability of what lies above the lower code, so that its mean is the
+// unrounded state's. A step adds at most |d| D to its variance (d the step's
+// move, D the distance of two codes), which is a spread of about a quarter of
+// v in the long run. What is rounded up past 1.875 takes 2 and with it the
+// block's next exponent; else a block's largest value could not grow.
+//   The random bits are an integer hash of the seed, the step, the tensor's
+// number and the value's place: nothing is kept between calls, and the same
+// call gives the same codes.
 //
 // Memory bound: 28 bytes a value with fp32 states and parameters, 16 with
 // 8-bit states, some 60 and 120 vector instructions. One thread holds 4
@@ -39,7 +52,8 @@
 // detector in fp32: the norm 55 us and the step 285 us (1.79 GB, 6.2 TB/s; a
 // part of the gradients comes from the memory-side cache), 412 together
 // before p, m and v went past the caches. With 8-bit states the step takes
-// 195 us (1.02 GB, 5.3 TB/s).
+// 195 us (1.02 GB, 5.3 TB/s), rounded to nearest; at random 3 to 5% more (196
+// and 188 us where to nearest took 188 and 181 in turn with it).
 #include <hip/hip_runtime.h>
 
 #include "train_ops.h"
@@ -58,7 +72,7 @@ static_assert(kPass % kBlock8 == 0 && kBlock8 == 64 * kValues,
 
 // Pointers travel as kernel arguments (below 4 KB), so a launch needs no
 // copy to the device and can be captured.
-constexpr int kTensors32 = 88, kTensors8 = 62, kTensorsNorm = 180;
+constexpr int kTensors32 = 88, kTensors8 = 60, kTensorsNorm = 180;
 
 template <int N>
 struct Table32 {
@@ -75,6 +89,7 @@ template <int N>
 struct Table8 : Table32<N> {
   unsigned char* ms[N];
   unsigned char* vs[N];
+  unsigned key[N];  // of the random bits
 };
 
 struct TableNorm {
@@ -197,6 +212,15 @@ __device__ inline float scale8(int e) {
   return e == 255 ? __int_as_float(0x7fc00000) : pow2_biased(e);
 }
 
+// A hash of 32 bits: products with odd numbers and shifts, each of them a
+// permutation, so that every input bit changes every output bit in half of
+// all cases (to the 1% that 16384 inputs can tell). ops/adamw.py has it too.
+__host__ __device__ inline unsigned mix(unsigned x) {
+  x = (x ^ x >> 16) * 0xac9b39d5u;
+  x = (x ^ x >> 15) * 0x8fe44835u;
+  return x ^ x >> 16;
+}
+
 // A code in the place of an fp32 number's exponent and first 3 bits is its
 // value times a power of two, the codes below the smallest normal one being
 // subnormal there too.
@@ -209,9 +233,21 @@ __device__ inline float decode8(unsigned code, float scale) {
   return kSigned && code > 127 ? -r : r;
 }
 
-// `inv` = 2^(127 - E).
-template <bool kSigned>
-__device__ inline unsigned encode8(float x, float inv) {
+// A number whose first 3 bits of mantissa are all there is, from x's magnitude
+// and 20 random bits: up with the probability of what is cut off. Infinities
+// and NaN stay in the largest exponent, and nothing else gets there.
+__device__ inline float cut(float x, unsigned bits) {
+  const unsigned b = __float_as_uint(x), mag = b & 0x7fffffffu;
+  const unsigned up = mag + bits;
+  return __uint_as_float(((up < 0x7f800000u ? up : mag) & 0x7ff00000u) |
+                         (b & 0x80000000u));
+}
+
+// `inv` = 2^(127 - E). kRandom: x is cut()'s, and `hash` gives the bits where
+// a small code has fewer than 3 of mantissa; `above`: the state is above zero.
+template <bool kSigned, bool kRandom>
+__device__ inline unsigned encode8(float x, float inv, bool above,
+                                   unsigned hash) {
   constexpr int low = Code8<kSigned>::low;
   const float r = fabsf(x) * inv;
   const int b = __float_as_int(r);
@@ -219,8 +255,16 @@ __device__ inline unsigned encode8(float x, float inv) {
   code = code > Code8<kSigned>::top ? Code8<kSigned>::top : code;
   const bool small = r < pow2_biased(127 - low);
   if (__any(small)) {                  // rare but for zeros
-    int c = (int)rintf(r * pow2_biased(127 + low + 3));
-    if (!kSigned && x > 0.0f && c == 0) c = 1;   // also where r is 0
+    const float q = r * pow2_biased(127 + low + 3);
+    int c;
+    if constexpr (kRandom) {
+      const float whole = floorf(q);
+      const unsigned u = mix(hash + (kSigned ? 1 : 2)) >> 8;
+      c = (int)whole + ((float)u * 0x1p-24f < q - whole);
+    } else {
+      c = (int)rintf(q);
+    }
+    if (!kSigned && above && c == 0) c = 1;   // also where r is 0
     code = small ? c : code;
   }
   if (kSigned) code |= (int)(__float_as_uint(x) >> 24) & 128;
@@ -245,15 +289,24 @@ __device__ inline int block_exponent(const float (&x)[kValues]) {
   return e < kMinExp ? kMinExp : e;
 }
 
-template <bool kSigned>
+// kRandom: `hash` has 20 bits for each moment, the first's the lower ones. (The
+// second's last 8 are the first's first 8, far too small a part to tell.)
+template <bool kSigned, bool kRandom>
 __device__ inline void store_block8(unsigned char* codes, unsigned char* scale,
-                                    long left, const float (&x)[kValues]) {
-  const int e = block_exponent(x);
+                                    long left, const float (&x)[kValues],
+                                    const unsigned (&hash)[kValues]) {
+  float y[kValues];
+#pragma unroll
+  for (int j = 0; j < kValues; ++j)
+    y[j] = !kRandom ? x[j]
+           : cut(x[j], kSigned ? hash[j] & 0xfffffu : hash[j] >> 12);
+  const int e = block_exponent(y);
   unsigned c[kValues] = {};
   if (e < 255) {                       // of the whole wave
     const float inv = __int_as_float(e < 254 ? (254 - e) << 23 : 0x400000);
 #pragma unroll
-    for (int j = 0; j < kValues; ++j) c[j] = encode8<kSigned>(x[j], inv);
+    for (int j = 0; j < kValues; ++j)
+      c[j] = encode8<kSigned, kRandom>(y[j], inv, x[j] > 0.0f, hash[j]);
   }
   if (left >= kValues) {
     const unsigned w = c[0] | (c[1] << 8) | (c[2] << 16) | (c[3] << 24);
@@ -308,7 +361,7 @@ __device__ inline void leave_middle(float& x, float state, float in,
 // One pass at a time: 60 registers, so that eight waves of a SIMD cover each
 // other's loads. Two at a time took 92 and 143 us in place of 125 for 48
 // million values.
-template <typename T, bool kLerp>
+template <typename T, bool kLerp, bool kRandom>
 __global__ __launch_bounds__(kThreads) void adamw8_kernel(
     Table8<kTensors8> t, Hyper h) {
   const int wg = turned(t), k = find_tensor(t, wg);
@@ -340,7 +393,7 @@ __global__ __launch_bounds__(kThreads) void adamw8_kernel(
       update<kLerp, false>(h, c, gf[j], pf[j], mf[j], vf[j]);
       between = min(between, min(middle(mf[j]), middle(vf[j])));
     }
-    if (kLerp && between == 0) {             // one wave in a few thousand
+    if (!kRandom && kLerp && between == 0) {   // one wave in a few thousand
       float m0[kValues], v0[kValues];
       decode_block8<true>(mc, me, m0);
       decode_block8<false>(vc, ve, v0);
@@ -354,9 +407,15 @@ __global__ __launch_bounds__(kThreads) void adamw8_kernel(
 #pragma unroll
     for (int j = 0; j < kValues; ++j)
       if (j >= left) mf[j] = vf[j] = 0.0f;   // no part in the maximum
+    unsigned hash[kValues] = {};
+    if constexpr (kRandom) {
+      const unsigned key = t.key[k] ^ (unsigned)(i >> 32) * 0x8fe44835u;
+#pragma unroll
+      for (int j = 0; j < kValues; ++j) hash[j] = mix((unsigned)i + j ^ key);
+    }
     stream_out(p + i, left, pf);
-    store_block8<true>(m + i, ms + b, left, mf);
-    store_block8<false>(v + i, vs + b, left, vf);
+    store_block8<true, kRandom>(m + i, ms + b, left, mf, hash);
+    store_block8<false, kRandom>(v + i, vs + b, left, vf, hash);
   }
 }
 
@@ -370,7 +429,7 @@ __global__ __launch_bounds__(kThreads) void pack8_kernel(
   if (b * kBlock8 >= n) return;
   float f[kValues];
   load_some(x + i, left, f);
-  store_block8<kSigned>(codes + i, scales + b, left, f);
+  store_block8<kSigned, false>(codes + i, scales + b, left, f, {});
 }
 
 // 16 bytes of the result a thread, four times: a wave's accesses lie together,
@@ -497,8 +556,12 @@ static hipError_t run_adamw(const AdamWTensors& a, const Hyper& h,
       for (int i = from; i < to; ++i) {
         t.ms[i - from] = a.ms[i];
         t.vs[i - from] = a.vs[i];
+        t.key[i - from] = a.key ? a.key[i] : 0;
       }
-      adamw8_kernel<T, kLerp><<<wg, kThreads, 0, stream>>>(t, h);
+      if (a.key)
+        adamw8_kernel<T, kLerp, true><<<wg, kThreads, 0, stream>>>(t, h);
+      else
+        adamw8_kernel<T, kLerp, false><<<wg, kThreads, 0, stream>>>(t, h);
     }
     to = from;
     const hipError_t e = hipGetLastError();
@@ -515,6 +578,11 @@ static hipError_t run_adamw(const AdamWTensors& a, const Hyper& h, int type,
     case kElemBF16: return run_adamw<bf16_t, kLerp>(a, h, stream);
     default: return run_adamw<fp16_t, kLerp>(a, h, stream);
   }
+}
+
+// A number's 32 bits after 32 others; the numbers in turn give a tensor's key.
+extern "C" unsigned adamw_key(unsigned key, unsigned number) {
+  return mix(key + number + 0xac9b39d5u);
 }
 
 extern "C" hipError_t adamw_launch(const AdamWTensors* a,

@@ -5,7 +5,7 @@
 #include <hip/hip_runtime.h>
 
 // Host views of the tensors of one type; `ms` and `vs` are null with fp32
-// states.
+// states, `key` where 8-bit ones are rounded to nearest.
 struct AdamWTensors {
   int count;
   void* const* p;
@@ -14,6 +14,7 @@ struct AdamWTensors {
   void* const* v;
   unsigned char* const* ms;
   unsigned char* const* vs;
+  const unsigned* key;
   const long* n;
 };
 
@@ -90,6 +91,7 @@ hipError_t linear_dz_launch(const LinearDz*, int type, hipStream_t);
 hipError_t linear_pad_launch(const void* from, void* to, int rows, int width,
                              long stride, int ld, int type, hipStream_t);
 
+unsigned adamw_key(unsigned key, unsigned number);
 hipError_t adamw_launch(const AdamWTensors*, const AdamWScalars*, int type,
                         hipStream_t);
 // Values that one workgroup of square_sum_launch takes, of so many altogether.

@@ -552,7 +552,8 @@ void adamw_step(const Tensors& p, const Tensors& g, const Tensors& m,
                 const std::optional<Tensors>& vs,
                 const std::optional<Tensor>& norm, double max_norm,
                 double step, double lr, double beta1, double beta2,
-                double eps, double weight_decay) {
+                double eps, double weight_decay,
+                std::optional<uint64_t> seed) {
   const size_t count = p.size();
   TORCH_CHECK(g.size() == count && m.size() == count && v.size() == count &&
                   ms.has_value() == vs.has_value() &&
@@ -639,11 +640,23 @@ void adamw_step(const Tensors& p, const Tensors& g, const Tensors& m,
   s.max_norm = (float)max_norm;
   s.norm = norm ? norm->data_ptr<float>() : nullptr;
 
+  // The random bits' keys go by the tensor's number in the call.
+  std::vector<unsigned> keys;
+  if (ms && seed) {
+    const auto number = (uint64_t)(int64_t)step;
+    unsigned key = 0;
+    for (const uint64_t word : {*seed, number})
+      key = adamw_key(adamw_key(key, (unsigned)word), (unsigned)(word >> 32));
+    for (size_t i = 0; i < count; ++i)
+      keys.push_back(adamw_key(key, (unsigned)i));
+  }
+
   // One launch takes tensors of one type.
   for (int type = 0; type < 3; ++type) {
     std::vector<void*> tp, tm, tv;
     std::vector<const void*> tg;
     std::vector<unsigned char*> tms, tvs;
+    std::vector<unsigned> tk;
     std::vector<long> tn;
     for (size_t i = 0; i < count; ++i) {
       if (p[i].numel() == 0 || elem_type(p[i], "adamw_step") != type) continue;
@@ -655,12 +668,14 @@ void adamw_step(const Tensors& p, const Tensors& g, const Tensors& m,
         tms.push_back((*ms)[i].data_ptr<uint8_t>());
         tvs.push_back((*vs)[i].data_ptr<uint8_t>());
       }
+      if (!keys.empty()) tk.push_back(keys[i]);
       tn.push_back(p[i].numel());
     }
     if (tp.empty()) continue;
     const AdamWTensors a{(int)tp.size(), tp.data(), tg.data(), tm.data(),
                          tv.data(), ms ? tms.data() : nullptr,
-                         ms ? tvs.data() : nullptr, tn.data()};
+                         ms ? tvs.data() : nullptr,
+                         tk.empty() ? nullptr : tk.data(), tn.data()};
     launched(adamw_launch(&a, &s, type, stream), "adamw_step");
   }
   for (size_t i = 0; i < count; ++i) {

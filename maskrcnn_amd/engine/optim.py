@@ -20,7 +20,9 @@ class AdamW(torch.optim.Optimizer):
     """AdamW with decoupled weight decay, states in 32 or 8 bits.
 
     params: as torch.optim's, float32, bfloat16 or float16, dense.
-    state_bits: 32, or 8 for codes with a scale for 256 values.
+    state_bits: 32, or 8 for codes with a scale for 256 values, rounded at
+    random (repeatably, by the step's number) so that they follow the fp32
+    states in the mean.
     max_grad_norm: clips the norm over the gradients of all groups; the last
     step's norm is kept on the device as .grad_norm. A step may not be
     captured into a graph, as its number and rate are the host's.
@@ -71,7 +73,7 @@ class AdamW(torch.optim.Optimizer):
                      for p in group["params"] if p.grad is not None]
             if grads:
                 norm = self.grad_norm = grad_norm(grads)
-        for group in self.param_groups:
+        for at, group in enumerate(self.param_groups):
             # Parameters that have missed steps have a number of their own;
             # a call takes those of one number and device.
             calls = {}
@@ -97,7 +99,8 @@ class AdamW(torch.optim.Optimizer):
                     if eight else None,
                     step=number, lr=group["lr"], betas=group["betas"],
                     eps=group["eps"], weight_decay=group["weight_decay"],
-                    grad_norm=norm, max_grad_norm=self.max_grad_norm or 0.0)
+                    grad_norm=norm, max_grad_norm=self.max_grad_norm or 0.0,
+                    seed=at if eight else None)
         return loss
 
     def load_state_dict(self, state_dict):

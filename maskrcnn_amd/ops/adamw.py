@@ -13,8 +13,11 @@ With betas from 0.5 on a state is formed as m + (1 - beta1) (c g - m) with one
 rounding of the result.
 
 8-bit states: 256 values in memory order share a power of two, and a value
-is its ratio to it with 3 bits of mantissa (pack_state8, unpack_state8); a
-step's new codes are those of the unrounded states.
+is its ratio to it with 3 bits of mantissa (pack_state8, unpack_state8).
+Without a seed a step's new codes are the nearest to the unrounded states.
+With one they are the code below or above, at random, so that their mean is
+the unrounded state: over many steps the nearest codes would lose whatever
+moves a state by less than half a code, a beta of 0.999 all of its decay.
 """
 
 from __future__ import annotations
@@ -38,11 +41,50 @@ def _is_dense(t):
     return torch.ops.aten.is_non_overlapping_and_dense(t)
 
 
-def _pack_torch(x, signed):
+# Bits of random numbers (csrc/hip/adamw.hip has the same).
+_WORD = 0xFFFFFFFF
+_ODD = (0xAC9B39D5, 0x8FE44835)
+
+
+def _mix(x):
+    """A hash of 32 bits, of an int or of int64 values."""
+    x = ((x ^ (x >> 16)) * _ODD[0]) & _WORD
+    x = ((x ^ (x >> 15)) * _ODD[1]) & _WORD
+    return x ^ (x >> 16)
+
+
+def _keys(seed, step, count):
+    """A key for each tensor of a call, by its number."""
+    key = 0
+    for word in (seed & _WORD, seed >> 32 & _WORD, step & _WORD, step >> 32):
+        key = _mix((key + word + _ODD[0]) & _WORD)
+    return [_mix((key + i + _ODD[0]) & _WORD) for i in range(count)]
+
+
+def _hashes(key, n):
+    at = torch.arange(n)
+    return _mix((at & _WORD) ^ (key ^ (((at >> 32) * _ODD[1]) & _WORD)))
+
+
+def _cut(x, bits):
+    """x up or down to 3 bits of mantissa, by 20 random bits."""
+    raw = x.view(torch.int32)
+    mag = raw & 0x7FFFFFFF
+    up = mag.long() + bits
+    y = torch.where(up < 0x7F800000, up, mag.long()) & 0x7FF00000
+    return (y.to(torch.int32) | (raw & -0x80000000)).view(torch.float32)
+
+
+def _pack_torch(x, signed, hashes=None):
     low, top = (14, 127) if signed else (30, 255)
     n = x.numel()
     flat = torch.zeros(-(-n // BLOCK8) * BLOCK8, dtype=torch.float32)
     flat[:n] = _dense(x)
+    above = flat > 0
+    if hashes is not None:
+        h = torch.zeros(flat.numel(), dtype=torch.int64)
+        h[:n] = hashes
+        flat = _cut(flat, h & 0xFFFFF if signed else h >> 12)
     bits = flat.view(torch.int32) & 0x7FFFFFFF
     blocks = bits.view(-1, BLOCK8)
     e = (blocks.amax(1) >> 23).clamp(min=_MIN_EXP) if n else \
@@ -54,15 +96,17 @@ def _pack_torch(x, signed):
     rb = r.view(torch.int32)
     code = ((rb + 0x7FFFF + ((rb >> 20) & 1)) >> 20) - ((126 - low) << 3)
     small = r < 2.0 ** -low
-    code = torch.where(
-        small, torch.round(torch.where(small, r, torch.zeros_like(r)) *
-                           2.0 ** (low + 3)).to(torch.int32),
-        code.clamp(max=top))
+    q = torch.where(small, r, torch.zeros_like(r)) * 2.0 ** (low + 3)
+    if hashes is None:
+        q = torch.round(q)
+    else:
+        u = (_mix((h + (1 if signed else 2)) & _WORD) >> 8) * 2.0 ** -24
+        q = torch.floor(q) + (u < q - torch.floor(q))
+    code = torch.where(small, q.to(torch.int32), code.clamp(max=top))
     if signed:
         code = code | ((flat.view(torch.int32) < 0).to(torch.int32) << 7)
     else:
-        code = torch.where((flat > 0) & (code == 0),
-                           torch.ones_like(code), code)
+        code = torch.where(above & (code == 0), torch.ones_like(code), code)
     code = torch.where((e == 255).repeat_interleave(BLOCK8),
                        torch.zeros_like(code), code)
     codes = torch.empty_strided(x.shape, x.stride(), dtype=torch.uint8)
@@ -131,14 +175,17 @@ def grad_norm(tensors) -> torch.Tensor:
 
 
 def _moved(state, value, beta, codes, lerp):
-    """The state after `value`, rounded once to fp32 (csrc/hip/adamw.hip)."""
+    """The state after `value`, rounded once to fp32 (csrc/hip/adamw.hip).
+    codes: None for fp32 states, else how they are rounded to 8 bits."""
     if not lerp:
         return state * beta + value * (1.0 - beta)
     weight = float(torch.tensor(1.0 - beta, dtype=torch.float32))
     wide = state.double() + (value - state).double() * weight
     x = wide.float()
-    if not codes:
+    if codes is None:
         return torch.where(state.isinf(), state + value, x)
+    if codes == "random":
+        return x
     bits = x.view(torch.int32)
     lost = (value - state).double() * weight + (state - x).double()
     up = (torch.sign(lost) * torch.sign(x)).to(torch.int32)
@@ -163,7 +210,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *,
                exp_avg_scales=None, exp_avg_sq_scales=None, step: int,
                lr: float, betas=(0.9, 0.999), eps: float = 1e-8,
                weight_decay: float = 0.0, grad_norm=None,
-               max_grad_norm: float = 0.0) -> None:
+               max_grad_norm: float = 0.0, seed: int = None) -> None:
     """Updates params and their states in place.
 
     params: float32, bfloat16 or float16, dense, in any mixture; grads: in
@@ -173,6 +220,13 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *,
     both for a state that begins). step: the number of this step, from 1.
     grad_norm: one float32 on the device (of grad_norm()); the gradients
     count as scaled to max_grad_norm where it is above that.
+    seed: new 8-bit codes are rounded at random, without bias, by a hash of
+    seed, step, the tensor's number in the lists and the value's place; the
+    same call gives the same codes. None: they are rounded to nearest, which
+    is for a step by itself. Over many steps give a seed: to nearest, a state
+    that a step moves by less than half a code does not move at all, and with
+    betas[1] above some 0.97 a second moment then never falls. fp32 states
+    take no seed into account.
 
     step and lr are the host's, so the call is refused while a stream is
     captured into a graph. A tensor to write may share memory with no other.
@@ -189,7 +243,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *,
         require_ext().adamw_step(
             params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales,
             exp_avg_sq_scales, grad_norm, max_grad_norm, step, lr, beta1,
-            beta2, eps, weight_decay)
+            beta2, eps, weight_decay,
+            None if seed is None else seed & (1 << 64) - 1)
         return
     eight = exp_avg_scales is not None
     if eight != (exp_avg_sq_scales is not None) or not (
@@ -201,9 +256,12 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *,
     if grad_norm is not None:
         clip = (torch.full_like(grad_norm, max_grad_norm) /
                 (grad_norm + 1e-6)).clamp(max=1.0)
+    random = eight and seed is not None
+    keys = _keys(seed, int(step), len(params)) if random else None
     scalars = (clip, beta1, beta2, eps, 1.0 - lr * weight_decay,
                lr / (1.0 - beta1 ** step),
-               1.0 / math.sqrt(1.0 - beta2 ** step), eight)
+               1.0 / math.sqrt(1.0 - beta2 ** step),
+               ("random" if random else "nearest") if eight else None)
     for i, (p, g, m, v) in enumerate(zip(params, grads, exp_avgs,
                                          exp_avg_sqs)):
         want = torch.uint8 if eight else torch.float32
@@ -224,6 +282,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *,
         for codes, scales, x, signed in (
                 (m, exp_avg_scales[i], mf, True),
                 (v, exp_avg_sq_scales[i], vf, False)):
-            new, exps = pack_state8(x, signed)
+            new, exps = _pack_torch(
+                x, signed, _hashes(keys[i], p.numel()) if random else None)
             codes.copy_(new)
             scales.copy_(exps)

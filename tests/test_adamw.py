@@ -543,3 +543,172 @@ def test_codes_are_the_unrounded_states(device):
     square = g * g
     want = (1.0 + square.double()) / 2
     assert torch.equal(unpack_state8(vc, vs, False), grid(want, False))
+
+
+# ------------------------------------------ 8-bit states rounded at random
+
+def eight(m, v):
+    """(codes of m, codes of v, the scales as adamw_step takes them)"""
+    (m, ms), (v, vs) = (map(list, zip(*[pack_state8(t, k == 0) for t in s]))
+                        for k, s in enumerate((m, v)))
+    return m, v, dict(exp_avg_scales=ms, exp_avg_sq_scales=vs)
+
+
+def held(m, v, scales, i=0):
+    return (unpack_state8(m[i], scales["exp_avg_scales"][i], True),
+            unpack_state8(v[i], scales["exp_avg_sq_scales"][i], False))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("betas", [(0.9, 0.999), (0.3, 0.2)])
+def test_seeded_codes_have_the_states_mean(device, dtype, betas):
+    """Over 400 seeds: each code lies next to the unrounded state, and their
+    mean is the state to six deviations (each at most half a distance of two
+    codes), value by value and over all values."""
+    n, seeds = 600, 400
+    p, g, m, v = tensors([n], dtype, device)
+    spread = torch.exp(3 * torch.randn(
+        n, generator=torch.Generator().manual_seed(1))).to(device)
+    m[0], v[0] = m[0] * spread, v[0] * spread
+    m, v, scales = eight(m, v)
+    hyper = dict(HYPER, betas=betas)
+    _, em, ev, _ = exact(p[0], g[0], *held(m, v, scales), 1.0, **hyper)
+    total = [0.0, 0.0]
+    for seed in range(seeds):
+        a = [[t.clone() for t in k] for k in (p, m, v)]
+        s = {k: [t.clone() for t in x] for k, x in scales.items()}
+        adamw_step(a[0], g, a[1], a[2], **s, seed=seed, **hyper)
+        if seed == 0:       # the update goes by the unrounded states
+            one = [[t.clone() for t in k] for k in (p, m, v)]
+            adamw_step(one[0], g, one[1], one[2], **hyper, **{
+                k: [t.clone() for t in x] for k, x in scales.items()})
+            assert torch.equal(one[0][0], a[0][0])
+        got = held(a[1], a[2], s)
+        for k, (x, want) in enumerate(zip(got, (em, ev))):
+            # The code's distance: an eighth of the power of two below; for
+            # the smallest, of the block's exponent or the next.
+            low = 14 if k == 0 else 30
+            _, e = torch.frexp(want.abs())
+            top = torch.zeros(-(-n // BLOCK) * BLOCK, dtype=torch.float64,
+                              device=device)
+            top[:n] = want.abs()
+            _, unit = torch.frexp(top.view(-1, BLOCK).amax(1))
+            unit = unit.repeat_interleave(BLOCK)[:n]
+            dist = 2.0 ** torch.maximum(e - 4, unit - low - 3).double()
+            err = 5 * U * (want.abs() + g[0].double().abs() ** (k + 1))
+            assert ((x.double() - want).abs() <= dist + err).all()
+            total[k] = total[k] + (x.double() - want) / dist
+    for t in total:
+        t = t / seeds
+        assert (t.abs() <= 6 * 0.5 / seeds ** 0.5).all()
+        assert abs(t.mean()) <= 6 * 0.5 / (seeds * n) ** 0.5
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_seeded_calls_repeat(device):
+    p, g, m, v = tensors([700, 700, 300], torch.float32, device)
+    for k in (p, g, m, v):
+        k[1].copy_(k[0])
+    m, v, scales = eight(m, v)
+
+    def step(seed, only=slice(None), **more):
+        a = [[t.clone() for t in k[only]] for k in (p, g, m, v)]
+        s = {k: [t.clone() for t in x[only]] for k, x in scales.items()}
+        adamw_step(*a, **s, seed=seed, **{**HYPER, **more})
+        return a[2] + a[3]
+    one = step(5)
+    assert all(torch.equal(a, b) for a, b in zip(one, step(5)))
+    # Other seeds, steps and tensors have bits of their own.
+    for other in (step(6), step(5 + (1 << 40)), step(-5), step(5, step=8)):
+        assert not torch.equal(one[0], other[0])
+        assert not torch.equal(one[3], other[3])
+    assert not torch.equal(one[0], one[1])
+    alone = step(5, slice(0, 1))
+    assert torch.equal(one[0], alone[0]) and torch.equal(one[3], alone[1])
+    # fp32 states take no seed into account.
+    a, b = (tensors([300], torch.float32, device) for _ in range(2))
+    adamw_step(*a, **HYPER)
+    adamw_step(*b, seed=1, **HYPER)
+    assert all(torch.equal(x[0], y[0]) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("n", [1, 255, 257, 600])
+def test_seeded_edges(device, n):
+    """Zeros stay zeros, a v above zero never gets the code of zero, the
+    largest finite states stay finite, and NaN stays in its block."""
+    z = torch.zeros(n, device=device)
+    for seed in range(20):
+        m, v, scales = eight([z], [z])
+        adamw_step([z.clone()], [z], m, v, **scales, seed=seed, **HYPER)
+        assert not m[0].any() and not v[0].any()
+        x = z + 1e-30
+        x[0] = 1.0
+        m, v, scales = eight([z + 3.3e38], [x])
+        adamw_step([z.clone()], [z], m, v, **scales, seed=seed,
+                   **dict(HYPER, betas=(0.9999999, 0.9999999)))
+        mm, vv = held(m, v, scales)
+        assert mm.isfinite().all() and (mm >= 1.875 * 2.0 ** 127).all()
+        assert (vv > 0).all() and 0.875 <= vv[0] <= 1.125
+    g = z.clone()
+    g[-1] = float("nan")
+    m, v, scales = eight([z + 1], [z + 1])
+    adamw_step([z.clone()], [g], m, v, **scales, seed=3, **HYPER)
+    for y in held(m, v, scales):
+        last = (n - 1) // BLOCK * BLOCK
+        assert y[last:].isnan().all() and y[:last].isfinite().all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_seeded_largest_value_grows(device):
+    """A block whose values lie at the exponent's last code, 1.875, and whose
+    steps are far below the distance to the next one, 2."""
+    n = 4096
+    z = torch.zeros(n, device=device)
+    m, v, scales = eight([z], [z + 1.875])
+    for step in range(1, 401):
+        adamw_step([z.clone()], [z + 4.0 ** 0.5], m, v, **scales, seed=0,
+                   step=step, lr=0.0, betas=(0.9, 0.999))
+    want = 4.0 - (4.0 - 1.875) * 0.999 ** 400
+    # Variance: 400 steps of at most (1 - beta2) (4 - v) D, D at most 1/4.
+    dev = (400 * 0.001 * 2.125 * 0.25 / n) ** 0.5
+    assert abs(float(held(m, v, scales)[1].double().mean()) - want) <= 6 * dev
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gpu_gives_the_cpu_seeded_states(dtype):
+    sizes = [1, 300, 4096, 10000, 0, 7]
+    p, g, m, v = tensors(sizes, dtype, "cpu")
+    m[2] *= torch.exp(6 * torch.randn(          # small codes as well
+        4096, generator=torch.Generator().manual_seed(1)))
+    m, v, scales = eight(m, v)
+    a = (p, g, m, v)
+    b = [[t.cuda() for t in k] for k in a]
+    bs = {k: [t.cuda() for t in s] for k, s in scales.items()}
+    for step in (1, 2, 50, (1 << 33) + 5):
+        h = dict(HYPER, step=step, seed=(1 << 50) + 3)
+        adamw_step(*a, **scales, **h)
+        adamw_step(*b, **bs, **h)
+        for x, y in zip((*a[2:], *scales.values()), (*b[2:], *bs.values())):
+            for s, t in zip(x, y):
+                assert torch.equal(s, t.cpu())
+
+
+@pytest.mark.gpu
+def test_seeded_places_past_32_bits():
+    n = (1 << 32) + 600
+    p = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    g = torch.full_like(p, 0.3)
+    m, v = (torch.zeros(n, dtype=torch.uint8, device="cuda")
+            for _ in range(2))
+    s = [torch.zeros(-(-n // BLOCK), dtype=torch.uint8, device="cuda")
+         for _ in range(2)]
+    adamw_step([p], [g], [m], [v], exp_avg_scales=s[:1],
+               exp_avg_sq_scales=s[1:], seed=0, step=1, lr=0.5)
+    for t in (m, v):
+        first, last = t[:600], t[-600:]
+        assert len(first.unique()) == 2 and len(last.unique()) == 2
+        assert not torch.equal(first, last)
+    assert (p[-600:] == p[0]).all() and p[0] < 0

@@ -317,3 +317,49 @@ def test_keras_map_without_the_heads_batch_norms():
     gone = set(full) - set(less)
     assert gone and all(k.startswith(("mrcnn_class_bn1/", "mrcnn_class_bn2/"))
                         for k in gone)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("beta2", [0.99, 0.999])
+@pytest.mark.parametrize("then", [1.0, 0.1, 0.0])
+@pytest.mark.parametrize("normal", [True, False])
+def test_8_bit_states_follow_over_many_steps(device, beta2, then, normal):
+    """3000 steps beside fp32 states, on normal or constant gradients, from
+    the middle on `then` times as large.
+
+    v in 8 bits has v's mean. A step that moves it by d between codes D apart
+    adds at most |d| D to its variance, with d = (1 - beta2)(g^2 - v) and D at
+    most v / 8; the older variance falls by beta2^2. The mean over the values
+    is held to six of its deviations.
+    """
+    n, steps = 2048, 3000
+    g = torch.Generator().manual_seed(0)
+    bank = torch.randn(500, n, generator=g) if normal else torch.ones(500, n)
+    bank = bank.to(device)
+    p, q = (nn.Parameter(torch.zeros(n, device=device)) for _ in range(2))
+    kw = dict(lr=1e-3, betas=(0.9, beta2), weight_decay=0.0)
+    wide, narrow = AdamW([p], **kw), AdamW([q], state_bits=8, **kw)
+    var = torch.zeros(n, dtype=torch.float64, device=device)
+    moved = [0.0, 0.0]
+    for t in range(steps):
+        p.grad = q.grad = bank[t % 500] * (1.0 if t < steps // 2 else then)
+        if t >= steps - 300:
+            was = p.detach().clone(), q.detach().clone()
+        if t:
+            v = wide.state[p]["exp_avg_sq"].double()
+            var = beta2 ** 2 * var + (1 - beta2) / 8 * (
+                p.grad.double().square() * v + v * v + var)
+        wide.step()
+        narrow.step()
+        if t >= steps - 300:
+            for i, (a, b) in enumerate(zip((p, q), was)):
+                moved[i] += float((a.detach() - b).double().square().mean())
+    s = narrow.state[q]
+    want = wide.state[p]["exp_avg_sq"].double().mean()
+    got = unpack_state8(s["exp_avg_sq"], s["exp_avg_sq_scale"],
+                        False).double().mean()
+    assert abs(got - want) <= 6 * (var.mean() / n).sqrt()
+    # Updates: 1 / v of a spread of a quarter to a half has a mean 1.07 to
+    # 1.33 times that of none, m's own rounding adds a fifth to its square.
+    if then:
+        assert 0.95 <= (moved[1] / moved[0]) ** 0.5 <= 1.35
