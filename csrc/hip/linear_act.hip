@@ -5,11 +5,14 @@
 //   dz = dy act'(z)    dx = dz W           dW = dz^T x      db = sum dz
 //
 // What is kept for the backward: act'(z), formed where z is still in fp32, so
-// that no erf or exp is computed twice. With 16-bit tensors it is a 16-bit
-// fixed point number, off by 2^-16 at most, a small part of what dz's one
-// rounding costs (the matrix cores take dz in the tensors' type; db sums it
-// unrounded); in bf16 or fp16 the derivative's own rounding would cost as
-// much again. ReLU's 0 and 1 are exact.
+// that no erf or exp is computed twice. With 16-bit tensors it has 16 bits too:
+// from 2^-7 on (2^-6 for fp16) steps of 2^-15, where bf16's or fp16's own
+// rounding would cost as much again as dz's (the matrix cores take dz in the
+// tensors' type; db sums it unrounded), and below that 8 (9) bits of mantissa
+// down to 2^-52 (2^-28): fixed point alone would lose the small derivatives of
+// GELU below -4 and SiLU below -9 in part, and below -4.84 and -13.6 in whole.
+// A kept one is off by 2^-16 at most, and below those borders by 2^-9 (2^-10) of
+// itself, half of bf16's own rounding. ReLU's 0 and 1 are exact.
 //
 // All three products are one kernel, D[m][n] = sum_k X(m,k) Y(n,k), where
 // either operand may lie with k consecutive or with its own index
@@ -297,19 +300,63 @@ __device__ inline float activate(float z, float& slope) {
   return z;
 }
 
-// The derivative as it is kept: fp32 as it is; else in steps of 2^-15 from
-// -1/4 (all of them lie between -0.13 and 1.13), the last number for NaN.
+// The derivative as it is kept: fp32 as it is; else a code of its magnitude in
+// 14 bits, or 16 where it is above zero (all derivatives lie between -0.13 and
+// 1.13): the two highest bits together are the sign, the last code is NaN.
+// Magnitudes from `line` on are whole numbers of 2^-15. Those below are the
+// exponent and first kBits bits of an fp32 number times a power of two, which
+// makes the codes meet at `line` and the smallest ones subnormal. bf16 has dz's
+// exponents to go with 2^-52; in fp16 dz ends at 2^-24 and has more bits.
 template <typename T>
 using Kept = std::conditional_t<sizeof(T) == 4, float, unsigned short>;
 
-__device__ inline float keep(float slope, float) { return slope; }
-__device__ inline float keep(float slope, unsigned short) {
-  return slope == slope ? rintf(slope * 32768.0f) + 8192.0f : 65535.0f;
+template <typename T>
+struct Code16 {
+  static constexpr int bits = std::is_same_v<T, fp16_t> ? 9 : 8;
+  static constexpr int below = 11776;               // codes below the line
+  static constexpr int drop = 23 - bits;            // bits of fp32's mantissa
+  static constexpr float line = 1.0f / (1 << (15 - bits));
+  // Whole numbers of 2^-15 start at 2^bits on the line.
+  static constexpr int shift = below - (1 << bits);
+  // The line's exponent is 127 + bits - 15, its code's below >> bits.
+  static constexpr int scale = 127 + bits - 15 - (below >> bits);
+  static_assert(below % (1 << bits) == 0 && scale > 0, "whole binades");
+  static_assert(shift + 36993 < 0xc000 && shift + 4225 < 0x3fff,
+                "GELU's 1.1289 and -0.1289 have codes");
+};
+
+template <typename T>
+__device__ inline Kept<T> keep(float slope) {
+  if constexpr (sizeof(T) == 4) {
+    return slope;
+  } else {
+    using C = Code16<T>;
+    const float a = fabsf(slope);
+    const unsigned b =
+        __float_as_uint(a * __int_as_float((127 - C::scale) << 23));
+    const unsigned few =
+        (b + (1 << (C::drop - 1)) - 1 + ((b >> C::drop) & 1)) >> C::drop;
+    const unsigned whole = (unsigned)(int)rintf(a * 32768.0f) + C::shift;
+    const unsigned code =
+        (a < C::line ? few : whole) | (slope < 0.0f ? 0xc000u : 0u);
+    return (Kept<T>)(slope == slope ? code : 0xffffu);
+  }
 }
-__device__ inline float kept(float k, float) { return k; }
-__device__ inline float kept(float k, unsigned short) {
-  return k == 65535.0f ? __int_as_float(0x7fc00000)
-                       : (k - 8192.0f) * (1.0f / 32768.0f);
+
+template <typename T>
+__device__ inline float kept(Kept<T> k) {
+  if constexpr (sizeof(T) == 4) {
+    return k;
+  } else {
+    using C = Code16<T>;
+    const bool negative = k >= 0xc000;
+    const unsigned code = negative ? k & 0x3fffu : k;
+    const float few = __uint_as_float(code << C::drop) *
+                      __int_as_float((127 + C::scale) << 23);
+    const float whole = (float)((int)code - C::shift) * (1.0f / 32768.0f);
+    const float a = code < C::below ? few : whole;
+    return k == 0xffff ? __int_as_float(0x7fc00000) : negative ? -a : a;
+  }
 }
 
 constexpr int kOut = 8;       // consecutive columns that a lane finishes
@@ -351,13 +398,19 @@ __device__ inline void finish(const LinearEpilogue& e, long m, int n, int N,
   K* slopes = e.kept ? (K*)e.kept + m * (long)N + n : nullptr;
   float slope;
   if (kAct != kActNone && slopes) {
-    float k[kOut];
+    K k[kOut];
 #pragma unroll
     for (int i = 0; i < kOut; ++i) {
       z[i] = activate<T, kAct>(z[i] + b[i], slope);
-      k[i] = keep(slope, K{});
+      k[i] = keep<T>(slope);
     }
-    store_some<K, kOut>(slopes, N - n, k);
+    if (n + kOut <= N) {
+      __builtin_memcpy(slopes, k, sizeof(k));
+    } else {
+#pragma unroll
+      for (int i = 0; i < kOut; ++i)
+        if (n + i < N) slopes[i] = k[i];
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < kOut; ++i)
@@ -654,7 +707,8 @@ __global__ __launch_bounds__(256) void dz_kernel(
   const int r0 = blockIdx.y * rows, r1 = r0 + rows < m ? r0 + rows : m;
   float sum[8] = {};
   for (int r = r0 + (threadIdx.x >> 5); r < r1; r += 8 * kDeep) {
-    float g[kDeep][8], s[kDeep][8];
+    float g[kDeep][8];
+    Kept<T> s[kDeep][8];
 #pragma unroll
     for (int d = 0; d < kDeep; ++d) {
       const int row = r + 8 * d;
@@ -662,7 +716,13 @@ __global__ __launch_bounds__(256) void dz_kernel(
       const Kept<T>* q = slopes + (long)row * n + c;
       if (row >= r1) continue;
       load_some<T, 8>(p, n - c, g[d]);
-      if (kAct) load_some<Kept<T>, 8>(q, n - c, s[d]);
+      if (!kAct) continue;
+      if (n - c >= 8) {
+        __builtin_memcpy(s[d], q, sizeof(s[d]));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[d][i] = i < n - c ? q[i] : Kept<T>{};
+      }
     }
 #pragma unroll
     for (int d = 0; d < kDeep; ++d) {
@@ -670,7 +730,7 @@ __global__ __launch_bounds__(256) void dz_kernel(
       if (row >= r1) continue;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        if (kAct) g[d][i] *= kept(s[d][i], Kept<T>{});
+        if (kAct) g[d][i] *= kept<T>(s[d][i]);
         sum[i] += g[d][i];
       }
       if (dz) {

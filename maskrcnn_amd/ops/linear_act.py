@@ -24,13 +24,27 @@ def _act_torch(z, act):
     if act == "relu":
         return z.clamp(min=0), (z > 0).to(z.dtype)
     if act == "gelu":
-        cdf = 0.5 * (1.0 + torch.erf(z * math.sqrt(0.5)))
+        cdf = 0.5 * torch.erfc(z * -math.sqrt(0.5))
         return z * cdf, cdf + z * torch.exp(-0.5 * z * z) / \
             math.sqrt(2.0 * math.pi)
     if act == "silu":
         s = torch.sigmoid(z)
         return z * s, s * (1.0 + z * (1.0 - s))
     return z, torch.ones_like(z)
+
+
+# Mantissa bits of a small derivative in 16 bits, and its smallest exponent.
+_KEPT = {torch.bfloat16: (8, -52), torch.float16: (9, -28)}
+
+
+def _keep(slope, dtype):
+    """The derivative as it is kept beside 16-bit tensors: in steps of 2^-15,
+    small ones in those of their own exponent (csrc/hip/linear_act.hip)."""
+    bits, least = _KEPT[dtype]
+    _, e = torch.frexp(slope)
+    step = torch.ldexp(torch.ones_like(slope),
+                       (e - 1).clamp(min=least, max=bits - 15) - bits)
+    return torch.round(slope / step) * step
 
 
 def _fwd_torch(x, weight, bias, act, residual):
@@ -43,9 +57,8 @@ def _fwd_torch(x, weight, bias, act, residual):
         y = y + residual.to(wide)
     if act == "none":
         return y.to(x.dtype), None
-    if x.dtype in (torch.bfloat16, torch.float16):
-        # Steps of 2^-15, as 16 bits hold it; ReLU's 0 and 1 are exact.
-        slope = torch.round(slope * 32768.0) / 32768.0
+    if x.dtype in _KEPT:
+        slope = _keep(slope, x.dtype)
     return y.to(x.dtype), slope
 
 
@@ -85,10 +98,10 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor,
     residual: [..., N] or None. All in one type, float32, bfloat16 or
     float16, of any strides; sums are in fp32. activation: "none", "relu",
     "gelu" (by erf) or "silu". Returns a contiguous [..., N] in x's type.
-    In 16 bits act'(z) is kept for the backward in steps of 2^-15 (ReLU's is
-    exact), and the gradient of z is rounded to x's type once. The gradients
-    have no gradients (create_graph). On the GPU rows may lie up to 8 MB
-    apart.
+    In 16 bits act'(z) is kept for the backward to 2^-16, and where it is
+    small to 2^-9 (bf16) or 2^-10 (fp16) of itself (ReLU's is exact); the
+    gradient of z is rounded to x's type once. The gradients have no gradients
+    (create_graph). On the GPU rows may lie up to 8 MB apart.
     """
     act = _INDEX.get(activation)
     if act is None:

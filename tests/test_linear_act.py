@@ -447,3 +447,35 @@ def test_bias_may_change_before_the_backward(device):
         b.add_(1.0)
     db, = torch.autograd.grad(y, b, dy)
     assert torch.allclose(db, dy.sum(0), rtol=1e-5, atol=1e-5)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype,bits,least", [(torch.bfloat16, 8, -61),
+                                              (torch.float16, 9, -38)])
+@pytest.mark.parametrize("act,lowest", [("gelu", -8.0), ("silu", -30.0)])
+def test_small_derivatives(device, dtype, bits, least, act, lowest):
+    """With one weight of 1 the gradient of x is the kept derivative times dy.
+
+    It is off by dz's rounding, by half of what the derivative is kept to
+    (steps of 2^-15, or `bits` bits of itself below 2^(bits - 15), or half the
+    smallest step), and by 2^-12 of itself for the functions: 16-bit GELU's
+    integral is off by 1% of itself at -8, which is 1/64 of its derivative,
+    and less above; fp32's exponentials by 1e-5 at most.
+    """
+    z = torch.linspace(lowest, 8.0, 2049).to(dtype).double()
+    dy = 1.0 if dtype == torch.bfloat16 else 1024.0
+    x = z.to(device, dtype)[:, None].requires_grad_()
+    one = torch.ones(1, 1, dtype=dtype, device=device)
+    dx, = torch.autograd.grad(linear_act(x, one, None, act), x,
+                              torch.full_like(x, dy))
+    _, slope = act64(z, act)
+    kept = torch.where(slope.abs() < 2.0 ** (bits - 15),
+                       slope.abs() * 2.0 ** -(bits + 1) + 2.0 ** least,
+                       2.0 ** -16)
+    info = torch.finfo(dtype)
+    lim = dy * (kept + slope.abs() * (info.eps / 2 * 1.01 + 2.0 ** -12)) + \
+        info.smallest_normal * info.eps / 2
+    off = (dx[:, 0].double().cpu() - dy * slope).abs()
+    assert (off <= lim).all(), z[off > lim]
+    big = slope.abs() * dy > info.smallest_normal
+    assert (dx[:, 0].cpu() != 0)[big].all()
