@@ -457,6 +457,16 @@ class LinearActNode
   }
 };
 
+// The kernels know no tangents: a result without one would count as a
+// derivative of zero.
+void refuse_forward_mode(std::initializer_list<const Tensor*> inputs,
+                         const char* what) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor* t : inputs)
+    TORCH_CHECK_NOT_IMPLEMENTED(t == nullptr || !t->_fw_grad(0).defined(), what,
+                                ": no forward-mode derivatives");
+}
+
 bool wants_grad(const std::optional<Tensor>& t) {
   return t && t->requires_grad();
 }
@@ -464,6 +474,7 @@ bool wants_grad(const std::optional<Tensor>& t) {
 Tensor linear_act(const Tensor& x, const Tensor& w,
                   const std::optional<Tensor>& bias, int64_t act,
                   const std::optional<Tensor>& residual) {
+  refuse_forward_mode({&x, &w, given(bias), given(residual)}, "linear_act");
   if (at::GradMode::is_enabled() &&
       (x.requires_grad() || w.requires_grad() || wants_grad(bias) ||
        wants_grad(residual)))
@@ -509,6 +520,7 @@ class LayerNormNode : public torch::autograd::Function<LayerNormNode> {
 
 Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& w,
                   const std::optional<Tensor>& b, double eps) {
+  refuse_forward_mode({&x, given(w), given(b)}, "layer_norm");
   if (at::GradMode::is_enabled() &&
       (x.requires_grad() || wants_grad(w) || wants_grad(b)))
     return LayerNormNode::apply(x, w, b, eps);

@@ -64,8 +64,8 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor = None,
 
     weight, bias: [C] or None (1 and 0), in x's type or float32, both in
     one type. Returns a contiguous tensor of x's shape and type. x may be
-    float32, bfloat16 or float16, of any strides. The gradients
-    have no gradients (create_graph).
+    float32, bfloat16 or float16, of any strides. The gradients have no
+    gradients (create_graph), and forward-mode derivatives are refused.
     """
     if x.is_cuda:
         return require_ext().layer_norm(x, weight, bias, eps)

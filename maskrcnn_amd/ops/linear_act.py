@@ -101,7 +101,8 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor,
     In 16 bits act'(z) is kept for the backward to 2^-16, and where it is
     small to 2^-9 (bf16) or 2^-10 (fp16) of itself (ReLU's is exact); the
     gradient of z is rounded to x's type once. The gradients have no gradients
-    (create_graph). On the GPU rows may lie up to 8 MB apart.
+    (create_graph), and forward-mode derivatives are refused. On the GPU rows
+    may lie up to 8 MB apart.
     """
     act = _INDEX.get(activation)
     if act is None:

@@ -374,3 +374,19 @@ def test_bias_may_change_before_the_backward(device):
         b.add_(1.0)
     db, = torch.autograd.grad(y, b, dy)
     assert torch.allclose(db, dy.sum(0), rtol=1e-5, atol=1e-5)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_is_refused(device, grad):
+    """A result without a tangent would count as a derivative of zero."""
+    args = inputs(4, 16, torch.float32, torch.float32, device)[:3]
+    with torch.autograd.forward_ad.dual_level():
+        for i in range(3):
+            given = [t.clone().requires_grad_(grad and i != j)
+                     for j, t in enumerate(args)]
+            given[i] = torch.autograd.forward_ad.make_dual(
+                given[i], torch.ones_like(given[i]))
+            with pytest.raises(NotImplementedError):
+                layer_norm(*given)
+    assert layer_norm(*args).isfinite().all()

@@ -479,3 +479,20 @@ def test_small_derivatives(device, dtype, bits, least, act, lowest):
     assert (off <= lim).all(), z[off > lim]
     big = slope.abs() * dy > info.smallest_normal
     assert (dx[:, 0].cpu() != 0)[big].all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_is_refused(device, grad):
+    """A result without a tangent would count as a derivative of zero."""
+    args = inputs(4, 16, 8, torch.float32, device)[:4]
+    with torch.autograd.forward_ad.dual_level():
+        for i in range(4):
+            given = [t.clone().requires_grad_(grad and i != j)
+                     for j, t in enumerate(args)]
+            given[i] = torch.autograd.forward_ad.make_dual(
+                given[i], torch.ones_like(given[i]))
+            x, w, b, r = given
+            with pytest.raises(NotImplementedError):
+                linear_act(x, w, b, "gelu", r)
+    assert linear_act(*args[:3]).isfinite().all()
