@@ -103,17 +103,40 @@ class AdamW(torch.optim.Optimizer):
                     seed=at if eight else None)
         return loss
 
+    def _check_saved(self, p, saved):
+        """Raises ValueError if `saved` is no state for p."""
+        want = torch.float32 if self.state_bits == 32 else torch.uint8
+        names = [n for m in _MOMENTS for n in m[:1 if want.is_floating_point
+                                                else 2]]
+        if "step" not in saved or any(
+                n not in saved or saved[n].dtype != want for n in names):
+            raise ValueError(f"AdamW: not states of {self.state_bits} bits")
+        for name, scale, _ in _MOMENTS:
+            if saved[name].shape != p.shape:
+                raise ValueError(
+                    f"AdamW: a saved {name} of {tuple(saved[name].shape)} "
+                    f"for a parameter of {tuple(p.shape)}")
+            if self.state_bits == 8 and (
+                    not torch.ops.aten.is_non_overlapping_and_dense(
+                        saved[name]) or
+                    saved[scale].shape != (-(-p.numel() // BLOCK8),)):
+                raise ValueError(f"AdamW: saved codes of {name} without "
+                                 "their scales")
+
     def load_state_dict(self, state_dict):
         """Loads another AdamW's state of the same state_bits. (The base
-        class would cast the states to their parameter's type.)"""
+        class would cast the states to their parameter's type.) A state that
+        does not fit raises ValueError and changes nothing."""
         want = torch.float32 if self.state_bits == 32 else torch.uint8
-        for state in state_dict["state"].values():
-            if "exp_avg" not in state or state["exp_avg"].dtype != want:
-                raise ValueError(f"AdamW: not states of {self.state_bits} "
-                                 "bits")
-        super().load_state_dict(state_dict)
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         params = [p for g in self.param_groups for p in g["params"]]
+        if len(ids) != len(params):
+            raise ValueError(f"AdamW: a state of {len(ids)} parameters for "
+                             f"{len(params)}")
+        for i, p in zip(ids, params):
+            if i in state_dict["state"]:
+                self._check_saved(p, state_dict["state"][i])
+        super().load_state_dict(state_dict)
         for i, p in zip(ids, params):
             if i not in state_dict["state"]:
                 continue

@@ -363,3 +363,52 @@ def test_8_bit_states_follow_over_many_steps(device, beta2, then, normal):
     # 1.33 times that of none, m's own rounding adds a fifth to its square.
     if then:
         assert 0.95 <= (moved[1] / moved[0]) ** 0.5 <= 1.35
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_refused_state_changes_nothing(device, bits):
+    """States of other shapes, one that would broadcast among them, scales
+    that are missing or too few, and a state of fewer parameters."""
+    def fresh():
+        torch.manual_seed(0)
+        ps = [nn.Parameter(torch.randn(n, device=device)) for n in (300, 91)]
+        opt = AdamW(ps, lr=1e-2, state_bits=bits)
+        for p in ps:
+            p.grad = torch.ones_like(p)
+        opt.step()
+        return ps, opt
+
+    def saved(**more):
+        state = copy.deepcopy(fresh()[1].state_dict())
+        state["param_groups"][0]["lr"] = 5.0
+        state["state"][1].update(more)
+        return state
+    dtype = torch.float32 if bits == 32 else torch.uint8
+    bad = [saved(**{name: torch.ones(n, dtype=dtype)})
+           for name in ("exp_avg", "exp_avg_sq") for n in (1, 81, (91, 1))]
+    bad.append(saved(exp_avg_sq=torch.ones(91, dtype=torch.bfloat16)))
+    if bits == 8:
+        bad += [saved(exp_avg_scale=torch.ones(2, dtype=dtype)),
+                saved(exp_avg_sq_scale=torch.ones(1)),
+                saved(exp_avg=torch.ones(182, dtype=dtype)[::2])]
+    for name in ("step", "exp_avg_sq") + (("exp_avg_scale",) * (bits == 8)):
+        bad.append(saved())
+        del bad[-1]["state"][1][name]
+    bad.append(saved())
+    bad[-1]["param_groups"][0]["params"] = [0]
+    want, same = fresh()
+    same.step()
+    for state in bad:
+        ps, opt = fresh()
+        with pytest.raises(ValueError):
+            opt.load_state_dict(state)
+        opt.step()
+        assert all(torch.equal(p, q) for p, q in zip(ps, want))
+        for p, q in zip(ps, want):
+            assert all(torch.equal(torch.as_tensor(v),
+                                   torch.as_tensor(same.state[q][k]))
+                       for k, v in opt.state[p].items())
+    ps, opt = fresh()
+    opt.load_state_dict(saved())
+    opt.step()
