@@ -19,8 +19,8 @@
 // Measured on one MI355X, where a copy reaches 4.9 to 5.4 TB/s: bf16
 // 131072x256 forward 24 us (134 MB, 5.6 TB/s), backward 32 + 4 us for the
 // partial sums' sum (201 MB); fp32 1000x12544 forward 20 us (100 MB, 5.0
-// TB/s). Rows above 16 packets of 2048 lanes go to the wide kernels, which
-// read x three times (mostly from the caches).
+// TB/s). Rows above 16384 values (2048 packets in 16 bits, 4096 in fp32) go to
+// the wide kernels, which read x three times (mostly from the caches).
 #include <hip/hip_runtime.h>
 
 #include "train_ops.h"
@@ -436,20 +436,26 @@ __global__ __launch_bounds__(1024) void sum_rows_kernel(
 
 namespace {
 
+// f(first row, rows) for as many rows at a time as a launch takes, which has
+// less than 2^32 threads.
+template <typename F>
+void each_launch(long all, int threads, int per, F f) {
+  const long most = (1L << 31) / threads * per;
+  for (long at = 0; at < all; at += most)
+    f(at, all - at < most ? all - at : most);
+}
+
 template <typename T, typename W, int kTeam, int kVecs, bool kRagged>
 void run_team(const NormArgs& a, bool backward, hipStream_t s) {
   constexpr int threads = threads_of<kTeam>(), per = threads / kTeam;
   if (!backward) {
-    // A launch has less than 2^32 threads.
-    constexpr long most = (1L << 31) / threads * per;
-    for (long at = 0; at < a.rows; at += most) {
-      const long rows = a.rows - at < most ? a.rows - at : most;
+    each_launch(a.rows, threads, per, [&](long at, long rows) {
       const unsigned grid = (unsigned)((rows + per - 1) / per);
       norm_fwd_kernel<T, W, kTeam, kVecs, kRagged><<<grid, threads, 0, s>>>(
           (const T*)a.x + at * a.x_stride, (const W*)a.w, (const W*)a.b,
           (T*)a.y + at * a.width, a.mean ? a.mean + at : nullptr,
           a.rstd ? a.rstd + at : nullptr, rows, a.width, a.x_stride, a.eps);
-    }
+    });
   } else {
     norm_bwd_kernel<T, W, kTeam, kVecs, kRagged><<<a.parts, threads, 0, s>>>(
         (const T*)a.dy, (const T*)a.x, (const W*)a.w, a.mean, a.rstd,
@@ -497,15 +503,21 @@ void run_types(const NormArgs& a, bool backward, hipStream_t s) {
                               : run_width<T, W, false>(a, backward, s))
     return;
   if (!backward) {
-    norm_fwd_wide_kernel<T, W><<<(unsigned)a.rows, kWide, 0, s>>>(
-        (const T*)a.x, (const W*)a.w, (const W*)a.b, (T*)a.y, a.mean, a.rstd,
-        a.width, a.x_stride, a.eps);
+    each_launch(a.rows, kWide, 1, [&](long at, long rows) {
+      norm_fwd_wide_kernel<T, W><<<(unsigned)rows, kWide, 0, s>>>(
+          (const T*)a.x + at * a.x_stride, (const W*)a.w, (const W*)a.b,
+          (T*)a.y + at * a.width, a.mean ? a.mean + at : nullptr,
+          a.rstd ? a.rstd + at : nullptr, a.width, a.x_stride, a.eps);
+    });
     return;
   }
   if (a.dx != nullptr)
-    norm_dx_wide_kernel<T, W><<<(unsigned)a.rows, kWide, 0, s>>>(
-        (const T*)a.dy, (const T*)a.x, (const W*)a.w, a.mean, a.rstd,
-        (T*)a.dx, a.width, a.dy_stride, a.x_stride);
+    each_launch(a.rows, kWide, 1, [&](long at, long rows) {
+      norm_dx_wide_kernel<T, W><<<(unsigned)rows, kWide, 0, s>>>(
+          (const T*)a.dy + at * a.dy_stride, (const T*)a.x + at * a.x_stride,
+          (const W*)a.w, a.mean + at, a.rstd + at, (T*)a.dx + at * a.width,
+          a.width, a.dy_stride, a.x_stride);
+    });
   if (a.part != nullptr)
     norm_dw_wide_kernel<T>
         <<<dim3((a.width + 256 * width_of<T>() - 1) / (256 * width_of<T>()),

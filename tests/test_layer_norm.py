@@ -390,3 +390,40 @@ def test_forward_mode_is_refused(device, grad):
             with pytest.raises(NotImplementedError):
                 layer_norm(*given)
     assert layer_norm(*args).isfinite().all()
+
+
+@pytest.mark.gpu
+def test_more_wide_rows_than_one_launch_has():
+    """Rows of 1024 threads each: 2^22 of them are 2^32."""
+    rows, width = (1 << 22) + 3, 16400
+    row = torch.zeros(width, dtype=torch.bfloat16, device="cuda")
+    row[::5] = 4.0
+    want = layer_norm(row)
+    y = layer_norm(row.expand(rows, width))
+    for part in (slice(0, 3), slice((1 << 21) - 2, (1 << 21) + 2),
+                 slice(rows - 5, rows)):
+        assert torch.equal(y[part], want.expand_as(y[part]))
+    del y
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
+def test_gradient_of_many_wide_rows():
+    """The backward's launch splits by rows as the forward's does: rows on
+    either side of the border, in a view of the same memory."""
+    rows, width = (1 << 21) + 2, 16400
+    row = torch.zeros(width, dtype=torch.bfloat16, device="cuda")
+    row[::5] = 4.0
+    dy = torch.zeros_like(row)
+    dy[7] = 1.0
+
+    def grad(x, d):
+        x = x.detach().requires_grad_()
+        y = layer_norm(x)
+        return torch.autograd.grad(y, x, d)[0]
+    want = grad(row[None], dy[None])
+    got = grad(row.expand(rows, width), dy.expand(rows, width))
+    for part in (slice(0, 3), slice(rows - 5, rows)):
+        assert torch.equal(got[part], want.expand_as(got[part]))
+    del got
+    torch.cuda.empty_cache()
