@@ -833,7 +833,7 @@ hipError_t run_pad(const void* from, void* to, int rows, int width,
 // counted in CUs. For bf16 1000x12544x1024 it takes 4 splits of 128-wide
 // tiles: 37 us, against 44 with 256-wide tiles in 12 splits and 43 with 3;
 // for 32000 rows 256-wide ones unsplit: 617 us, against 845 with 128.
-extern "C" void linear_plan(LinearProduct* a, int type) {
+extern "C" bool linear_plan(LinearProduct* a, int type) {
   struct Shape { int tile; double step, alone, rest; };
   static const Shape kHalf[] = {{256, 1.55, 1.55, 6.0},
                                 {128, 0.55, 0.48, 2.5},
@@ -847,6 +847,8 @@ extern "C" void linear_plan(LinearProduct* a, int type) {
   for (int i = 0; i < count; ++i) {
     const int t = shapes[i].tile;
     const long tiles = (long)((a->m + t - 1) / t) * ((a->n + t - 1) / t);
+    // A launch has less than 2^32 threads, of 256 or 512 a tile (run_tiles).
+    if (tiles >= 1L << (t == 64 ? 24 : 23)) continue;
     for (int s = 1; s <= 32 && (s == 1 || (s * 2 <= steps && tiles * s <= 2048));
          ++s) {
       const int each = (steps + s - 1) / s;
@@ -863,10 +865,12 @@ extern "C" void linear_plan(LinearProduct* a, int type) {
       }
     }
   }
+  if (best == 0.0) return false;
   // Four rows of tiles by all columns at a time share more of both operands
   // in an L2 than one row does, once a row is longer than that.
   a->group = (a->n + a->tile - 1) / a->tile > 4 ? 4 : 1;
   a->ld_part = (a->n + kOut - 1) / kOut * kOut;
+  return true;
 }
 
 extern "C" hipError_t linear_product_launch(const LinearProduct* a, int type,

@@ -82,7 +82,7 @@ struct LinearDz {
 };
 
 extern "C" {
-void linear_plan(LinearProduct*, int type);
+bool linear_plan(LinearProduct*, int type);   // false: too large a launch
 hipError_t linear_product_launch(const LinearProduct*, int type, hipStream_t);
 int linear_dz_strips(int m, int n);
 hipError_t linear_dz_launch(const LinearDz*, int type, hipStream_t);

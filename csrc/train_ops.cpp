@@ -212,7 +212,8 @@ void product(LinearProduct& a, int type, const Tensor& like,
   const int64_t row = std::max(a.ldx, a.ldy) * like.element_size();
   TORCH_CHECK(near(row), "linear_act: rows of ", row,
               " bytes are too far apart");
-  linear_plan(&a, type);
+  TORCH_CHECK(linear_plan(&a, type), "linear_act: a product of ", a.m, " x ",
+              a.n, " values is too large for a launch");
   Tensor part;
   if (a.splits > 1) {
     part = torch::empty({a.splits, a.m, a.ld_part},

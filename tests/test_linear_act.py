@@ -496,3 +496,26 @@ def test_forward_mode_is_refused(device, grad):
             with pytest.raises(NotImplementedError):
                 linear_act(x, w, b, "gelu", r)
     assert linear_act(*args[:3]).isfinite().all()
+
+
+@pytest.mark.gpu
+def test_as_many_rows_as_are_taken():
+    """2^30 rows: 64-wide tiles would be 2^32 threads, which no launch has.
+    In fp32 the larger tile's would be as many, and the call is refused."""
+    m = 1 << 30
+    x = torch.ones(m, 1, dtype=torch.bfloat16, device="cuda")
+    x[::1000] = 3.0
+    w = torch.full((1, 1), 2.0, dtype=torch.bfloat16, device="cuda")
+    y = linear_act(x, w)
+    for part in (slice(0, 5000), slice(m // 2 - 2500, m // 2 + 2500),
+                 slice(m - 5000, m)):
+        assert torch.equal(y[part], 2 * x[part])
+    assert int((y > 2).sum()) == -(-m // 1000)
+    del x, y
+    x = torch.ones(m, 1, device="cuda")
+    with pytest.raises(RuntimeError, match="too large"):
+        linear_act(x, w.float())
+    y = linear_act(x[:m - 64], w.float())
+    assert bool((y[-1000:] == 2).all()) and float(y.min()) == 2
+    del x, y
+    torch.cuda.empty_cache()
