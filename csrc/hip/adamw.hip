@@ -637,11 +637,16 @@ extern "C" hipError_t norm_launch(const double* partial, int count, float* out,
 extern "C" hipError_t pack8_launch(const float* x, unsigned char* codes,
                                    unsigned char* scales, long n,
                                    bool is_signed, hipStream_t stream) {
-  const unsigned wg = (unsigned)((n + kPass - 1) / kPass);
-  if (is_signed)
-    pack8_kernel<true><<<wg, kThreads, 0, stream>>>(x, codes, scales, n);
-  else
-    pack8_kernel<false><<<wg, kThreads, 0, stream>>>(x, codes, scales, n);
+  constexpr long most = 1L << 33;     // a launch has less than 2^32 threads
+  for (; n > 0; n -= most, x += most, codes += most,
+                scales += most / kBlock8) {
+    const long some = n < most ? n : most;
+    const unsigned wg = (unsigned)((some + kPass - 1) / kPass);
+    if (is_signed)
+      pack8_kernel<true><<<wg, kThreads, 0, stream>>>(x, codes, scales, some);
+    else
+      pack8_kernel<false><<<wg, kThreads, 0, stream>>>(x, codes, scales, some);
+  }
   return hipGetLastError();
 }
 

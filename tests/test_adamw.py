@@ -712,3 +712,21 @@ def test_seeded_places_past_32_bits():
         assert len(first.unique()) == 2 and len(last.unique()) == 2
         assert not torch.equal(first, last)
     assert (p[-600:] == p[0]).all() and p[0] < 0
+
+
+@pytest.mark.gpu
+def test_pack_more_than_one_launch_has():
+    n = (1 << 34) + 300
+    x = torch.zeros(n, device="cuda")
+    at = torch.tensor([0, (1 << 33) - 1, 1 << 33, (1 << 34) + 1, n - 1],
+                      device="cuda")
+    x[at] = torch.tensor([1.0, 2.0, 3.0, 4.0, 5.0], device="cuda")
+    codes, scales = pack_state8(x, True)
+    assert int(codes.count_nonzero()) == 5
+    for i, want in zip(at.tolist(), (1.0, 2.0, 3.0, 4.0, 5.0)):
+        part = slice(i // BLOCK * BLOCK, min(i // BLOCK * BLOCK + BLOCK, n))
+        got = unpack_state8(codes[part], scales[i // BLOCK:i // BLOCK + 1],
+                            True)
+        assert float(got[i % BLOCK]) == want
+    del x, codes, scales
+    torch.cuda.empty_cache()
