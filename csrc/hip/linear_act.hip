@@ -254,14 +254,22 @@ struct Operand {
 // ---------------------------------------------------------------- epilogue
 
 // The normal distribution at z: its density's exponential and its integral.
-// fp32 tensors take erf; for 16-bit ones the integral is Abramowitz and
-// Stegun's 7.1.26, off by 7.5e-8 at most and a fifth of erf's instructions,
-// which took 10 us of a 25 us forward of 3999x1024x1024.
+// fp32 tensors take erfc, whose small values below 0 do not cancel as 1 + erf
+// does; for 16-bit ones the integral is Abramowitz and Stegun's 7.1.26, off by
+// 7.5e-8 at most and a fifth of erf's instructions, which took 10 us of a 25 us
+// forward of 3999x1024x1024. The exponential's instruction, and below the
+// reciprocal's, are for 16 bits likewise: with the factor's rounding they are
+// off by 0.5 |z| units in fp32's last place, 40 at the far end of SiLU.
+template <typename T>
+__device__ inline float exponential(float x) {
+  return sizeof(T) == 4 ? expf(x) : __expf(x);
+}
+
 template <typename T>
 __device__ inline void normal(float z, float& e, float& cdf) {
-  e = __expf(-0.5f * z * z);
+  e = exponential<T>(-0.5f * z * z);
   if constexpr (sizeof(T) == 4) {
-    cdf = 0.5f * (1.0f + erff(z * 0.70710678f));
+    cdf = 0.5f * erfcf(z * -0.70710678f);
   } else {
     const float t =
         __builtin_amdgcn_rcpf(1.0f + 0.3275911f * 0.70710678f * fabsf(z));
@@ -274,8 +282,10 @@ __device__ inline void normal(float z, float& e, float& cdf) {
   }
 }
 
+template <typename T>
 __device__ inline float sigmoid(float z) {
-  return __builtin_amdgcn_rcpf(1.0f + __expf(-z));
+  const float d = 1.0f + exponential<T>(-z);
+  return sizeof(T) == 4 ? 1.0f / d : __builtin_amdgcn_rcpf(d);
 }
 
 // act(z); slope: act'(z), of the same exponential.
@@ -286,7 +296,7 @@ __device__ inline float activate(float z, float& slope) {
     return z < 0.0f ? 0.0f : z;                             // NaN stays
   }
   if constexpr (kAct == kActSilu) {
-    const float s = sigmoid(z);
+    const float s = sigmoid<T>(z);
     slope = s * (1.0f + z * (1.0f - s));
     return z * s;
   }

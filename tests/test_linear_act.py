@@ -519,3 +519,33 @@ def test_as_many_rows_as_are_taken():
     assert bool((y[-1000:] == 2).all()) and float(y.min()) == 2
     del x, y
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("act,lowest", [("gelu", -8.0), ("silu", -80.0)])
+def test_fp32_functions(device, act, lowest):
+    """Values and derivatives in fp32 with one weight of 1, relative to
+    themselves: 16 units for the exponential (2), erfc (8), quotients, sums
+    and products, and z^2 more where the exponents' arguments z^2 / 2 and
+    (z / sqrt 2)^2 are rounded, twice each. Near the derivative's zero, within
+    the terms that cancel there. (64-bit erfc: ndtr's small values cancel, to
+    1e-17 where they are 6e-16.)"""
+    z = torch.linspace(lowest, 8.0, 4097).double()
+    z = z.float().double()
+    x = z.to(device, torch.float32)[:, None].requires_grad_()
+    y = linear_act(x, torch.ones(1, 1, device=device), None, act)
+    dx, = torch.autograd.grad(y, x, torch.ones_like(y))
+    s = torch.sigmoid(z)
+    if act == "gelu":
+        s = 0.5 * torch.erfc(z * -math.sqrt(0.5))
+        more = z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    else:
+        more = s * z * (1 - s)
+    want, slope = z * s, s + more
+    rel = (16 + (2 * z * z if act == "gelu" else 0)) * U
+    tiny = torch.finfo(torch.float32).smallest_normal
+    off = (y[:, 0].detach().double().cpu() - want).abs()
+    assert (off <= rel * want.abs() + tiny).all(), z[off > rel * want.abs()]
+    terms = torch.where(z > -3, s + more.abs(), slope.abs())
+    off = (dx[:, 0].double().cpu() - slope).abs()
+    assert (off <= rel * terms + tiny).all(), z[off > rel * terms]
