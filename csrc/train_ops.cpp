@@ -588,7 +588,8 @@ void adamw_step(const Tensors& p, const Tensors& g, const Tensors& m,
               "would stay the same in every replay of a captured graph");
 
   Ranges ranges;
-  ranges.all.reserve(count * (ms ? 6 : 4));
+  ranges.all.reserve(count * (ms ? 6 : 4) + 1);
+  if (norm) ranges.add(*norm, false);
   Tensors copies;               // gradients laid out like their parameter
   std::vector<const void*> grads(count);
   for (size_t i = 0; i < count; ++i) {

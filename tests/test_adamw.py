@@ -730,3 +730,19 @@ def test_pack_more_than_one_launch_has():
         assert float(got[i % BLOCK]) == want
     del x, codes, scales
     torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
+def test_norm_in_a_tensor_to_write_is_refused():
+    """Workgroups read it at any time, before and after it would change."""
+    p, g, m, v = tensors([300, 8], torch.float32, "cuda")
+    before = [t.clone() for k in (p, m, v) for t in k]
+    for t in (p[0], m[1], v[0]):
+        with pytest.raises(RuntimeError, match="shares memory"):
+            adamw_step(p, g, m, v, grad_norm=t[3].abs_(), max_grad_norm=1.0,
+                       **HYPER)
+    for a, b in zip((t for k in (p, m, v) for t in k), before):
+        assert torch.equal(a.abs(), b.abs())
+    # A gradient is only read.
+    g[0][0] = 2.0
+    adamw_step(p, g, m, v, grad_norm=g[0][0], max_grad_norm=1.0, **HYPER)
