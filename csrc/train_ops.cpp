@@ -703,8 +703,7 @@ void adamw_step(const Tensors& p, const Tensors& g, const Tensors& m,
   }
 }
 
-Tensor grad_norm(const Tensors& g) {
-  TORCH_CHECK(!g.empty(), "grad_norm: no tensors");
+Tensor norm_of(const Tensors& g) {
   const auto device = g[0].device();
   TORCH_CHECK(device.is_cuda(), "grad_norm: tensors must be on GPU");
   const c10::DeviceGuard guard(device);
@@ -745,6 +744,40 @@ Tensor grad_norm(const Tensors& g) {
                        (int)parts, out.data_ptr<float>(), current()),
            "grad_norm");
   return out;
+}
+
+// d |g| / d g = g / |g|, for a norm that is a part of a loss.
+class GradNormNode : public torch::autograd::Function<GradNormNode> {
+ public:
+  static Tensor forward(torch::autograd::AutogradContext* ctx,
+                        at::TensorList g) {
+    Tensors saved = g.vec();
+    saved.push_back(norm_of(saved));
+    ctx->save_for_backward(saved);
+    return saved.back();
+  }
+
+  static torch::autograd::variable_list backward(
+      torch::autograd::AutogradContext* ctx,
+      torch::autograd::variable_list grads) {
+    auto saved = ctx->get_saved_variables();
+    const Tensor scale = grads[0] / saved.back();
+    saved.pop_back();
+    for (Tensor& t : saved)
+      t = (t.to(torch::kFloat) * scale).to(t.scalar_type());
+    return saved;
+  }
+};
+
+Tensor grad_norm(const Tensors& g) {
+  TORCH_CHECK(!g.empty(), "grad_norm: no tensors");
+  bool wanted = false;
+  for (const Tensor& t : g) {
+    refuse_forward_mode({&t}, "grad_norm");
+    wanted |= t.requires_grad();
+  }
+  return wanted && at::GradMode::is_enabled()
+             ? GradNormNode::apply(at::TensorList(g)) : norm_of(g);
 }
 
 std::tuple<Tensor, Tensor> pack_state8(const Tensor& x, bool is_signed) {

@@ -164,7 +164,7 @@ def unpack_state8(codes: torch.Tensor, scales: torch.Tensor, signed: bool,
 
 def grad_norm(tensors) -> torch.Tensor:
     """2-norm over all values of a list of tensors, as one fp32 value on
-    their device. Squares are summed in 64 bits."""
+    their device. Squares are summed in 64 bits. Differentiable."""
     tensors = list(tensors)
     if not tensors:
         raise RuntimeError("grad_norm: no tensors")

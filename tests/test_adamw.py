@@ -746,3 +746,39 @@ def test_norm_in_a_tensor_to_write_is_refused():
     # A gradient is only read.
     g[0][0] = 2.0
     adamw_step(p, g, m, v, grad_norm=g[0][0], max_grad_norm=1.0, **HYPER)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_norm_has_a_gradient(device):
+    """t / |g| for each tensor: three roundings, one of them to its type. And
+    a gradient of it, and none where none is wanted."""
+    g = torch.Generator().manual_seed(2)
+    t = [torch.randn(n, generator=g).to(device, d)
+         for n, d in ((5, torch.float32), (300, torch.bfloat16),
+                      (0, torch.float32), (7, torch.float16))]
+    assert not grad_norm(t).requires_grad
+    for x in t[1:]:
+        x.requires_grad_()
+    with torch.no_grad():
+        assert not grad_norm(t).requires_grad
+    norm = grad_norm(t)
+    got = torch.autograd.grad(norm * 3.0, t[1:], retain_graph=True)
+    n = float(norm.detach())
+    for x, d in zip(t[1:], got):
+        want = 3.0 * x.detach().double() / n
+        half = torch.finfo(x.dtype).eps / 2
+        assert d.dtype == x.dtype and d.shape == x.shape
+        assert ((d.double() - want).abs() <= (half * 1.01 + 4 * U) *
+                want.abs() + torch.finfo(x.dtype).smallest_normal).all()
+    x = torch.tensor([3.0, 4.0], device=device, requires_grad=True)
+    d, = torch.autograd.grad(grad_norm([x]), x, create_graph=True)
+    dd, = torch.autograd.grad(d[0], x)
+    # d/dx of x0 / |x| is (1 - x0^2 / n^2) / n and -x0 x1 / n^3.
+    want = torch.tensor([0.128, -0.096], device=device)
+    assert ((dd - want).abs() <= 16 * U).all()
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x.detach(),
+                                                   torch.ones_like(x))
+        if device == "cuda":
+            with pytest.raises(NotImplementedError):
+                grad_norm([dual])
