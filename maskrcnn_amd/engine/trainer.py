@@ -24,6 +24,12 @@ from ..data.loader import make_data_loader
 log = logging.getLogger(__name__)
 
 
+def optimizer_kind(config):
+    """config.OPTIMIZER; SGD where a configuration of a caller's own class
+    has none."""
+    return getattr(config, "OPTIMIZER", "sgd")
+
+
 def build_optimizer(model, config, learning_rate):
     """config.OPTIMIZER: SGD + momentum, or AdamW with states in 32 or 8
     bits, which clips the gradients' norm itself. Weight decay is applied
@@ -54,16 +60,16 @@ def build_optimizer(model, config, learning_rate):
             decay.append(p)
     groups = [{"params": decay, "weight_decay": config.WEIGHT_DECAY},
               {"params": no_decay, "weight_decay": 0.0}]
-    if config.OPTIMIZER == "sgd":
+    kind = optimizer_kind(config)
+    if kind == "sgd":
         return torch.optim.SGD(groups, lr=learning_rate,
                                momentum=config.LEARNING_MOMENTUM)
-    if config.OPTIMIZER not in ("adamw", "adamw8"):
-        raise ValueError(f"OPTIMIZER {config.OPTIMIZER!r}: sgd, adamw or "
-                         "adamw8")
+    if kind not in ("adamw", "adamw8"):
+        raise ValueError(f"OPTIMIZER {kind!r}: sgd, adamw or adamw8")
     from .optim import AdamW
     return AdamW(groups, lr=learning_rate, betas=config.ADAMW_BETAS,
                  eps=config.ADAMW_EPS,
-                 state_bits=8 if config.OPTIMIZER == "adamw8" else 32,
+                 state_bits=8 if kind == "adamw8" else 32,
                  max_grad_norm=config.GRADIENT_CLIP_NORM)
 
 
@@ -267,7 +273,7 @@ class Trainer:
                 # saved weights only; SGD momentum + epoch make resume
                 # exact). Latest-only: overwritten each epoch.
                 torch.save({"optimizer": optimizer.state_dict(),
-                            "kind": cfg.OPTIMIZER, "epoch": epoch},
+                            "kind": optimizer_kind(cfg), "epoch": epoch},
                            os.path.join(self.wrapper.log_dir,
                                         "train_state.pth"))
             self.wrapper.epoch += 1
@@ -291,10 +297,11 @@ class Trainer:
                             "at %d: skipping optimizer restore",
                             state.get("epoch"), self.wrapper.epoch)
                 return False
-            if state.get("kind", "sgd") != self.config.OPTIMIZER:
+            kind = optimizer_kind(self.config)
+            if state.get("kind", "sgd") != kind:
                 log.warning("train_state.pth is of optimizer %s, not %s: "
                             "skipping optimizer restore",
-                            state.get("kind", "sgd"), self.config.OPTIMIZER)
+                            state.get("kind", "sgd"), kind)
                 return False
             optimizer.load_state_dict(state["optimizer"])
             log.info("restored optimizer state from %s", path)

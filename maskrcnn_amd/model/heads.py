@@ -35,7 +35,7 @@ class FPNClassifierHead(nn.Module):
         self.roi_align = PyramidROIAlign(pool, config.IMAGE_SHAPE,
                                          mode="crop_and_resize")
         # 7x7 conv with VALID padding == fully-connected over the pooled tile.
-        norm = config.CLASSIF_HEAD_NORM
+        norm = getattr(config, "CLASSIF_HEAD_NORM", "batch")
         if norm not in ("batch", "layer"):
             raise ValueError(f"CLASSIF_HEAD_NORM {norm!r}: batch or layer")
         self.layer_norm = norm == "layer"

@@ -119,7 +119,8 @@ def assign_keras_arrays(model, arrays: Dict[str, np.ndarray],
     import torch
 
     wmap = keras_weight_map(model.config.BACKBONE,
-                            model.config.CLASSIF_HEAD_NORM)
+                            getattr(model.config, "CLASSIF_HEAD_NORM",
+                                    "batch"))
     state = model.state_dict()
     exclude = set(exclude or [])
     loaded, unexpected = [], []

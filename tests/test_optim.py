@@ -412,3 +412,15 @@ def test_a_refused_state_changes_nothing(device, bits):
     ps, opt = fresh()
     opt.load_state_dict(saved())
     opt.step()
+
+
+def test_configurations_without_the_new_fields(shapes_config):
+    """A class of the caller's own: the batch-normed head and SGD."""
+    class Old:
+        POOL_SIZE, FPN_CLASSIF_FC_LAYERS_SIZE, NUM_CLASSES = 7, 64, 5
+        TRAIN_BN, IMAGE_SHAPE = False, [128, 128, 3]
+        WEIGHT_DECAY, LEARNING_MOMENTUM = 1e-4, 0.9
+    head = FPNClassifierHead(Old(), in_channels=16)
+    assert not head.layer_norm and hasattr(head, "mrcnn_class_bn1")
+    opt = build_optimizer(head, Old(), 1e-3)
+    assert isinstance(opt, torch.optim.SGD)
