@@ -244,7 +244,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *,
             params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales,
             exp_avg_sq_scales, grad_norm, max_grad_norm, step, lr, beta1,
             beta2, eps, weight_decay,
-            None if seed is None else seed & (1 << 64) - 1)
+            None if seed is None else int(seed) & (1 << 64) - 1)
         return
     eight = exp_avg_scales is not None
     if eight != (exp_avg_sq_scales is not None) or not (
@@ -257,7 +257,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *,
         clip = (torch.full_like(grad_norm, max_grad_norm) /
                 (grad_norm + 1e-6)).clamp(max=1.0)
     random = eight and seed is not None
-    keys = _keys(seed, int(step), len(params)) if random else None
+    keys = _keys(int(seed), int(step), len(params)) if random else None
     scalars = (clip, beta1, beta2, eps, 1.0 - lr * weight_decay,
                lr / (1.0 - beta1 ** step),
                1.0 / math.sqrt(1.0 - beta2 ** step),

@@ -2,6 +2,7 @@
 
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -619,6 +620,7 @@ def test_seeded_calls_repeat(device):
         return a[2] + a[3]
     one = step(5)
     assert all(torch.equal(a, b) for a, b in zip(one, step(5)))
+    assert all(torch.equal(a, b) for a, b in zip(one, step(np.int64(5))))
     # Other seeds, steps and tensors have bits of their own.
     for other in (step(6), step(5 + (1 << 40)), step(-5), step(5, step=8)):
         assert not torch.equal(one[0], other[0])
