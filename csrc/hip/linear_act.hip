@@ -7,12 +7,19 @@
 // What is kept for the backward: act'(z), formed where z is still in fp32, so
 // that no erf or exp is computed twice. With 16-bit tensors it has 16 bits too:
 // from 2^-7 on (2^-6 for fp16) steps of 2^-15, where bf16's or fp16's own
-// rounding would cost as much again as dz's (the matrix cores take dz in the
-// tensors' type; db sums it unrounded), and below that 8 (9) bits of mantissa
-// down to 2^-52 (2^-28): fixed point alone would lose the small derivatives of
-// GELU below -4 and SiLU below -9 in part, and below -4.84 and -13.6 in whole.
-// A kept one is off by 2^-16 at most, and below those borders by 2^-9 (2^-10) of
+// rounding would show in dx and dW, and below that 8 (9) bits of mantissa down
+// to 2^-52 (2^-28): fixed point alone would lose the small derivatives of GELU
+// below -4 and SiLU below -9 in part, and below -4.84 and -13.6 in whole. A
+// kept one is off by 2^-16 at most, and below those borders by 2^-9 (2^-10) of
 // itself, half of bf16's own rounding. ReLU's 0 and 1 are exact.
+//
+// dz of 16-bit tensors has more bits than they do, where act'(z) is no 0 or 1.
+// The matrix cores take it as two numbers, the nearest one and what that has
+// lost (db sums it as it is): with one alone dx and dW were off by sqrt(2) of
+// their own rounding, and by 2 to 3 times that where their terms cancel. Each
+// step of k is then two, one for either part, the other operand the same, which
+// comes from the L2: 1024x1024 from 3999 in fp16 29 us in place of 17 (dW) and
+// 22 of 15 (dx), 8192x4096x4096 bf16 with all gradients 1060 in place of 668.
 //
 // All three products are one kernel, D[m][n] = sum_k X(m,k) Y(n,k), where
 // either operand may lie with k consecutive or with its own index
@@ -149,6 +156,7 @@ struct Operand {
   static constexpr int kUnits = kPackets / kUnit;
 
   const char* base;     // at the tile's first row, k = 0
+  long second;          // from there to the second part
   int ld;               // bytes
   int rows;             // of this tile
   int k;                // k altogether
@@ -171,7 +179,8 @@ struct Operand {
   }
 
   __device__ void init(const void* p, long ld_values, int first, int total,
-                       int k_total, int wave, int lane) {
+                       int k_total, int wave, int lane, long to_second) {
+    second = to_second;
     ld = (int)(ld_values * (long)sizeof(T));
     k = k_total;
     rows = total - first < kR ? total - first : kR;
@@ -198,14 +207,18 @@ struct Operand {
   };
 
   // Step `step`'s part of the operand; from `end` on nothing is in range.
+  // kTwo: steps go in pairs of the same k, the odd ones in the second part.
+  template <bool kTwo>
   __device__ Step at_step(int step, int end) const {
-    const int k0 = step * kK, left = step < end ? k - k0 : 0;
+    const int at = kTwo ? step >> 1 : step;
+    const int k0 = at * kK, left = step < end ? k - k0 : 0;
+    const char* part = kTwo && step & 1 ? base + second : base;
     if constexpr (!kTrans)
-      return {descriptor(base + (long)step * kRow,
+      return {descriptor(part + (long)at * kRow,
                          step_range(rows, ld, left / kPer)),
               left / kPer};
     const int rows_k = left < kK ? left : kK;
-    return {descriptor(base + (long)k0 * ld,
+    return {descriptor(part + (long)k0 * ld,
                        rows_k > 0 ? (rows_k - 1) * ld + rows * (int)sizeof(T)
                                   : 0),
             0};
@@ -458,8 +471,8 @@ __device__ inline void with_act(int act, F f) {
 // steps, with buffers of their own. Two waves a SIMD have 256 registers each,
 // which holds the sums in ordinary ones: with more, the compiler moves
 // hundreds of sums between the two kinds in each step.
-template <typename T, bool kXT, bool kYT, int kBM, int kBN, int kWM, int kWN,
-          int kGroups, int kAhead>
+template <typename T, bool kXT, bool kYT, bool kTwo, int kBM, int kBN, int kWM,
+          int kWN, int kGroups, int kAhead>
 __global__ __launch_bounds__(kWM * kWN * kGroups * 64, 2) void product_kernel(
     LinearProduct a) {
   constexpr int kWaves = kWM * kWN;
@@ -490,10 +503,10 @@ __global__ __launch_bounds__(kWM * kWN * kGroups * 64, 2) void product_kernel(
   const int xr = wave / kWN * (kBM / kWM), yr = wave % kWN * (kBN / kWN);
   X x;
   Y y;
-  x.init(a.x, a.ldx, m0, a.ext_x, a.kx, wave, lane);
-  y.init(a.y, a.ldy, n0, a.ext_y, a.ky, wave, lane);
+  x.init(a.x, a.ldx, m0, a.ext_x, a.kx, wave, lane, a.second);
+  y.init(a.y, a.ldy, n0, a.ext_y, a.ky, wave, lane, 0);
 
-  const int steps = (a.kx + X::kK - 1) / X::kK;
+  const int steps = (a.kx + X::kK - 1) / X::kK * (kTwo ? 2 : 1);
   const int first_all = split * a.steps_per_split;
   const int last_all = first_all + a.steps_per_split < steps
                            ? first_all + a.steps_per_split : steps;
@@ -508,12 +521,12 @@ __global__ __launch_bounds__(kWM * kWN * kGroups * 64, 2) void product_kernel(
   f32x4 acc[kMI][kNI] = {};
   i32x4 xf[2][kMI], yf[2][kNI];
   const auto load_x = [&](int step, unsigned to) {
-    const auto s = x.at_step(step, last);
+    const auto s = x.template at_step<kTwo>(step, last);
 #pragma unroll
     for (int i = 0; i < X::kLoads; ++i) x.load(s, i, at_lds + to, wave);
   };
   const auto load_y = [&](int step, unsigned to) {
-    const auto s = y.at_step(step, last);
+    const auto s = y.template at_step<kTwo>(step, last);
 #pragma unroll
     for (int i = 0; i < Y::kLoads; ++i) y.load(s, i, at_lds + to, wave);
   };
@@ -548,7 +561,7 @@ __global__ __launch_bounds__(kWM * kWN * kGroups * 64, 2) void product_kernel(
   constexpr int kReads = (kMI + kNI + kMI - 1) / kMI < 2
                              ? 2 : (kMI + kNI + kMI - 1) / kMI;
   for (int s = first; s < first + turns; ++s) {
-    const auto xs = x.at_step(s + kAhead, last);
+    const auto xs = x.template at_step<kTwo>(s + kAhead, last);
 #pragma unroll
     for (int i = 0; i < kMI; ++i) {
 #pragma unroll
@@ -561,7 +574,7 @@ __global__ __launch_bounds__(kWM * kWN * kGroups * 64, 2) void product_kernel(
       __builtin_amdgcn_sched_barrier(0);
     }
     arrived<(kAhead - 1) * X::kLoads + (kAhead - 2) * Y::kLoads>();
-    const auto ys = y.at_step(s + kAhead, last);
+    const auto ys = y.template at_step<kTwo>(s + kAhead, last);
 #pragma unroll
     for (int i = 0; i < kMI; ++i) {
 #pragma unroll
@@ -709,8 +722,8 @@ __global__ __launch_bounds__(256) void join_kernel(LinearProduct a) {
 // loads are all in flight.
 template <typename T, bool kAct>
 __global__ __launch_bounds__(256) void dz_kernel(
-    const T* dy, const Kept<T>* slopes, T* dz, float* part, int m, int n,
-    long ld_dy, int ld_dz, int rows) {
+    const T* dy, const Kept<T>* slopes, T* dz, long second, float* part,
+    int m, int n, long ld_dy, int ld_dz, int rows) {
   constexpr int kDeep = 4;
   __shared__ float lds[8][256 + 8];
   const int c = blockIdx.x * 256 + (threadIdx.x & 31) * 8;
@@ -744,7 +757,16 @@ __global__ __launch_bounds__(256) void dz_kernel(
         sum[i] += g[d][i];
       }
       if (dz) {
-        store_some<T, 8>(dz + (long)row * ld_dz + c, ld_dz - c, g[d]);
+        T* out = dz + (long)row * ld_dz + c;
+        store_some<T, 8>(out, ld_dz - c, g[d]);
+        if (kAct && second) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float lost = g[d][i] - (float)(T)g[d][i];
+            g[d][i] = __builtin_isfinite(lost) ? lost : 0.0f;
+          }
+          store_some<T, 8>(out + second, ld_dz - c, g[d]);
+        }
       }
     }
   }
@@ -787,13 +809,14 @@ __global__ __launch_bounds__(256) void pad_kernel(const T* from, T* to,
   }
 }
 
-template <typename T, bool kXT, bool kYT>
+template <typename T, bool kXT, bool kYT, bool kTwo>
 void run_tiles(const LinearProduct& a, hipStream_t s) {
   const unsigned grid = (unsigned)(((a.m + a.tile - 1) / a.tile) *
                                    ((a.n + a.tile - 1) / a.tile) * a.splits);
   if constexpr (sizeof(T) == 2) {
     if (a.tile == 256) {
-      product_kernel<T, kXT, kYT, 256, 256, 2, 4, 1, 2><<<grid, 512, 0, s>>>(a);
+      product_kernel<T, kXT, kYT, kTwo, 256, 256, 2, 4, 1, 2>
+          <<<grid, 512, 0, s>>>(a);
       return;
     }
   }
@@ -804,20 +827,27 @@ void run_tiles(const LinearProduct& a, hipStream_t s) {
   // 53 -> 46, 1000x12544x1024 33 -> 31, few steps as before. Otherwise the
   // other workgroups' work covers its waits.
   if (a.tile == 128 && grid <= 256)
-    product_kernel<T, kXT, kYT, 128, 128, 2, 2, 2, 2><<<grid, 512, 0, s>>>(a);
+    product_kernel<T, kXT, kYT, kTwo, 128, 128, 2, 2, 2, 2>
+        <<<grid, 512, 0, s>>>(a);
   else if (a.tile == 128)
-    product_kernel<T, kXT, kYT, 128, 128, 2, 4, 1, 2><<<grid, 512, 0, s>>>(a);
+    product_kernel<T, kXT, kYT, kTwo, 128, 128, 2, 4, 1, 2>
+        <<<grid, 512, 0, s>>>(a);
   else if (grid <= 256)
-    product_kernel<T, kXT, kYT, 64, 64, 2, 2, 2, 4><<<grid, 512, 0, s>>>(a);
+    product_kernel<T, kXT, kYT, kTwo, 64, 64, 2, 2, 2, 4>
+        <<<grid, 512, 0, s>>>(a);
   else
-    product_kernel<T, kXT, kYT, 64, 64, 2, 2, 1, 2><<<grid, 256, 0, s>>>(a);
+    product_kernel<T, kXT, kYT, kTwo, 64, 64, 2, 2, 1, 2>
+        <<<grid, 256, 0, s>>>(a);
 }
 
 template <typename T>
 hipError_t run_product(const LinearProduct& a, hipStream_t s) {
-  if (a.x_trans) run_tiles<T, true, true>(a, s);
-  else if (a.y_trans) run_tiles<T, false, true>(a, s);
-  else run_tiles<T, false, false>(a, s);
+  constexpr bool parts = sizeof(T) == 2;     // fp32 has no second part
+  if (!a.y_trans) run_tiles<T, false, false, false>(a, s);
+  else if (a.x_trans && a.second) run_tiles<T, true, true, parts>(a, s);
+  else if (a.x_trans) run_tiles<T, true, true, false>(a, s);
+  else if (a.second) run_tiles<T, false, true, parts>(a, s);
+  else run_tiles<T, false, true, false>(a, s);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.part == nullptr) return e;
   const long threads = (long)a.m * (a.ld_part / kOut);
@@ -852,7 +882,8 @@ extern "C" bool linear_plan(LinearProduct* a, int type) {
   const Shape* shapes = type == kElemF32 ? kFull : kHalf;
   const int count = type == kElemF32 ? 2 : 3;
   const int per = type == kElemF32 ? 32 : 64;
-  const int steps = a->kx > per ? (a->kx + per - 1) / per : 1;
+  const int steps = (a->kx > per ? (a->kx + per - 1) / per : 1) *
+                    (a->second ? 2 : 1);
   double best = 0.0;
   for (int i = 0; i < count; ++i) {
     const int t = shapes[i].tile;
@@ -907,11 +938,11 @@ static hipError_t run_dz(const LinearDz& a, hipStream_t s) {
   const auto* kept = (const Kept<T>*)a.kept;
   if (kept != nullptr)
     dz_kernel<T, true><<<grid, 256, 0, s>>>((const T*)a.dy, kept, (T*)a.dz,
-                                            a.part, a.m, a.n, a.ld_dy,
-                                            a.ld_dz, rows);
+                                            a.second, a.part, a.m, a.n,
+                                            a.ld_dy, a.ld_dz, rows);
   else
     dz_kernel<T, false><<<grid, 256, 0, s>>>((const T*)a.dy, kept, (T*)a.dz,
-                                             a.part, a.m, a.n, a.ld_dy,
+                                             0, a.part, a.m, a.n, a.ld_dy,
                                              a.ld_dz, rows);
   return hipGetLastError();
 }

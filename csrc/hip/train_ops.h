@@ -62,6 +62,8 @@ struct LinearEpilogue {
 struct LinearProduct {
   const void *x, *y;
   long ldx, ldy;           // values between rows in memory
+  long second;             // bytes from x to its second part, which is added
+                           // to it (X = x + second part), or 0: it has one
   bool x_trans, y_trans;   // k is not the consecutive index
   int m, n;                // of D
   int ext_x, ext_y;        // of the operands in memory, m and n or padded
@@ -75,6 +77,8 @@ struct LinearProduct {
 struct LinearDz {
   const void *dy, *kept;   // kept: of the epilogue, null: no activation
   void* dz;                // null: sums alone
+  long second;             // values from dz to its second part, what the first
+                           // one's rounding lost, or 0: none
   float* part;             // `strips` rows of norm_part_half(n) column sums,
                            // or null
   long ld_dy;

@@ -330,12 +330,17 @@ std::vector<Tensor> linear_bwd(const Tensor& dy,
   Tensor dz = g;
   long ld_dz = ldg;
   LinearDz z{};
+  // Of a slope that is no 0 or 1, dz has more than 16 bits: the products take
+  // it as the sum of two numbers.
+  const bool parts = products && type != 0 && act > kActRelu;
   if (products && !as_is) {
-    dz = torch::empty({M, Np}, fresh);
+    dz = torch::empty({parts ? 2 * M : M, Np}, fresh);
     ld_dz = Np;
     z.dz = dz.data_ptr();
     z.ld_dz = (int)Np;
+    z.second = parts ? M * Np : 0;
   }
+  const long second = z.second * x.element_size();
   if (z.dz != nullptr || want_db) {
     z.dy = g.data_ptr();
     z.kept = act == kActNone ? nullptr : kept.data_ptr();
@@ -361,6 +366,7 @@ std::vector<Tensor> linear_bwd(const Tensor& dy,
     const Operand wo(as_matrix(w, N, K), type, stream);
     LinearProduct a{};
     a.x = dz.data_ptr();
+    a.second = second;
     a.ldx = ld_dz;
     a.kx = (int)Np;
     a.m = a.ext_x = (int)M;
@@ -377,6 +383,7 @@ std::vector<Tensor> linear_bwd(const Tensor& dy,
     const Operand xo(as_matrix(x, M, K), type, stream);
     LinearProduct a{};
     a.x = dz.data_ptr();
+    a.second = second;
     a.ldx = ld_dz;
     a.x_trans = a.y_trans = true;
     a.kx = a.ky = (int)M;

@@ -100,9 +100,9 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor,
     "gelu" (by erf) or "silu". Returns a contiguous [..., N] in x's type.
     In 16 bits act'(z) is kept for the backward to 2^-16, and where it is
     small to 2^-9 (bf16) or 2^-10 (fp16) of itself (ReLU's is exact); the
-    gradient of z is rounded to x's type once. The gradients have no gradients
-    (create_graph), and forward-mode derivatives are refused. On the GPU rows
-    may lie up to 8 MB apart.
+    gradient of z goes into the products as two numbers of x's type. The
+    gradients have no gradients (create_graph), and forward-mode derivatives
+    are refused. On the GPU rows may lie up to 8 MB apart.
     """
     act = _INDEX.get(activation)
     if act is None:

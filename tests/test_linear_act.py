@@ -549,3 +549,53 @@ def test_fp32_functions(device, act, lowest):
     terms = torch.where(z > -3, s + more.abs(), slope.abs())
     off = (dx[:, 0].double().cpu() - slope).abs()
     assert (off <= rel * terms + tiny).all(), z[off > rel * terms]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.parametrize("shape", [
+    (1, 2, 1055), (4, 2, 2095), (16, 1, 2), (48, 735, 4), (64, 64, 64),
+    (65, 130, 129), (200, 72, 257), (700, 264, 513), (5, 9, 6000),
+    (6000, 9, 5)])
+def test_gradients_take_dz_whole(device, dtype, act, shape):
+    """dz is no 16-bit number on its way into the products: dx and dW are off
+    by their own rounding, by what the derivative is kept to (2^-16) and by
+    fp32's sums, as in check(); in fp16 by 2^-25 of the second part's own
+    smallest step. (Its rounding would add 2^-9 or 2^-12 of each term, many
+    times the result's where the terms cancel.)"""
+    m, k, n = shape
+    x, w, b, _, dy = inputs(m, k, n, dtype, device, seed=sum(shape))
+    x, w = (t.requires_grad_() for t in (x, w))
+    dx, dw = torch.autograd.grad(linear_act(x, w, b, act), (x, w), dy)
+    X, W, B, D = (t.detach().double() for t in (x, w, b, dy))
+    z = X @ W.t() + B
+    _, slope = act64(z, act)
+    dz = D * slope
+    info = torch.finfo(dtype)
+    half = info.eps / 2 * (1 + 2.0 ** -6)
+    tiny = info.smallest_normal * info.eps
+    es = 1.6 * U * (k + 8) * (X.abs() @ W.t().abs() + B.abs()) + \
+        8 * U * (1 + z.abs()) + 2.0 ** -16
+    edz = D.abs() * es + (U + half ** 2) * dz.abs() + tiny / 2
+    want = dz @ W
+    compare("dx", dx, want, half * want.abs() + edz @ W.abs() +
+            2 * U * (2 * n + 8) * (dz.abs() @ W.abs()) + tiny)
+    want = dz.t() @ X
+    compare("dw", dw, want, half * want.abs() + edz.t() @ X.abs() +
+            2 * U * (2 * m + 40) * (dz.abs().t() @ X.abs()) + tiny)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_not_finite_gradients_stay_where_they_are(device, dtype):
+    x, w, b, _, dy = inputs(70, 72, 80, dtype, device)
+    dy[3, 5] = float("inf")
+    dy[9, 7] = float("nan")
+    x, w = (t.requires_grad_() for t in (x, w))
+    for act in ACTS[2:]:
+        dx, dw = torch.autograd.grad(linear_act(x, w, b, act), (x, w), dy)
+        assert dx[3].isinf().all() and dx[9].isnan().all()
+        assert dw[5].isinf().all() and dw[7].isnan().all()
+        dx[3] = dx[9] = dw[5] = dw[7] = 0
+        assert dx.isfinite().all() and dw.isfinite().all()
