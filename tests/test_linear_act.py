@@ -599,3 +599,36 @@ def test_not_finite_gradients_stay_where_they_are(device, dtype):
         assert dw[5].isinf().all() and dw[7].isnan().all()
         dx[3] = dx[9] = dw[5] = dw[7] = 0
         assert dx.isfinite().all() and dw.isfinite().all()
+
+
+@pytest.mark.gpu
+def test_second_part_past_32_bits():
+    """dz of more than 2^32 bytes lies in front of its second part. In dx and
+    in dW a derivative of 1.118 meets minus the bf16 number nearest to it,
+    and what is left is the second part."""
+    m, n, near = 140_000, 16_384, 1.1171875
+    x = torch.zeros(m, 8, dtype=torch.bfloat16, device="cuda")
+    w = torch.zeros(n, 8, dtype=torch.bfloat16, device="cuda")
+    dy = torch.zeros(m, n, dtype=torch.bfloat16, device="cuda")
+    x[:, :2] = 1.0
+    x[m - 1, 0] = 8.0                   # derivative 1 in the last row
+    w[:, 0] = 1.203125
+    w[n - 2, 0] = 8.0                   # and in the last column but one
+    w[n - 1, 7] = w[n - 2, 7] = 1.0
+    rows = torch.tensor([0, 131_072], device="cuda")
+    dy[rows, n - 1] = 1.0
+    dy[rows, n - 2] = -near
+    dy[m - 1, n - 1] = -2 * near
+    _, slope = act64(w[n - 1, 0].double(), "gelu")
+    left = float(slope) - near
+    assert 2.0 ** -11 < left < 2.0 ** -8
+    x, w = (t.requires_grad_() for t in (x, w))
+    dx, dw = torch.autograd.grad(linear_act(x, w, None, "gelu"), (x, w), dy)
+    # The derivatives of 1 are off by 8 U, the other is kept to 2^-16.
+    lim = 2.0 ** -16 + 2.0 ** -20 + 2.0 ** -8 * left
+    assert ((dx[rows, 7].double() - left).abs() <= lim).all()
+    assert abs(float(dw[n - 1, 1]) - 2 * left) <= 2 * lim
+    assert int(dx[:, 7].count_nonzero()) == 3
+    assert int(dw[:, 1].count_nonzero()) == 2
+    del dy, dx, dw
+    torch.cuda.empty_cache()
