@@ -359,8 +359,8 @@ __device__ inline void leave_middle(float& x, float state, float in,
 }
 
 // One pass at a time: 60 registers, so that eight waves of a SIMD cover each
-// other's loads. Two at a time took 92 and 143 us in place of 125 for 48
-// million values.
+// other's loads. Two at a time took 92 registers, and 143 us in place of 125
+// for 48 million values.
 template <typename T, bool kLerp, bool kRandom>
 __global__ __launch_bounds__(kThreads) void adamw8_kernel(
     Table8<kTensors8> t, Hyper h) {

@@ -57,7 +57,8 @@
 //   64-wide tiles: with many steps the L2s, which give 20 TB/s (dW of
 //     3999x1024x1024 17 us); with few the latency of loads and of the launch:
 //     100x1024x81 7.2 us, of which a launch of one step takes 5.
-//   fp32: the matrix cores, 126 to 136 TFLOP/s, as the library's.
+//   fp32: the matrix cores, busy 94% at 4096x4096x4096: 145 TFLOP/s forward and
+//     backward (the library's 8192x8192x8192 153), 104 to 119 at 3999x1024x1024.
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
