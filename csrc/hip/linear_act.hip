@@ -328,7 +328,7 @@ __device__ inline float activate(float z, float& slope) {
 // 14 bits, or 16 where it is above zero (all derivatives lie between -0.13 and
 // 1.13): the two highest bits together are the sign, the last code is NaN.
 // Magnitudes from `line` on are whole numbers of 2^-15. Those below are the
-// exponent and first kBits bits of an fp32 number times a power of two, which
+// exponent and first `bits` bits of an fp32 number times a power of two, which
 // makes the codes meet at `line` and the smallest ones subnormal. bf16 has dz's
 // exponents to go with 2^-52; in fp16 dz ends at 2^-24 and has more bits.
 template <typename T>
