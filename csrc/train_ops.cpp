@@ -408,14 +408,20 @@ bool is_capturing(hipStream_t stream, const char* what) {
 // A leaf's gradient goes through the accumulator that a live graph of it
 // holds, on the stream where that was made. In the capture of a backward this
 // would tie that stream to the captured one, which ends the process. Whether
-// it is another one than the forward's shows in the forward.
+// it is another one than the forward's shows in the forward, also behind casts
+// and views of the leaf (the head's weights are cast to its inputs' type).
 bool held_elsewhere(const Tensor& x,
                     std::initializer_list<const Tensor*> inputs) {
   const auto stream = c10::hip::getCurrentHIPStream(x.device().index());
   for (const Tensor* t : inputs) {
-    if (t == nullptr || !t->is_leaf() || !t->requires_grad()) continue;
-    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
-    const auto at = node ? node->stream() : std::nullopt;
+    if (t == nullptr || !t->requires_grad()) continue;
+    auto node = t->is_leaf()
+                    ? torch::autograd::impl::try_get_grad_accumulator(*t)
+                    : t->grad_fn();
+    for (int i = 0; i < 8 && node && node->num_outputs() == 1; ++i)
+      node = node->next_edge(0).function;
+    if (!node || node->num_outputs() != 0) continue;
+    const auto at = node->stream();
     if (at && at->id() != stream.unwrap().id()) return true;
   }
   return false;

@@ -632,3 +632,29 @@ def test_second_part_past_32_bits():
     assert int(dw[:, 1].count_nonzero()) == 2
     del dy, dx, dw
     torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
+def test_captured_backward_of_a_held_leaf_behind_a_cast():
+    """fp32 weights, cast and flattened as the box head does it."""
+    x, _, b, r, dy = inputs(40, 64, 32, torch.bfloat16, "cuda")
+    w = torch.randn(32, 16, 2, 2, device="cuda", requires_grad=True)
+
+    def layer():
+        return linear_act(x, w.reshape(32, -1).to(x.dtype), b, "relu", r)
+    held = layer()
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="free that graph"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            y = layer()
+            torch.autograd.grad(y, w, dy)
+    want, = torch.autograd.grad(held, w, dy)
+    del held, y
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = layer()
+        got, = torch.autograd.grad(y, w, dy)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
